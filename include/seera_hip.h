@@ -441,6 +441,172 @@ int seera_hip_broadcast_mul_4d(const float *A, const float *B, float *C,
                                int aN, int aC, int aH, int aW, int bN, int bC,
                                int bH, int bW);
 
+/* ---- sequence models: gated scan, block norm, AdamW (no counterpart in the
+ * reference, whose layers are Dense, Conv2D and pooling) ----
+ *
+ * Activations are fp32, fp16 or bf16 (SEERA_DTYPE_*); weights, states, saved
+ * statistics and the gradients of weights are fp32. Arithmetic, states, sums
+ * and statistics are fp32; a 16-bit output is rounded once, when it is stored.
+ * Pointers marked "optional" may be NULL. Pointers must be aligned to their
+ * type; every other alignment, row distance and size is taken (the widest
+ * loads need 16-byte aligned pointers and row distances). Outputs are
+ * overwritten. The _async forms follow the workspace rule of HIP graphs
+ * (below): one eager call of the same sizes before a capture. */
+enum {
+    SEERA_DTYPE_F32 = 0,
+    SEERA_DTYPE_F16 = 1,
+    SEERA_DTYPE_BF16 = 2,
+};
+
+/* Gated linear recurrence over time, per sequence and channel:
+ *   SEERA_GATE_LINEAR   a = f             h_t = a_t h_{t-1} + x_t
+ *   SEERA_GATE_SIGMOID  a = sigmoid(f)    h_t = a_t h_{t-1} + (1 - a_t) x_t
+ * x, f, h hold [batch, time] rows of `channels` values; row (b, t) is row
+ * b * time + t of its matrix, or t * batch + b with time_major != 0. Rows of x
+ * and f are ldx and ldf elements apart (so both may be column slices of one
+ * projection); rows of h are contiguous.
+ *   h0       [batch, channels] fp32, the state before the first step; optional (zeros)
+ *   lengths  [batch] int32 on the device, steps of each sequence; optional (all
+ *            `time`). Values below 0 count as 0, above time as time. Rows t >= length
+ *            are not read; h is 0 there
+ *   hT       [batch, channels] fp32, the state after the last step; optional. It
+ *            may be h0 itself, so that one buffer carries a generation's state
+ * time == 1 is the step of a model that generates token by token; time == 0
+ * copies h0 to hT. A gate of exactly 0 (f = -inf under SIGMOID) starts anew. */
+enum { SEERA_GATE_LINEAR = 0, SEERA_GATE_SIGMOID = 1 };
+int seera_hip_gated_scan_fwd(const void *x, const void *f, const float *h0,
+                             const int *lengths, void *h, float *hT, int batch,
+                             int time, int channels, int64_t ldx, int64_t ldf,
+                             int gate, int time_major, int dtype);
+int seera_hip_gated_scan_fwd_async(const void *x, const void *f,
+                                   const float *h0, const int *lengths, void *h,
+                                   float *hT, int batch, int time, int channels,
+                                   int64_t ldx, int64_t ldf, int gate,
+                                   int time_major, int dtype, void *stream);
+/* Its gradients. h is the forward's output, dh [batch, time] rows (contiguous)
+ * and dhT [batch, channels] fp32 (optional, zeros) the gradients of h and hT.
+ * With g_t = dh_t + a_{t+1} g_{t+1} (dhT at the last step):
+ *   LINEAR   dx = g            df = g h_{t-1}          (x is not read, may be NULL)
+ *   SIGMOID  dx = g (1 - a)    df = g (h_{t-1} - x) a (1 - a)
+ * and dh0 = a_0 g_0 (optional; it may be dhT itself). dx and df are 0 in rows
+ * t >= length. */
+int seera_hip_gated_scan_bwd(const void *x, const void *f, const float *h0,
+                             const int *lengths, const void *h, const void *dh,
+                             const float *dhT, void *dx, void *df, float *dh0,
+                             int batch, int time, int channels, int64_t ldx,
+                             int64_t ldf, int64_t lddx, int64_t lddf, int gate,
+                             int time_major, int dtype);
+int seera_hip_gated_scan_bwd_async(const void *x, const void *f,
+                                   const float *h0, const int *lengths,
+                                   const void *h, const void *dh,
+                                   const float *dhT, void *dx, void *df,
+                                   float *dh0, int batch, int time,
+                                   int channels, int64_t ldx, int64_t ldf,
+                                   int64_t lddx, int64_t lddf, int gate,
+                                   int time_major, int dtype, void *stream);
+
+/* The norms after a block and before the next one, with the block's gate, its
+ * residual scale and the residual between them, for `rows` rows of `cols`
+ * (at most 16384) values:
+ *   z = rms(y) w1          (z = y without w1)
+ *   u = z act(g) s         (without the factors that are NULL)
+ *   r_out = r + u          (r_out = u without r)
+ *   n_out = rms(r_out) w2  (only with w2; of r_out as it is stored, rounded)
+ *   rms(v) = v * rstd, rstd = 1 / sqrt(mean(v^2) + eps)
+ * g, r, w1, s, w2 are optional. So w2 alone is a plain norm, w1 with g the gated
+ * norm inside a block. y and g have rows ldy and ldg elements apart; all other
+ * matrices are contiguous. w1, s, w2: [cols] fp32. r_out is optional where
+ * n_out is written; rstd1 [rows] (with w1) and rstd2 [rows] (with w2) are
+ * optional and needed by the backward. r_out and n_out may be r, or y or g where
+ * that has contiguous rows: a row is read before it is written. */
+enum { SEERA_GATE_ACT_SILU = 0, SEERA_GATE_ACT_SIGMOID = 1 };
+int seera_hip_block_norm_fwd(const void *y, const void *g, const void *r,
+                             const float *w1, const float *s, const float *w2,
+                             void *r_out, void *n_out, float *rstd1,
+                             float *rstd2, int rows, int cols, int64_t ldy,
+                             int64_t ldg, float eps, int act, int dtype);
+int seera_hip_block_norm_fwd_async(const void *y, const void *g, const void *r,
+                                   const float *w1, const float *s,
+                                   const float *w2, void *r_out, void *n_out,
+                                   float *rstd1, float *rstd2, int rows,
+                                   int cols, int64_t ldy, int64_t ldg,
+                                   float eps, int act, int dtype, void *stream);
+/* Its gradients, from those of r_out (dr_out, optional with w2) and of n_out (dn,
+ * with w2). y, g, w1, s, w2, r_out, rstd1, rstd2 as the forward had and gave them
+ * (r_out and rstd2 with w2, rstd1 with w1; y is not read where no w1, g or s is
+ * given). Writes dy, dg (with g), dr (optional), dw1 (with w1), ds (with s), dw2
+ * (with w2); the three sums over rows are taken in a fixed order. rows == 0 gives
+ * zero weight gradients. dr may be dr_out or dn; dy and dg may be y and g where
+ * their row distances agree. */
+int seera_hip_block_norm_bwd(const void *y, const void *g, const void *r_out,
+                             const float *w1, const float *s, const float *w2,
+                             const float *rstd1, const float *rstd2,
+                             const void *dr_out, const void *dn, void *dy,
+                             void *dg, void *dr, float *dw1, float *ds,
+                             float *dw2, int rows, int cols, int64_t ldy,
+                             int64_t ldg, int64_t lddy, int64_t lddg, int act,
+                             int dtype);
+int seera_hip_block_norm_bwd_async(const void *y, const void *g,
+                                   const void *r_out, const float *w1,
+                                   const float *s, const float *w2,
+                                   const float *rstd1, const float *rstd2,
+                                   const void *dr_out, const void *dn, void *dy,
+                                   void *dg, void *dr, float *dw1, float *ds,
+                                   float *dw2, int rows, int cols, int64_t ldy,
+                                   int64_t ldg, int64_t lddy, int64_t lddg,
+                                   int act, int dtype, void *stream);
+
+/* One tensor of an AdamW step. The array of these lies in host memory and is
+ * read during the call only; the pointers in it are device pointers.
+ *   m, v     the moments: fp32 [count] with state_bits 32, codes (uint8 [count])
+ *            with state_bits 8, whose m_exp and v_exp (uint8 [ceil(count / 128)])
+ *            hold the exponent that 128 codes share. All-zero bytes are zeros
+ *   param16  a rounded copy of param written with it (optional), of param16_dtype
+ *            SEERA_DTYPE_F16 or SEERA_DTYPE_BF16
+ * 8-bit codes: with E the exponent byte, a code c of v is the fp32 number with
+ * the bits c << 20, times 2^(E - 31); of m that of the low seven bits, times
+ * 2^(E - 15), negative with the top bit. E = 255 marks a block that held an
+ * infinity or NaN: its values are NaN. Rounding is up or down with the remainder
+ * as its probability, from a hash of (seed, place in the list, index): unbiased,
+ * and the same in every run. A positive v keeps a code of at least 1. */
+typedef struct seera_adamw_tensor {
+    float *param;
+    const void *grad;
+    void *m;
+    void *v;
+    uint8_t *m_exp;
+    uint8_t *v_exp;
+    void *param16;
+    int64_t count;
+    double weight_decay;
+    int grad_dtype;
+    int param16_dtype;
+    int state_bits;
+    int reserved;
+} seera_adamw_tensor;
+/* AdamW over n tensors in place, with t = step (from 1) and
+ * g = grad * *grad_scale (a device fp32; optional, 1):
+ *   m = beta1 m + (1 - beta1) g      v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay)
+ *           - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * param takes m and v as computed, before they are rounded to 8 bits. */
+int seera_hip_adamw_step(const seera_adamw_tensor *tensors, int n, double lr,
+                         double beta1, double beta2, double eps, int64_t step,
+                         uint32_t seed, const float *grad_scale);
+int seera_hip_adamw_step_async(const seera_adamw_tensor *tensors, int n,
+                               double lr, double beta1, double beta2,
+                               double eps, int64_t step, uint32_t seed,
+                               const float *grad_scale, void *stream);
+/* The moments as fp32, into m_values[i] and v_values[i] ([count] on the device;
+ * the arrays of pointers lie in host memory, a NULL in them skips one). Of a
+ * tensor only count, m, v, m_exp, v_exp and state_bits are used. */
+int seera_hip_adamw_state_values(const seera_adamw_tensor *tensors, int n,
+                                 float *const *m_values,
+                                 float *const *v_values);
+int seera_hip_adamw_state_values_async(const seera_adamw_tensor *tensors, int n,
+                                       float *const *m_values,
+                                       float *const *v_values, void *stream);
+
 /* ---- timing (no reference counterpart; used by bench.py) ---- */
 
 /* Events on `stream`: create / record / elapsed milliseconds / destroy. */

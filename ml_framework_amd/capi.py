@@ -19,10 +19,28 @@ SEERA_ACT_NONE, SEERA_ACT_RELU = 0, 1
 SEERA_ERR_INVALID_ARGUMENT = 1
 SEERA_ERR_HIP = 2
 SEERA_ERR_OUT_OF_MEMORY = 3
+SEERA_DTYPE_F32, SEERA_DTYPE_F16, SEERA_DTYPE_BF16 = 0, 1, 2
+SEERA_GATE_LINEAR, SEERA_GATE_SIGMOID = 0, 1
+SEERA_GATE_ACT_SILU, SEERA_GATE_ACT_SIGMOID = 0, 1
 
 _vp, _i, _sz, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
 _conv14 = [_vp, _vp, _vp] + [_i] * 11
 _conv16 = [_vp] * 5 + [_i] * 11
+_i64, _d = ctypes.c_int64, ctypes.c_double
+_scan_fwd = [_vp] * 6 + [_i] * 3 + [_i64] * 2 + [_i] * 3
+_scan_bwd = [_vp] * 10 + [_i] * 3 + [_i64] * 4 + [_i] * 3
+_norm_fwd = [_vp] * 10 + [_i] * 2 + [_i64] * 2 + [_f] + [_i] * 2
+_norm_bwd = [_vp] * 16 + [_i] * 2 + [_i64] * 4 + [_i] * 2
+_adamw = [_vp, _i, _d, _d, _d, _d, _i64, ctypes.c_uint32, _vp]
+
+
+class AdamwTensor(ctypes.Structure):
+    """seera_adamw_tensor: one tensor of an AdamW step. An array of these, or any
+    host buffer of the same layout, is what seera_hip_adamw_step takes."""
+    _fields_ = [("param", _vp), ("grad", _vp), ("m", _vp), ("v", _vp), ("m_exp", _vp), ("v_exp", _vp),
+                ("param16", _vp), ("count", _i64), ("weight_decay", _d), ("grad_dtype", _i),
+                ("param16_dtype", _i), ("state_bits", _i), ("reserved", _i)]
+
 
 # name -> (argtypes, restype); mirrors include/seera_hip.h one for one.
 PROTOTYPES: dict[str, tuple[list, object]] = {
@@ -109,6 +127,19 @@ PROTOTYPES: dict[str, tuple[list, object]] = {
        for n in ("elemadd", "elemsub", "elemdiv", "elemmult")},
     "seera_hip_broadcast_add_4d": ([_vp] * 3 + [_i] * 8, _i),
     "seera_hip_broadcast_mul_4d": ([_vp] * 3 + [_i] * 8, _i),
+    # sequence models: gated scan, block norm, AdamW
+    "seera_hip_gated_scan_fwd": (_scan_fwd, _i),
+    "seera_hip_gated_scan_fwd_async": (_scan_fwd + [_vp], _i),
+    "seera_hip_gated_scan_bwd": (_scan_bwd, _i),
+    "seera_hip_gated_scan_bwd_async": (_scan_bwd + [_vp], _i),
+    "seera_hip_block_norm_fwd": (_norm_fwd, _i),
+    "seera_hip_block_norm_fwd_async": (_norm_fwd + [_vp], _i),
+    "seera_hip_block_norm_bwd": (_norm_bwd, _i),
+    "seera_hip_block_norm_bwd_async": (_norm_bwd + [_vp], _i),
+    "seera_hip_adamw_step": (_adamw, _i),
+    "seera_hip_adamw_step_async": (_adamw + [_vp], _i),
+    "seera_hip_adamw_state_values": ([_vp, _i, _vp, _vp], _i),
+    "seera_hip_adamw_state_values_async": ([_vp, _i, _vp, _vp, _vp], _i),
 }
 
 _lib = None
