@@ -51,6 +51,7 @@ int optional(const char* op, size_t bytes, std::initializer_list<const void*> pt
 int scan_shape(const ScanShape& s, std::initializer_list<int64_t> lds, bool* work) {
     const char* op = "gated_scan";
     if (s.batch < 0 || s.time < 0 || s.channels < 0) return bad(op, "dims must be >= 0");
+    if (s.time > 1 << 30) return bad(op, "time is above 2^30");  // tiles step past the end in int
     if (s.gate != SEERA_GATE_LINEAR && s.gate != SEERA_GATE_SIGMOID) return fail(SEERA_ERR_INVALID_ARGUMENT, "%s: unknown gate %d", op, s.gate);
     if (s.time_major != 0 && s.time_major != 1) return bad(op, "time_major must be 0 or 1");
     if (!dtype_bytes(s.dtype)) return fail(SEERA_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", op, s.dtype);
