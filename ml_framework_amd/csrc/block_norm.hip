@@ -1,6 +1,7 @@
 // block_norm.hip -- the norms after and before a block with its gate, residual
 // scale and residual, forward and backward (seera_hip_block_norm_fwd / _bwd).
 #include <algorithm>
+#include <type_traits>
 
 #include "io_types.h"
 #include "runtime.h"
@@ -11,10 +12,40 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float block_sum(float v, float* part) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// The sum over a wave's 64 lanes, in every lane. The lanes are added in a fixed
+// order: along rows of 16, then over the four rows.
+__device__ __forceinline__ float wave_sum(float v) {
+    auto add = [&](auto ctrl, auto rows) {
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr:1
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});  // row_shr:2
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});  // row_shr:4
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});  // row_shr:8
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// The sum over the NT threads of a row. Consecutive calls use alternating halves
+// of `part`, so one barrier each is enough.
+template <int NT>
+__device__ __forceinline__ float row_sum(float v, float* part, int half) {
+    v = wave_sum(v);
+    if (NT == 64) return v;
+    constexpr int W = NT / 64;
+    float* at = part + half * W;
+    if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
     __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += at[w];
+    return s;
+}
+
+__device__ __forceinline__ float block_sum(float v, float* part) {
+    __syncthreads();
+    v = wave_sum(v);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = 0.f;
@@ -23,46 +54,282 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     return s;
 }
 
+// 1 / (1 + e^-g) and its slope; the activation and its slope from them.
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
 __device__ __forceinline__ float act_of(int act, float g) { return act == SEERA_GATE_ACT_SILU ? g * sigmoid(g) : sigmoid(g); }
 __device__ __forceinline__ float slope_of(int act, float g) {
     const float q = sigmoid(g), d = q * (1.f - q);
-    return act == SEERA_GATE_ACT_SILU ? q + g * d : d;
+    return act == SEERA_GATE_ACT_SILU ? fmaf(g, d, q) : d;
 }
 
+// 16 bytes of a row, moved as one access at any alignment of T (the hardware
+// takes unaligned addresses). CUT: the row's last pack may be cut, and goes value
+// by value. A pack past the row's end is zeros and is not stored.
 template <class T>
-__global__ __launch_bounds__(kThreads) void norm_fwd_row(NormFwd p, NormShape s) {
-    extern __shared__ float row_r[];
-    __shared__ float part[kThreads / 64];
-    const int64_t row = blockIdx.x;
-    const T* y = (const T*)p.y + row * p.ldy;
-    const T* g = (const T*)p.g + row * p.ldg;
-    const T* r = (const T*)p.r + row * s.cols;
+struct Wide {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+template <bool CUT, class T>
+__device__ __forceinline__ void load_wide(Wide<T>& to, const T* row, int c, int cols) {
+    constexpr int N = Wide<T>::N;
+    if (!CUT) {
+        // no branch: lanes past the end load the last pack and drop it
+        uint32_t bits[4];
+        __builtin_memcpy(bits, row + min(c, cols - N), 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bits[i] = c < cols ? bits[i] : 0u;
+        __builtin_memcpy(&to, bits, 16);
+    } else if (c + N <= cols) {
+        __builtin_memcpy(&to, row + c, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) to.v[i] = c + i < cols ? row[c + i] : from_f32<T>(0.f);
+    }
+}
+template <bool CUT, class T>
+__device__ __forceinline__ void store_wide(T* row, int c, int cols, const Wide<T>& from) {
+    constexpr int N = Wide<T>::N;
+    if (c + N <= cols) {
+        __builtin_memcpy(row + c, &from, sizeof(from));
+    } else if (CUT) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c + i < cols) row[c + i] = from.v[i];
+    }
+}
+// N fp32 weights from column c on; what lies past the end is of no effect.
+template <bool CUT, int N>
+__device__ __forceinline__ void load_weights(float (&to)[N], const float* w, int c, int cols) {
+    if (!CUT) {
+        __builtin_memcpy(to, w + min(c, cols - N), sizeof(to));
+    } else if (c + N <= cols) {
+        __builtin_memcpy(to, w + c, sizeof(to));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = c + i < cols ? w[c + i] : 0.f;
+    }
+}
+
+// A row in the registers of NT threads, K wide packs each; ROWS rows a block.
+template <class T, int K, int NT, int ROWS, bool CUT>
+__global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape s) {
+    constexpr int N = Wide<T>::N;
+    __shared__ float part[2 * (NT / 64) * ROWS];
+    const int tid = threadIdx.x % NT;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT;
+    if (ROWS > 1 && row >= s.rows) return;  // whole waves: such rows take no barrier
+    const T* yr = (const T*)p.y + row * p.ldy;
+    const T* gr = (const T*)p.g + row * p.ldg;
+    const T* rr = (const T*)p.r + row * s.cols;
+    Wide<T> y[K], g[K], r[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) load_wide<CUT>(y[k], yr, (k * NT + tid) * N, s.cols);
+    if (p.g)
+#pragma unroll
+        for (int k = 0; k < K; ++k) load_wide<CUT>(g[k], gr, (k * NT + tid) * N, s.cols);
+    if (p.r)
+#pragma unroll
+        for (int k = 0; k < K; ++k) load_wide<CUT>(r[k], rr, (k * NT + tid) * N, s.cols);
     float rstd1 = 1.f;
     if (p.w1) {
         float sum = 0.f;
-        for (int c = threadIdx.x; c < s.cols; c += kThreads) sum += to_f32(y[c]) * to_f32(y[c]);
-        rstd1 = rsqrtf(block_sum(sum, part) / s.cols + p.eps);
-        if (p.rstd1 && threadIdx.x == 0) p.rstd1[row] = rstd1;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum = fmaf(to_f32(y[k].v[i]), to_f32(y[k].v[i]), sum);
+        rstd1 = rsqrtf(row_sum<NT>(sum, part, 0) / s.cols + p.eps);
+        if (p.rstd1 && tid == 0) p.rstd1[row] = rstd1;
     }
     float sum = 0.f;
-    for (int c = threadIdx.x; c < s.cols; c += kThreads) {
-        float u = to_f32(y[c]);
-        if (p.w1) u = u * rstd1 * p.w1[c];
-        if (p.g) u *= act_of(s.act, to_f32(g[c]));
-        if (p.s) u *= p.s[c];
-        if (p.r) u += to_f32(r[c]);
-        const T kept = from_f32<T>(u);
-        if (p.r_out) ((T*)p.r_out)[row * s.cols + c] = kept;
-        u = to_f32(kept);
-        row_r[c] = u;
-        sum += u * u;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * NT + tid) * N;
+        float u[N], w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = to_f32(y[k].v[i]);
+        if (p.w1) {
+            load_weights<CUT>(w, p.w1, c, s.cols);
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] = u[i] * rstd1 * w[i];
+        }
+        if (p.g)
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] *= act_of(s.act, to_f32(g[k].v[i]));
+        if (p.s) {
+            load_weights<CUT>(w, p.s, c, s.cols);
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] *= w[i];
+        }
+        if (p.r)
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] += to_f32(r[k].v[i]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            y[k].v[i] = from_f32<T>(u[i]);  // as it is kept
+            sum = fmaf(to_f32(y[k].v[i]), to_f32(y[k].v[i]), sum);
+        }
+        if (p.r_out) store_wide<CUT>((T*)p.r_out + row * s.cols, c, s.cols, y[k]);
     }
     if (!p.w2) return;
-    const float rstd2 = rsqrtf(block_sum(sum, part) / s.cols + p.eps);
-    if (p.rstd2 && threadIdx.x == 0) p.rstd2[row] = rstd2;
-    for (int c = threadIdx.x; c < s.cols; c += kThreads)
-        ((T*)p.n_out)[row * s.cols + c] = from_f32<T>(row_r[c] * rstd2 * p.w2[c]);
+    const float rstd2 = rsqrtf(row_sum<NT>(sum, part, 1) / s.cols + p.eps);
+    if (p.rstd2 && tid == 0) p.rstd2[row] = rstd2;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * NT + tid) * N;
+        float w[N];
+        load_weights<CUT>(w, p.w2, c, s.cols);
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[k].v[i] = from_f32<T>(to_f32(y[k].v[i]) * rstd2 * w[i]);
+        store_wide<CUT>((T*)p.n_out + row * s.cols, c, s.cols, y[k]);
+    }
+}
+
+// The backward of rows that lie in the registers of NT threads, K wide packs
+// each. A block takes rows `blockIdx.x + k gridDim.x`, with NEXT the next row's
+// loads in flight while the present one is computed, and keeps its sums over
+// rows of dw1, ds, dw2 in registers: partial[block][3][cols].
+template <class T, int K>
+struct NormRow {
+    Wide<T> y[K], g[K], r[K], d[K], n[K];
+    float rstd1, rstd2;
+};
+template <class T, int K, int NT, bool NEXT, bool HOLD, bool CUT>
+__global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, float* partial) {
+    constexpr int N = Wide<T>::N;
+    __shared__ float part[2 * (NT / 64)];
+    const bool inner = p.w1 || p.g || p.s;
+    float h1[K][N], hs[K][N], h2[K][N], sum1[K][N], sums[K][N], sum2[K][N];
+    auto column = [](int k) { return (int)(k * NT + threadIdx.x) * N; };
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum1[k][i] = sums[k][i] = sum2[k][i] = 0.f;
+    }
+    // the weights: held in registers, or read again for each row
+    auto weights = [&](float (&to)[K][N], const float* w) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) to[k][i] = 1.f;
+            int c = column(k);
+            if (!HOLD) asm volatile("" : "+v"(c));  // an address of this row's own: the loads stay in the loop
+            if (w) load_weights<CUT>(to[k], w, c, s.cols);
+        }
+    };
+    if (HOLD) weights(h1, p.w1), weights(hs, p.s), weights(h2, p.w2);
+    auto load = [&](NormRow<T, K>& to, int64_t row) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = column(k);
+            if (inner) load_wide<CUT>(to.y[k], (const T*)p.y + row * p.ldy, c, s.cols);
+            if (p.g) load_wide<CUT>(to.g[k], (const T*)p.g + row * p.ldg, c, s.cols);
+            if (p.w2) {
+                load_wide<CUT>(to.r[k], (const T*)p.r_out + row * s.cols, c, s.cols);
+                load_wide<CUT>(to.n[k], (const T*)p.dn + row * s.cols, c, s.cols);
+            }
+            if (p.dr_out) load_wide<CUT>(to.d[k], (const T*)p.dr_out + row * s.cols, c, s.cols);
+        }
+        to.rstd1 = p.w1 ? p.rstd1[row] : 1.f;
+        if (p.w2) to.rstd2 = p.rstd2[row];
+    };
+    const float inv = 1.f / s.cols;
+    NormRow<T, K> now, next;
+    int64_t row = blockIdx.x;
+    if (NEXT) load(now, row);
+    for (; row < s.rows; row += gridDim.x) {
+        if (!NEXT) load(now, row);
+        else if (row + gridDim.x < s.rows) load(next, row + gridDim.x);
+        float d[K][N];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[k][i] = p.dr_out ? to_f32(now.d[k].v[i]) : 0.f;
+        if (p.w2) {
+            if (!HOLD) weights(h2, p.w2);
+            float dot = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float hat = to_f32(now.r[k].v[i]) * now.rstd2, dn = to_f32(now.n[k].v[i]);
+                    sum2[k][i] = fmaf(dn, hat, sum2[k][i]);
+                    dot = fmaf(dn * h2[k][i], hat, dot);
+                }
+            dot = row_sum<NT>(dot, part, 0) * inv;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float hat = to_f32(now.r[k].v[i]) * now.rstd2;
+                    d[k][i] = fmaf(now.rstd2, to_f32(now.n[k].v[i]) * h2[k][i] - hat * dot, d[k][i]);
+                }
+        }
+        if (!HOLD) weights(h1, p.w1), weights(hs, p.s);
+        float dot = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            Wide<T> out;
+            if (p.dr) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) out.v[i] = from_f32<T>(d[k][i]);
+                store_wide<CUT>((T*)p.dr + row * s.cols, column(k), s.cols, out);
+            }
+            if (p.g) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float g = to_f32(now.g[k].v[i]), q = sigmoid(g), slope = q * (1.f - q);
+                    const float act = s.act == SEERA_GATE_ACT_SILU ? g * q : q, z = to_f32(now.y[k].v[i]) * now.rstd1 * h1[k][i];
+                    sums[k][i] = fmaf(d[k][i] * z, act, sums[k][i]);
+                    d[k][i] *= hs[k][i];
+                    out.v[i] = from_f32<T>(d[k][i] * z * (s.act == SEERA_GATE_ACT_SILU ? fmaf(g, slope, q) : slope));
+                    d[k][i] *= act;
+                }
+                store_wide<CUT>((T*)p.dg + row * p.lddg, column(k), s.cols, out);
+            } else if (p.s) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    sums[k][i] = fmaf(d[k][i], to_f32(now.y[k].v[i]) * now.rstd1 * h1[k][i], sums[k][i]);
+                    d[k][i] *= hs[k][i];
+                }
+            }
+            if (p.w1) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float hat = to_f32(now.y[k].v[i]) * now.rstd1;
+                    sum1[k][i] = fmaf(d[k][i], hat, sum1[k][i]);
+                    d[k][i] *= h1[k][i];
+                    dot = fmaf(d[k][i], hat, dot);
+                }
+            }
+        }
+        if (p.w1) {
+            dot = row_sum<NT>(dot, part, 1) * inv;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) d[k][i] = now.rstd1 * (d[k][i] - to_f32(now.y[k].v[i]) * now.rstd1 * dot);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            Wide<T> out;
+#pragma unroll
+            for (int i = 0; i < N; ++i) out.v[i] = from_f32<T>(d[k][i]);
+            store_wide<CUT>((T*)p.dy + row * p.lddy, column(k), s.cols, out);
+        }
+        if (NEXT) now = next;
+    }
+    float* to = partial + (int64_t)blockIdx.x * 3 * s.cols;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = column(k) + i;
+            if (c >= s.cols) continue;
+            if (p.w1) to[c] = sum1[k][i];
+            if (p.s) to[s.cols + c] = sums[k][i];
+            if (p.w2) to[2 * s.cols + c] = sum2[k][i];
+        }
 }
 
 // partial: [gridDim.x][3][cols] sums over the block's rows of dw1, ds, dw2.
@@ -123,34 +390,86 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_rows(NormBwd p, NormShape s
     }
 }
 
-// out[k][c] = sum over blocks, in order, of partial[block][k][c].
-__global__ __launch_bounds__(kThreads) void norm_bwd_sums(const float* partial, int blocks, int cols, float* dw1, float* ds, float* dw2) {
-    const int i = blockIdx.x * kThreads + threadIdx.x;
-    if (i >= 3 * cols) return;
-    float* out = i < cols ? dw1 : i < 2 * cols ? ds : dw2;
+// out[k][c] = sum over blocks of partial[block][k][c], in a fixed order: 16
+// interleaved chains, then their sum. 32 columns a block.
+constexpr int kSumCols = 32, kSumRows = 16;
+__global__ __launch_bounds__(kSumCols * kSumRows) void norm_bwd_sums(const float* partial, int blocks, int cols, float* dw1, float* ds, float* dw2) {
+    __shared__ float part[kSumRows][kSumCols + 1];
+    const int k = blockIdx.y, lane = threadIdx.x % kSumCols, chain = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + lane;
+    float* out = k == 0 ? dw1 : k == 1 ? ds : dw2;
     if (!out) return;
     float sum = 0.f;
-    for (int b = 0; b < blocks; ++b) sum += partial[(int64_t)b * 3 * cols + i];
-    out[i % cols] = sum;
+    if (c < cols) {
+#pragma unroll 8
+        for (int b = chain; b < blocks; b += kSumRows) sum += partial[((int64_t)b * 3 + k) * cols + c];
+    }
+    part[chain][lane] = sum;
+    __syncthreads();
+    if (chain || c >= cols) return;
+#pragma unroll
+    for (int i = 1; i < kSumRows; ++i) sum += part[i][lane];
+    out[c] = sum;
 }
 
-template <class T>
-int fwd_t(const NormShape& s, const NormFwd& a, hipStream_t st) {
-    hipLaunchKernelGGL((norm_fwd_row<T>), dim3(s.rows), dim3(kThreads), s.cols * sizeof(float), st, a, s);
+template <class T, int K, int NT, int ROWS>
+int fwd_launch(const NormShape& s, const NormFwd& a, hipStream_t st) {
+    const dim3 grid((s.rows + ROWS - 1) / ROWS), block(NT * ROWS);
+    if (s.cols % Wide<T>::N) hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, true>), grid, block, 0, st, a, s);
+    else hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, false>), grid, block, 0, st, a, s);
     SEERA_HIP_TRY(hipGetLastError());
     return SEERA_OK;
 }
 
+// A row in one wave up to 32 (16-bit) or 16 (fp32) values a lane: no barrier, and
+// many rows in flight; wider ones in 256 or 1024 threads.
+template <class T>
+int fwd_t(const NormShape& s, const NormFwd& a, hipStream_t st) {
+    constexpr int N = Wide<T>::N;
+    const int packs = (s.cols + N - 1) / N;
+    if (packs <= 64) return fwd_launch<T, 1, 64, 4>(s, a, st);
+    if (packs <= 128) return fwd_launch<T, 2, 64, 4>(s, a, st);
+    if (packs <= 256) return fwd_launch<T, 4, 64, 4>(s, a, st);
+    if (packs <= 512) return fwd_launch<T, 2, 256, 1>(s, a, st);
+    if (packs <= 1024) return fwd_launch<T, 4, 256, 1>(s, a, st);
+    if (packs <= 2048) return fwd_launch<T, 2, 1024, 1>(s, a, st);
+    if constexpr (N == 4) return fwd_launch<T, 4, 1024, 1>(s, a, st);
+    return SEERA_OK;  // 16384 columns of 16 bits are 2048 packs
+}
+
+template <class T, int K, int NT, bool NEXT, bool HOLD>
+void bwd_launch(const NormShape& s, const NormBwd& a, int blocks, float* to, hipStream_t st) {
+    if (s.cols % Wide<T>::N) hipLaunchKernelGGL((norm_bwd_regs<T, K, NT, NEXT, HOLD, true>), dim3(blocks), dim3(NT), 0, st, a, s, to);
+    else hipLaunchKernelGGL((norm_bwd_regs<T, K, NT, NEXT, HOLD, false>), dim3(blocks), dim3(NT), 0, st, a, s, to);
+}
+
+// Rows of more than 1024 packs: fp32 ones up to 8192 columns still fit.
+template <class T>
+void bwd_wide(const NormShape& s, const NormBwd& a, int blocks, float* to, hipStream_t st) {
+    if constexpr (sizeof(T) == 4)
+        if (s.cols <= 8192) return bwd_launch<T, 4, 512, false, false>(s, a, blocks, to, st);
+    hipLaunchKernelGGL((norm_bwd_rows<T>), dim3(blocks), dim3(kThreads), s.cols * sizeof(float), st, a, s, to);
+}
+
 template <class T>
 int bwd_t(const NormShape& s, const NormBwd& a, hipStream_t st) {
-    const int blocks = std::min(s.rows, 1024);
+    constexpr int N = Wide<T>::N;
+    const int packs = (s.cols + N - 1) / N;
+    const int threads = packs <= 64 ? 64 : packs <= 128 ? 128 : packs <= 256 ? 256 : 512;
+    const int blocks = (int)std::min<int64_t>(s.rows, (int64_t)device_cus() * std::max(1, 512 / threads));
     void* ws = nullptr;
     SEERA_TRY(workspace((size_t)std::max(blocks, 1) * 3 * s.cols * sizeof(float), &ws, st));
     if (blocks) {
-        hipLaunchKernelGGL((norm_bwd_rows<T>), dim3(blocks), dim3(kThreads), s.cols * sizeof(float), st, a, s, (float*)ws);
+        float* to = (float*)ws;
+        if (packs <= 64) bwd_launch<T, 1, 64, true, true>(s, a, blocks, to, st);
+        else if (packs <= 128) bwd_launch<T, 1, 128, true, true>(s, a, blocks, to, st);
+        else if (packs <= 256) bwd_launch<T, 1, 256, true, true>(s, a, blocks, to, st);
+        else if (packs <= 512) bwd_launch<T, 1, 512, true, true>(s, a, blocks, to, st);
+        else if (packs <= 1024) bwd_launch<T, 2, 512, N == 4, false>(s, a, blocks, to, st);
+        else bwd_wide<T>(s, a, blocks, to, st);
         SEERA_HIP_TRY(hipGetLastError());
     }
-    hipLaunchKernelGGL(norm_bwd_sums, dim3((3 * s.cols + kThreads - 1) / kThreads), dim3(kThreads), 0, st, (const float*)ws, blocks, s.cols,
+    if (!a.w1 && !a.s && !a.w2) return SEERA_OK;
+    hipLaunchKernelGGL(norm_bwd_sums, dim3((s.cols + kSumCols - 1) / kSumCols, 3), dim3(kSumCols * kSumRows), 0, st, (const float*)ws, blocks, s.cols,
                        a.w1 ? a.dw1 : nullptr, a.s ? a.ds : nullptr, a.w2 ? a.dw2 : nullptr);
     SEERA_HIP_TRY(hipGetLastError());
     return SEERA_OK;
