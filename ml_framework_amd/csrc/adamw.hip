@@ -39,114 +39,262 @@ __device__ __forceinline__ uint32_t encode(float a, uint32_t e, int top, uint32_
 // The exponent whose 1.875-fold reaches the block's largest value (its bits).
 __device__ __forceinline__ uint32_t shared_exponent(uint32_t largest) { return largest >= 0x7f800000u ? 255u : (largest + 0x0fffffu) >> 23; }
 
-__device__ __forceinline__ float load_grad(const void* g, int dtype, int64_t i) {
-    return dtype == SEERA_DTYPE_F32 ? ((const float*)g)[i] : dtype == SEERA_DTYPE_F16 ? to_f32(((const f16_t*)g)[i]) : to_f32(((const bf16_t*)g)[i]);
+// What a launch works on: up to kMost tensors in the kernel's arguments, so that
+// a step needs no copy to the device and may be captured in a graph. Thread block
+// b works on values [(b - first) * kChunk, ...) of the last tensor with first <= b.
+constexpr int kMost = 48, kChunk = 4096, kThreads = 256;
+struct Slot {
+    float* param;      // adamw_values: where m's values go
+    const void* grad;  // adamw_values: where v's values go
+    void *m, *v;
+    uint8_t *m_exp, *v_exp;
+    void* param16;
+    int64_t count;
+    float keep;        // 1 - lr * weight_decay
+    uint32_t key;      // of the rounding's random bits
+};
+struct Batch {
+    Slot slot[kMost];
+    unsigned first[kMost];
+    uint8_t bits[kMost], grad_dtype[kMost], copy[kMost];
+    int count;
+};
+
+// The block's slot, by one comparison in each of 48 lanes.
+__device__ __forceinline__ int slot_of(const Batch& b) {
+    const int lane = threadIdx.x & 63;
+    const bool begun = lane < b.count && b.first[min(lane, kMost - 1)] <= blockIdx.x;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(begun)) - 1);
 }
 
-// One block of 128 threads for 128 values.
-__global__ __launch_bounds__(kBlock) void adamw_block(seera_adamw_tensor t, AdamwStep s, float keep, uint32_t key) {
-    __shared__ uint32_t most[4];
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    const bool in = i < t.count;
-    const bool codes = t.state_bits == 8;
-    float m = 0.f, v = 0.f;
-    if (in) {
-        float g = load_grad(t.grad, t.grad_dtype, i);
-        if (s.grad_scale) g *= *s.grad_scale;
-        if (codes) {
-            const uint32_t cm = ((const uint8_t*)t.m)[i], cv = ((const uint8_t*)t.v)[i];
-            m = decode(cm & 127, t.m_exp[blockIdx.x], 15);
-            if (cm & 128) m = -m;
-            v = decode(cv, t.v_exp[blockIdx.x], 31);
-        } else {
-            m = ((const float*)t.m)[i];
-            v = ((const float*)t.v)[i];
-        }
-        m = m * s.beta1 + g * s.one_minus_beta1;
-        v = v * s.beta2 + (g * g) * s.one_minus_beta2;
-        float p = t.param[i];
-        p = p * keep - s.step_size * m / (sqrtf(v) * s.inv_sqrt_corr2 + s.eps);
-        t.param[i] = p;
-        if (t.param16) {
-            if (t.param16_dtype == SEERA_DTYPE_F16) ((f16_t*)t.param16)[i] = from_f32<f16_t>(p);
-            else ((bf16_t*)t.param16)[i] = from_f32<bf16_t>(p);
-        }
-        if (!codes) {
-            ((float*)t.m)[i] = m;
-            ((float*)t.v)[i] = v;
-        }
+// N consecutive values; the cut ones at the tensor's end one by one. Whole ones are
+// one access at any alignment of T.
+template <class T, int N>
+__device__ __forceinline__ void load_some(T (&to)[N], const void* from, int64_t i, int live) {
+    const T* p = (const T*)from + i;
+    if (live == N) {
+        __builtin_memcpy(to, p, sizeof(to));
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) to[k] = k < live ? p[k] : (T)0;
     }
-    if (!codes) return;
-    uint32_t am = __float_as_uint(fabsf(m)), av = __float_as_uint(v) & 0x7fffffffu;
-    for (int o = 32; o > 0; o >>= 1) {
-        am = max(am, (uint32_t)__shfl_xor((int)am, o, 64));
-        av = max(av, (uint32_t)__shfl_xor((int)av, o, 64));
+}
+template <class T, int N>
+__device__ __forceinline__ void store_some(void* to, int64_t i, const T (&from)[N], int live) {
+    T* p = (T*)to + i;
+    if (live == N) {
+        __builtin_memcpy(p, from, sizeof(from));
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < live) p[k] = from[k];
     }
-    if ((threadIdx.x & 63) == 0) {
-        most[threadIdx.x >> 6] = am;
-        most[2 + (threadIdx.x >> 6)] = av;
-    }
-    __syncthreads();
-    const uint32_t em = shared_exponent(max(most[0], most[1])), ev = shared_exponent(max(most[2], most[3]));
-    if (in) {
-        const uint32_t random = mix((uint32_t)i * 0x9E3779B9u + key);
-        ((uint8_t*)t.m)[i] = (uint8_t)(min(encode(fabsf(m), em, 15, random & 0xffffu), 127u) | (m < 0.f ? 128u : 0u));
-        uint32_t cv = min(encode(v, ev, 31, random >> 16), 255u);
-        if (v > 0.f && cv == 0) cv = 1;
-        ((uint8_t*)t.v)[i] = (uint8_t)cv;
-    }
-    if (threadIdx.x == 0) {
-        t.m_exp[blockIdx.x] = (uint8_t)em;
-        t.v_exp[blockIdx.x] = (uint8_t)ev;
+}
+template <class T, int N>
+__device__ __forceinline__ void load_as_f32(float (&to)[N], const void* from, int64_t i, int live) {
+    T raw[N];
+    load_some(raw, from, i, live);
+#pragma unroll
+    for (int k = 0; k < N; ++k) to[k] = to_f32(raw[k]);
+}
+template <int N>
+__device__ __forceinline__ void load_grads(float (&to)[N], const void* from, int dtype, int64_t i, int live) {
+    if (dtype == SEERA_DTYPE_F32) load_as_f32<float>(to, from, i, live);
+    else if (dtype == SEERA_DTYPE_F16) load_as_f32<f16_t>(to, from, i, live);
+    else load_as_f32<bf16_t>(to, from, i, live);
+}
+template <class T, int N>
+__device__ __forceinline__ void store_rounded(void* to, int64_t i, const float (&from)[N], int live) {
+    T raw[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) raw[k] = from_f32<T>(from[k]);
+    store_some(to, i, raw, live);
+}
+
+// The largest of the 16 lanes of a row, in each of them.
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+}
+
+// N values of the step: the moments and the parameter.
+template <int N>
+__device__ __forceinline__ void update(const AdamwStep& s, float keep, float scale, const float (&g)[N], float (&m)[N], float (&v)[N], float (&p)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const float gk = g[k] * scale;
+        m[k] = m[k] * s.beta1 + gk * s.one_minus_beta1;
+        v[k] = v[k] * s.beta2 + (gk * gk) * s.one_minus_beta2;
+        p[k] = p[k] * keep - s.step_size * m[k] / (sqrtf(v[k]) * s.inv_sqrt_corr2 + s.eps);
     }
 }
 
-__global__ __launch_bounds__(kBlock) void state_values(seera_adamw_tensor t, float* m_out, float* v_out) {
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (i >= t.count) return;
-    if (t.state_bits == 32) {
-        if (m_out) m_out[i] = ((const float*)t.m)[i];
-        if (v_out) v_out[i] = ((const float*)t.v)[i];
+template <int N>
+__device__ __forceinline__ void store_params(const Slot& t, int copy, int64_t i, const float (&p)[N], int live) {
+    store_some(t.param, i, p, live);
+    if (copy == SEERA_DTYPE_F16) store_rounded<f16_t>(t.param16, i, p, live);
+    else if (copy == SEERA_DTYPE_BF16) store_rounded<bf16_t>(t.param16, i, p, live);
+}
+
+__global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
+    const int at = slot_of(b);
+    const Slot t = b.slot[at];
+    const int bits = b.bits[at], dtype = b.grad_dtype[at], copy = b.copy[at];
+    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * kChunk;
+    const int64_t end = min(begin + kChunk, t.count);
+    const float scale = s.grad_scale ? *s.grad_scale : 1.f;
+    if (bits == 32) {
+        constexpr int N = 4;
+#pragma unroll 2
+        for (int64_t i = begin + threadIdx.x * N; i < end; i += kThreads * N) {
+            const int live = (int)min((int64_t)N, t.count - i);
+            float g[N], m[N], v[N], p[N];
+            load_grads(g, t.grad, dtype, i, live);
+            load_some(m, t.m, i, live);
+            load_some(v, t.v, i, live);
+            load_some(p, t.param, i, live);
+            update(s, t.keep, scale, g, m, v, p);
+            store_some(t.m, i, m, live);
+            store_some(t.v, i, v, live);
+            store_params(t, copy, i, p, live);
+        }
         return;
     }
-    if (m_out) {
-        const uint32_t c = ((const uint8_t*)t.m)[i];
-        const float a = decode(c & 127, t.m_exp[blockIdx.x], 15);
-        m_out[i] = c & 128 ? -a : a;
+    // 8 values a lane: the 16 lanes of a row hold the 128 that share an exponent
+    constexpr int N = 8;
+    for (int64_t i = begin + threadIdx.x * N; i < (end + kBlock - 1) / kBlock * kBlock; i += kThreads * N) {
+        const int live = (int)max((int64_t)0, min((int64_t)N, t.count - i));
+        const int64_t block = i / kBlock;
+        float g[N], m[N], v[N], p[N];
+        uint8_t cm[N], cv[N];
+        load_grads(g, t.grad, dtype, i, live);
+        load_some(cm, t.m, i, live);
+        load_some(cv, t.v, i, live);
+        load_some(p, t.param, i, live);
+        uint32_t em = t.m_exp[block], ev = t.v_exp[block];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            m[k] = decode(cm[k] & 127, em, 15);
+            if (cm[k] & 128) m[k] = -m[k];
+            v[k] = decode(cv[k], ev, 31);
+        }
+        update(s, t.keep, scale, g, m, v, p);
+        store_params(t, copy, i, p, live);
+        uint32_t am = 0, av = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (k < live) {
+                am = max(am, __float_as_uint(m[k]) & 0x7fffffffu);
+                av = max(av, __float_as_uint(v[k]) & 0x7fffffffu);
+            }
+        }
+        em = shared_exponent(row_max(am));
+        ev = shared_exponent(row_max(av));
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const uint32_t random = mix((uint32_t)(i + k) * 0x9E3779B9u + t.key);
+            cm[k] = (uint8_t)(min(encode(fabsf(m[k]), em, 15, random & 0xffffu), 127u) | (m[k] < 0.f ? 128u : 0u));
+            const uint32_t c = min(encode(v[k], ev, 31, random >> 16), 255u);
+            cv[k] = (uint8_t)(v[k] > 0.f ? max(c, 1u) : c);
+        }
+        store_some(t.m, i, cm, live);
+        store_some(t.v, i, cv, live);
+        if ((threadIdx.x & 15) == 0) {
+            t.m_exp[block] = (uint8_t)em;
+            t.v_exp[block] = (uint8_t)ev;
+        }
     }
-    if (v_out) v_out[i] = decode(((const uint8_t*)t.v)[i], t.v_exp[blockIdx.x], 31);
 }
 
-int blocks_of(int64_t count, unsigned* out) {
-    const int64_t blocks = (count + kBlock - 1) / kBlock;
-    if (blocks > kMaxGridX) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: a tensor is too large");
-    *out = (unsigned)blocks;
+__global__ __launch_bounds__(kThreads) void adamw_values(Batch b) {
+    const int at = slot_of(b);
+    const Slot t = b.slot[at];
+    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * kChunk;
+    const int64_t end = min(begin + kChunk, t.count);
+    float *m_out = t.param, *v_out = (float*)t.grad;
+    constexpr int N = 4;
+    for (int64_t i = begin + threadIdx.x * N; i < end; i += kThreads * N) {
+        const int live = (int)min((int64_t)N, t.count - i);
+        float x[N];
+        uint8_t c[N];
+        if (b.bits[at] == 32) {
+            if (m_out) load_some(x, t.m, i, live), store_some(m_out, i, x, live);
+            if (v_out) load_some(x, t.v, i, live), store_some(v_out, i, x, live);
+            continue;
+        }
+        if (m_out) {
+            load_some(c, t.m, i, live);
+            const uint32_t e = t.m_exp[i / kBlock];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                x[k] = decode(c[k] & 127, e, 15);
+                if (c[k] & 128) x[k] = -x[k];
+            }
+            store_some(m_out, i, x, live);
+        }
+        if (v_out) {
+            load_some(c, t.v, i, live);
+            const uint32_t e = t.v_exp[i / kBlock];
+#pragma unroll
+            for (int k = 0; k < N; ++k) x[k] = decode(c[k], e, 31);
+            store_some(v_out, i, x, live);
+        }
+    }
+}
+
+// Launches `kernel` over all tensors, kMost at a time (fewer where the grid of
+// those would pass its limit).
+template <class Fill, class Launch>
+int batches(const seera_adamw_tensor* tensors, int n, Fill&& fill, Launch&& launch) {
+    Batch b;
+    int64_t blocks = 0;
+    b.count = 0;
+    for (int i = 0; i < n; ++i) {
+        const seera_adamw_tensor& t = tensors[i];
+        if (t.count == 0) continue;
+        const int64_t more = (t.count + kChunk - 1) / kChunk;
+        if (more > kMaxGridX) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: tensor %d is too large", i);
+        if (b.count == kMost || blocks + more > kMaxGridX) {
+            launch(b, (unsigned)blocks);
+            SEERA_HIP_TRY(hipGetLastError());
+            b.count = 0;
+            blocks = 0;
+        }
+        Slot& s = b.slot[b.count];
+        s.m = t.m, s.v = t.v, s.m_exp = t.m_exp, s.v_exp = t.v_exp, s.count = t.count;
+        fill(s, t, i);
+        b.first[b.count] = (unsigned)blocks;
+        b.bits[b.count] = (uint8_t)t.state_bits;
+        b.grad_dtype[b.count] = (uint8_t)t.grad_dtype;
+        b.copy[b.count] = t.param16 ? (uint8_t)t.param16_dtype : 0;
+        ++b.count;
+        blocks += more;
+    }
+    if (b.count == 0) return SEERA_OK;
+    launch(b, (unsigned)blocks);
+    SEERA_HIP_TRY(hipGetLastError());
     return SEERA_OK;
 }
 
 }  // namespace
 
 int adamw_step(const seera_adamw_tensor* tensors, int n, const AdamwStep& step, hipStream_t st) {
-    for (int i = 0; i < n; ++i) {
-        unsigned blocks = 0;
-        SEERA_TRY(blocks_of(tensors[i].count, &blocks));
-        if (!blocks) continue;
-        hipLaunchKernelGGL(adamw_block, dim3(blocks), dim3(kBlock), 0, st, tensors[i], step, (float)(1.0 - step.lr * tensors[i].weight_decay),
-                           mix((uint32_t)i * 0x9E3779B9u + step.seed));
-        SEERA_HIP_TRY(hipGetLastError());
-    }
-    return SEERA_OK;
+    return batches(
+        tensors, n,
+        [&](Slot& s, const seera_adamw_tensor& t, int i) {
+            s.param = t.param, s.grad = t.grad, s.param16 = t.param16;
+            s.keep = (float)(1.0 - step.lr * t.weight_decay);
+            s.key = mix((uint32_t)i * 0x9E3779B9u + step.seed);
+        },
+        [&](const Batch& b, unsigned blocks) { hipLaunchKernelGGL(adamw_many, dim3(blocks), dim3(kThreads), 0, st, b, step); });
 }
 
 int adamw_state_values(const seera_adamw_tensor* tensors, int n, float* const* m_values, float* const* v_values, hipStream_t st) {
-    for (int i = 0; i < n; ++i) {
-        unsigned blocks = 0;
-        SEERA_TRY(blocks_of(tensors[i].count, &blocks));
-        if (!blocks || (!m_values[i] && !v_values[i])) continue;
-        hipLaunchKernelGGL(state_values, dim3(blocks), dim3(kBlock), 0, st, tensors[i], m_values[i], v_values[i]);
-        SEERA_HIP_TRY(hipGetLastError());
-    }
-    return SEERA_OK;
+    return batches(
+        tensors, n, [&](Slot& s, const seera_adamw_tensor&, int i) { s.param = m_values[i], s.grad = v_values[i]; },
+        [&](const Batch& b, unsigned blocks) { hipLaunchKernelGGL(adamw_values, dim3(blocks), dim3(kThreads), 0, st, b); });
 }
 
 }  // namespace seera
