@@ -8,6 +8,7 @@
 // channel). The forward reads x, f and writes h; the backward reads x, f, h,
 // dh and writes dx, df: memory bound.
 #include <algorithm>
+#include <type_traits>
 
 #include "io_types.h"
 #include "runtime.h"
@@ -16,20 +17,27 @@
 namespace seera {
 namespace {
 
-// a and 1 - a of a gate, each with its own small relative error: sigmoid is
-// taken from e^-|f|, so that neither side cancels.
+// A gate's small side: min(a, 1 - a) of a sigmoid, from e^-|f|, so that neither
+// side cancels; the other one is 1 minus it, rounded without a bias.
+__device__ __forceinline__ float small_side(float f) {
+    const float e = __expf(-fabsf(f));
+    return e * __builtin_amdgcn_rcpf(1.f + e);
+}
+// a and 1 - a from f and the small side (LINEAR: a = f and a factor of 1).
 template <int GATE>
-__device__ __forceinline__ void gates(float f, float& a, float& rest) {
+__device__ __forceinline__ void sides(float f, float small, float& a, float& rest) {
     if (GATE == SEERA_GATE_LINEAR) {
         a = f;
         rest = 1.f;
     } else {
-        const float e = __expf(-fabsf(f));
-        const float s = e * __builtin_amdgcn_rcpf(1.f + e);  // the smaller of the two
-        const float l = 1.f - s;                             // near 1: rounded without a bias
-        a = f >= 0.f ? l : s;
-        rest = f >= 0.f ? s : l;
+        const float large = 1.f - small;
+        a = f >= 0.f ? large : small;
+        rest = f >= 0.f ? small : large;
     }
+}
+template <int GATE>
+__device__ __forceinline__ void gates(float f, float& a, float& rest) {
+    sides<GATE>(f, GATE == SEERA_GATE_LINEAR ? 0.f : small_side(f), a, rest);
 }
 
 __device__ __forceinline__ int steps_of(const int* lengths, int b, int time) {
@@ -119,22 +127,21 @@ __global__ __launch_bounds__(256) void scan_bwd_steps(ScanBwd p, ScanShape s, in
 
 // ---- tiles: long sequences ----
 //
-// A block of kTile threads owns CL * V channels of one sequence and walks its
-// time segment in tiles. Each thread holds L consecutive steps of V channels in
+// A block of NT threads owns CL * V channels of one sequence and walks its time
+// segment in tiles. Each thread holds L consecutive steps of V channels in
 // registers and composes them to one affine map; the maps are composed over a
 // wave's slots (shuffles), then over the waves (shared memory), always in the
 // order of time, so a result does not depend on timing. With its carry each
 // thread then runs its steps again from registers: x, f (dh, h) are read once.
 // The next tile's loads are issued before the present one is computed.
 //
-// DIR 0 runs forward (maps a, b), 1 backward in time (maps a, a dh).
-
-constexpr int kTile = 512, kWaves = kTile / 64;
+// DIR 0 runs forward (maps a, b), 1 backward in time (maps a, a dh). A step's
+// place in the walk is u, from 0 at the segment's first step of the walk.
 
 struct Segments {
     int count, steps;       // of the time axis; steps is a multiple of the tile
     float2* maps;           // [count][batch * channels]: a segment's composed map
-    const float* carry;     // [count][batch * channels]: the state before a segment; null: h0 / dhT
+    float* start;           // [batch * channels]: h0 or dhT, kept apart from hT or dh0, which may be the same memory
 };
 
 struct ScanPtrs {
@@ -151,18 +158,21 @@ struct Steps {
     Pack<T, V> v[L];
 };
 
-template <class T, int V, int CL, int L, int GATE, int DIR, bool MAPS>
-__global__ __launch_bounds__(kTile) void scan_tiles(ScanPtrs p, ScanShape s, Segments seg, int groups, int64_t blocks) {
-    constexpr int SL = 64 / CL, kSlots = kWaves * SL, kSteps = kSlots * L;
+template <class T, int V, int CL, int NT, int L, int GATE, int DIR, bool MAPS>
+__global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segments seg, unsigned groups, unsigned blocks) {
+    constexpr int W = NT / 64, SL = 64 / CL, kSteps = W * SL * L;
     typedef Pack<T, V> P;
-    __shared__ float2 totals[2][kWaves][CL][V];
-    // neighbouring channel groups on one die: they share lines where rows are not aligned to them
-    const int64_t chunk = (blocks + 7) / 8, id = (int64_t)(blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
-    if (id >= blocks) return;
-    const int group = (int)(id % groups), b = (int)(id / groups % s.batch), part = (int)(id / groups / s.batch);
+    typedef Steps<T, V, L> S;
+    __shared__ float2 totals[2][W][CL][V];
+    // neighbouring channel groups on one die: they share lines of memory
+    const unsigned chunk = (blocks + 7) / 8, id = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= chunk || id >= blocks) return;
+    const unsigned rest_id = id / groups, group = id - rest_id * groups, order = rest_id / (unsigned)s.batch, b = rest_id - order * (unsigned)s.batch;
+    // `part` of the walk; the second launch begins with the parts that the first one read last, which are in the cache
+    const unsigned part = MAPS || seg.count == 1 ? order : seg.count - 1 - order;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, cl = lane % CL, slot = lane / CL;
-    const int segment = DIR == 0 ? part : seg.count - 1 - part;
-    const int begin = segment * seg.steps, end = min(begin + seg.steps, s.time);
+    const int segment = DIR == 0 ? (int)part : seg.count - 1 - (int)part;
+    const int begin = segment * seg.steps, end = min(begin + seg.steps, s.time), length = end - begin;
     const int n = steps_of(p.lengths, b, s.time);
     const int channel = (group * CL + cl) * V;
     const bool active = channel < s.channels;
@@ -171,59 +181,64 @@ __global__ __launch_bounds__(kTile) void scan_tiles(ScanPtrs p, ScanShape s, Seg
     const int64_t state = (int64_t)b * s.channels + c, states = (int64_t)s.batch * s.channels;
     const int first = (wave * SL + slot) * L;  // of the thread's steps in a tile
 
-    // step u of the walk is time t(u); beyond the segment's end it repeats the last
-    auto time_of = [&](int u) { return DIR == 0 ? min(begin + u, end - 1) : max(end - 1 - u, begin); };
-    auto load = [&](const void* base, int64_t ld, int u0, int shift, Steps<T, V, L>& to) {
+    // Addresses: the row of a tile's step i is uniform but for the thread's first
+    // step, whose distance is 32 bits (launch_tiles sees to it). In a tile that is
+    // not whole, steps past the segment's end repeat its last, or are not loaded where
+    // a thread has none before it.
+    const int64_t dir = DIR == 0 ? 1 : -1;
+    auto low_row = [&](int u0) { return row0 + (int64_t)(DIR == 0 ? begin + u0 : end - u0 - kSteps) * step; };
+    const unsigned from_low = DIR == 0 ? first : kSteps - 1 - first;
+    auto load = [&](const void* base, int64_t ld, int u0, int shift, auto whole, S& to) {
+        const int64_t stride = dir * step * ld * (int64_t)sizeof(T);
+        if (decltype(whole)::value) {
+            const char* q = (const char*)base + (low_row(u0) - shift * step) * ld * (int64_t)sizeof(T);
+            const unsigned mine = from_low * (unsigned)(step * ld * (int64_t)sizeof(T)) + c * (unsigned)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int64_t row = row0 + max(time_of(u0 + first + i) - shift, 0) * step;
-            to.v[i] = *(const P*)((const T*)base + row * ld + c);
+            for (int i = 0; i < L; ++i, q += stride) to.v[i] = *(const P*)(q + mine);
+        } else {
+#pragma unroll
+            for (int i = 0; i < L; ++i) to.v[i] = P{};
+            if (u0 + first >= length) return;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int u = min(u0 + first + i, length - 1), t = max((DIR == 0 ? begin + u : end - 1 - u) - shift, 0);
+                to.v[i] = *(const P*)((const char*)base + ((row0 + t * step) * ld + c) * (int64_t)sizeof(T));
+            }
         }
+    };
+    constexpr bool kNeedX = DIR == 0 || (!MAPS && GATE == SEERA_GATE_SIGMOID), kNeedH = DIR == 1 && !MAPS;
+    auto load_all = [&](int u0, auto whole, S& x, S& f, S& d, S& h) {
+        load(p.f, p.ldf, u0, 0, whole, f);
+        if (kNeedX) load(p.x, p.ldx, u0, 0, whole, x);
+        if (DIR == 1) load(p.dh, s.channels, u0, 0, whole, d);
+        if (kNeedH) load(p.h, s.channels, u0, 1, whole, h);
+    };
+    // inside the segment, the sequence, and (for h one step before) past its first step
+    auto is_whole = [&](int u0) {
+        if (u0 + kSteps > length) return false;
+        return DIR == 0 ? begin + u0 + kSteps <= n : end - u0 <= n && end - u0 - kSteps > 0;
+    };
+    auto load_tile = [&](int u0, S& x, S& f, S& d, S& h) {
+        if (is_whole(u0)) load_all(u0, std::true_type{}, x, f, d, h);
+        else load_all(u0, std::false_type{}, x, f, d, h);
     };
 
     float carry[V], h0[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        carry[v] = MAPS ? 0.f : seg.carry ? seg.carry[segment * states + state + v] : p.init ? p.init[state + v] : 0.f;
-        h0[v] = DIR == 1 && !MAPS && p.h0 ? p.h0[state + v] : 0.f;
+        const float* init = MAPS || seg.count == 1 ? p.init : seg.start;
+        carry[v] = init ? init[state + v] : 0.f;
+        h0[v] = kNeedH && p.h0 ? p.h0[state + v] : 0.f;
+        if (MAPS && part == 0 && active && wave == 0 && slot == 0) seg.start[state + v] = carry[v];
+        if (MAPS) carry[v] = 0.f;
     }
-    float whole[V];  // MAPS: the product of the segment's a
+    float product[V];  // MAPS: of the segment's a
 #pragma unroll
-    for (int v = 0; v < V; ++v) whole[v] = 1.f;
+    for (int v = 0; v < V; ++v) product[v] = 1.f;
 
-    constexpr bool kNeedX = DIR == 0 || (!MAPS && GATE == SEERA_GATE_SIGMOID), kNeedH = DIR == 1 && !MAPS;
-    Steps<T, V, L> rx, rf, rd, rh, nx, nf, nd, nh;
-    auto load_all = [&](int u0, Steps<T, V, L>& x, Steps<T, V, L>& f, Steps<T, V, L>& d, Steps<T, V, L>& h) {
-        load(p.f, p.ldf, u0, 0, f);
-        if (kNeedX) load(p.x, p.ldx, u0, 0, x);
-        if (DIR == 1) load(p.dh, s.channels, u0, 0, d);
-        if (kNeedH) load(p.h, s.channels, u0, 1, h);
-    };
-    const int length = end - begin;
-    load_all(0, rx, rf, rd, rh);
     int parity = 0;
-    for (int u0 = 0; u0 < length; u0 += kSteps, parity ^= 1) {
-        if (u0 + kSteps < length) load_all(u0 + kSteps, nx, nf, nd, nh);
-        float a[L][V], m[L][V];  // m: b, or dh
-        float A[V], B[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int u = u0 + first + i;
-            const bool live = u < length && (DIR == 0 ? begin + u : end - 1 - u) < n;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float rest;
-                gates<GATE>(to_f32(rf.v[i].v[v]), a[i][v], rest);
-                m[i][v] = DIR == 0 ? rest * to_f32(rx.v[i].v[v]) : to_f32(rd.v[i].v[v]);
-                a[i][v] = live ? a[i][v] : 1.f;
-                m[i][v] = live ? m[i][v] : 0.f;
-                B[v] = DIR == 0 ? fmaf(a[i][v], B[v], m[i][v]) : a[i][v] * (m[i][v] + B[v]);
-                A[v] *= a[i][v];
-            }
-        }
-        // the composition of this slot and the wave's slots before it
+    // From the maps of all slots: z, the state before this one; `carry` moves behind the last.
+    auto compose = [&](float (&A)[V], float (&B)[V], float (&z)[V]) {
 #pragma unroll
         for (int d = 1; d < SL; d *= 2) {
 #pragma unroll
@@ -239,100 +254,144 @@ __global__ __launch_bounds__(kTile) void scan_tiles(ScanPtrs p, ScanShape s, Seg
 #pragma unroll
             for (int v = 0; v < V; ++v) totals[parity][wave][cl][v] = make_float2(A[v], B[v]);
         __syncthreads();
-        float mine[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) mine[v] = carry[v];
+        for (int v = 0; v < V; ++v) z[v] = carry[v];
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w)
+        for (int w = 0; w < W; ++w)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float2 t = totals[parity][w][cl][v];
                 carry[v] = fmaf(t.x, carry[v], t.y);
-                if (MAPS) whole[v] *= t.x;
-                if (w + 1 == wave) mine[v] = carry[v];
+                if (MAPS) product[v] *= t.x;
+                if (!MAPS && w + 1 == wave) z[v] = carry[v];
             }
-        if (!MAPS) {
-            float z[V];
+        parity ^= 1;
+        if (SL > 1 && !MAPS)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                z[v] = mine[v];
-                if (SL > 1) {
-                    const float pa = __shfl_up(A[v], CL, 64), pb = __shfl_up(B[v], CL, 64);
-                    if (slot > 0) z[v] = fmaf(pa, mine[v], pb);
-                }
+                const float pa = __shfl_up(A[v], CL, 64), pb = __shfl_up(B[v], CL, 64);
+                if (slot > 0) z[v] = fmaf(pa, z[v], pb);
             }
+    };
+    S rx, rf, rd, rh, nx, nf, nd, nh;
+    auto compute = [&](int u0, auto whole_tile) {
+        constexpr bool kWhole = decltype(whole_tile)::value;
+        // kept for the second run: a and b; backward the gates' small sides (f and dh
+        // are in registers as they came)
+        float a[DIR == 0 ? L : 1][V], m[L][V];
+        float A[V], B[V];
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const int u = u0 + first + i, t = time_of(u);
-                const bool live = t < n;
-                P o, o2;
+        for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int u = u0 + first + i;
+            if (!kWhole && !(u < length && (DIR == 0 ? begin + u : end - 1 - u) < n)) {
+                // a step outside: a = 1, nothing added
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    if (DIR == 0) {
-                        z[v] = fmaf(a[i][v], z[v], m[i][v]);
-                        o.v[v] = from_f32<T>(live ? z[v] : 0.f);
-                    } else {
-                        const float g = m[i][v] + z[v];
-                        z[v] = a[i][v] * g;
-                        const float before = t > 0 ? to_f32(rh.v[i].v[v]) : h0[v];
-                        float one = g, two = g * before;
-                        if (GATE == SEERA_GATE_SIGMOID) {
-                            // 1 - a again, from f: the difference would cancel for a near 1
-                            float again, rest;
-                            gates<GATE>(to_f32(rf.v[i].v[v]), again, rest);
-                            one = g * rest;
-                            two = one * (before - to_f32(rx.v[i].v[v])) * a[i][v];
-                        }
-                        o.v[v] = from_f32<T>(live ? one : 0.f);
-                        o2.v[v] = from_f32<T>(live ? two : 0.f);
-                    }
-                }
-                if (active && u < length) {
-                    const int64_t row = row0 + t * step;
-                    *(P*)((T*)p.out + row * p.ldo + c) = o;
-                    if (DIR == 1) *(P*)((T*)p.out2 + row * p.ldo2 + c) = o2;
+                    rf.v[i].v[v] = from_f32<T>(GATE == SEERA_GATE_LINEAR ? 1.f : __builtin_inff());
+                    (DIR == 0 ? rx : rd).v[i].v[v] = from_f32<T>(0.f);
                 }
             }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float f = to_f32(rf.v[i].v[v]), small = GATE == SEERA_GATE_LINEAR ? 0.f : small_side(f);
+                float ai, rest;
+                sides<GATE>(f, small, ai, rest);
+                if (DIR == 0) {
+                    a[i][v] = ai;
+                    m[i][v] = rest * to_f32(rx.v[i].v[v]);
+                    B[v] = fmaf(ai, B[v], m[i][v]);
+                } else {
+                    m[i][v] = small;
+                    B[v] = ai * (to_f32(rd.v[i].v[v]) + B[v]);
+                }
+                A[v] *= ai;
+            }
         }
+        float z[V];
+        compose(A, B, z);
+        if (MAPS) return;
+        auto run = [&](int i, P& o, P& o2) {
+            const int u = u0 + first + i, t = DIR == 0 ? begin + u : end - 1 - u;
+            const bool live = kWhole || t < n;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (DIR == 0) {
+                    z[v] = fmaf(a[i][v], z[v], m[i][v]);
+                    o.v[v] = from_f32<T>(live ? z[v] : 0.f);
+                } else {
+                    float ai, rest;
+                    sides<GATE>(to_f32(rf.v[i].v[v]), m[i][v], ai, rest);
+                    const float g = to_f32(rd.v[i].v[v]) + z[v];
+                    z[v] = ai * g;
+                    const float before = kWhole || t > 0 ? to_f32(rh.v[i].v[v]) : h0[v];
+                    const float one = g * rest;
+                    const float two = GATE == SEERA_GATE_SIGMOID ? one * (before - to_f32(rx.v[i].v[v])) * ai : g * before;
+                    o.v[v] = from_f32<T>(live ? one : 0.f);
+                    o2.v[v] = from_f32<T>(live ? two : 0.f);
+                }
+            }
+        };
+        const int64_t stride = dir * step * p.ldo * (int64_t)sizeof(T), stride2 = dir * step * p.ldo2 * (int64_t)sizeof(T);
+        char* q = (char*)p.out + low_row(u0) * p.ldo * (int64_t)sizeof(T);
+        char* q2 = (char*)p.out2 + low_row(u0) * p.ldo2 * (int64_t)sizeof(T);
+        const unsigned mine = from_low * (unsigned)(step * p.ldo * (int64_t)sizeof(T)) + c * (unsigned)sizeof(T);
+        const unsigned mine2 = from_low * (unsigned)(step * p.ldo2 * (int64_t)sizeof(T)) + c * (unsigned)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < L; ++i, q += stride, q2 += stride2) {
+            P o, o2;
+            run(i, o, o2);
+            if (active && (kWhole || u0 + first + i < length)) {
+                *(P*)(q + mine) = o;
+                if (DIR == 1) *(P*)(q2 + mine2) = o2;
+            }
+        }
+    };
+    load_tile(0, rx, rf, rd, rh);
+    if (!MAPS && part > 0) {
+        // the segments before this one: each slot composes its share of their maps
+        constexpr int kSlots = W * SL;
+        const int per = ((int)part + kSlots - 1) / kSlots, from = (wave * SL + slot) * per;
+        float A[V], B[V], z[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
+        for (int k = from; k < min(from + per, (int)part); ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float2 m = seg.maps[(DIR == 0 ? k : seg.count - 1 - k) * states + state + v];
+                B[v] = fmaf(m.x, B[v], m.y);
+                A[v] *= m.x;
+            }
+        compose(A, B, z);
+    }
+    for (int u0 = 0; u0 < length; u0 += kSteps) {
+        if (u0 + kSteps < length) load_tile(u0 + kSteps, nx, nf, nd, nh);
+        if (is_whole(u0)) compute(u0, std::true_type{});
+        else compute(u0, std::false_type{});
         rx = nx, rf = nf, rd = nd, rh = nh;
     }
     if (!active || wave || slot) return;
     if (MAPS) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) seg.maps[segment * states + state + v] = make_float2(whole[v], carry[v]);
-    } else if (part == seg.count - 1 && p.last) {
+        for (int v = 0; v < V; ++v) seg.maps[segment * states + state + v] = make_float2(product[v], carry[v]);
+    } else if ((int)part == seg.count - 1 && p.last) {
 #pragma unroll
         for (int v = 0; v < V; ++v) p.last[state + v] = carry[v];
     }
 }
 
-// The state before each segment, from the segments' maps in the order of the walk.
-__global__ __launch_bounds__(256) void scan_carries(const float2* maps, const float* init, float* carry, int64_t states, int count, int reverse) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= states) return;
-    float c = init ? init[i] : 0.f;
-#pragma unroll 8
-    for (int k = 0; k < count; ++k) {
-        const int64_t at = (reverse ? count - 1 - k : k) * states + i;
-        carry[at] = c;
-        if (k + 1 < count) {
-            const float2 m = maps[at];
-            c = fmaf(m.x, c, m.y);
-        }
-    }
-}
-
-template <class T, int V, int CL, int L, int GATE, int DIR>
-int launch_tiles(const ScanShape& s, const ScanPtrs& p, hipStream_t st) {
-    constexpr int kSteps = kWaves * (64 / CL) * L;
-    const int groups = (s.channels + CL * V - 1) / (CL * V);
+// Launches the tiles; parts > 1 splits time (where it is long enough) for a second
+// pass over x, f (f, dh), in exchange for that many times the blocks.
+template <class T, int V, int CL, int NT, int L, int GATE, int DIR>
+int launch_tiles(const ScanShape& s, const ScanPtrs& p, int64_t parts, hipStream_t st) {
+    constexpr int kSteps = NT / CL * L;
+    const unsigned groups = (s.channels + CL * V - 1) / (CL * V);
     const int64_t chains = (int64_t)groups * s.batch, states = (int64_t)s.batch * s.channels;
-    Segments seg{1, s.time, nullptr, nullptr};
     const int tiles = (s.time + kSteps - 1) / kSteps;
-    // few chains: split time, so that every compute unit has a block
-    const int64_t want = (2 * device_cus() + chains - 1) / chains;
-    if (chains < device_cus() / 2 && tiles > 2) {
-        const int per = (int)std::max<int64_t>(2, (tiles + want - 1) / want);
+    Segments seg{1, s.time, nullptr, nullptr};
+    if (parts > 1 && tiles > 1) {
+        const int per = (int)std::max<int64_t>(1, (tiles + parts - 1) / parts);
         seg.count = (tiles + per - 1) / per;
         seg.steps = per * kSteps;
     }
@@ -342,23 +401,37 @@ int launch_tiles(const ScanShape& s, const ScanPtrs& p, hipStream_t st) {
     if (seg.count > 1) {
         void* ws = nullptr;
         const size_t n = (size_t)seg.count * states;
-        SEERA_TRY(workspace(n * (sizeof(float2) + sizeof(float)), &ws, st));
+        SEERA_TRY(workspace(n * sizeof(float2) + states * sizeof(float), &ws, st));
         seg.maps = (float2*)ws;
-        float* carry = (float*)(seg.maps + n);
-        hipLaunchKernelGGL((scan_tiles<T, V, CL, L, GATE, DIR, true>), grid(blocks - chains), dim3(kTile), 0, st, p, s, seg, groups, blocks - chains);
+        seg.start = (float*)(seg.maps + n);
+        hipLaunchKernelGGL((scan_tiles<T, V, CL, NT, L, GATE, DIR, true>), grid(blocks - chains), dim3(NT), 0, st, p, s, seg, groups, (unsigned)(blocks - chains));
         SEERA_HIP_TRY(hipGetLastError());
-        hipLaunchKernelGGL(scan_carries, dim3((unsigned)((states + 255) / 256)), dim3(256), 0, st, seg.maps, p.init, carry, states, seg.count, DIR);
-        SEERA_HIP_TRY(hipGetLastError());
-        seg.carry = carry;
     }
-    hipLaunchKernelGGL((scan_tiles<T, V, CL, L, GATE, DIR, false>), grid(blocks), dim3(kTile), 0, st, p, s, seg, groups, blocks);
+    hipLaunchKernelGGL((scan_tiles<T, V, CL, NT, L, GATE, DIR, false>), grid(blocks), dim3(NT), 0, st, p, s, seg, groups, (unsigned)blocks);
     SEERA_HIP_TRY(hipGetLastError());
     return SEERA_OK;
 }
 
+// V: values that may be moved as one in a narrow tile (4 bytes, or one value where
+// nothing is aligned to that), WV: in a wide one.
+template <class T, int V, int WV, int GATE, int DIR>
+int choose_tiles(const ScanShape& s, const ScanPtrs& p, hipStream_t st) {
+    constexpr int E = (int)sizeof(T);
+    constexpr int kFull = 128 / (V * E), kHalf = std::min(64, 64 / (V * E));  // lanes over 128 and 64 bytes of channels
+    constexpr int kValues = DIR == 0 ? 16 : 8;                                // a thread's, of x, f (and dh, h)
+    const int64_t cus = device_cus();
+    auto chains = [&](int bytes) { return (int64_t)s.batch * ((s.channels * (int64_t)E + bytes - 1) / bytes); };
+    if (s.time <= 32) return launch_tiles<T, V, kFull, 128, 8 / V, GATE, DIR>(s, p, 1, st);
+    if (s.time <= 128) return launch_tiles<T, V, kFull, 256, 8 / V, GATE, DIR>(s, p, 1, st);
+    if (chains(128) >= 2 * cus) return launch_tiles<T, V, kFull, 512, kValues / V, GATE, DIR>(s, p, 1, st);
+    if (chains(64) * 4 >= cus * (DIR == 0 ? 2 : 3)) return launch_tiles<T, V, kHalf, 512, kValues / V, GATE, DIR>(s, p, 1, st);
+    const int64_t wide = chains(64 * WV * E);
+    return launch_tiles<T, WV, 64, 512, 16 / WV, GATE, DIR>(s, p, (2 * cus + wide - 1) / wide, st);
+}
+
 // Whether V values of T may be moved as one: sizes, row distances and addresses.
 template <class T, int V>
-bool packs(const ScanShape& s, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
+bool packs(const ScanShape& s, const std::initializer_list<const void*>& ptrs, const std::initializer_list<int64_t>& lds) {
     if (s.channels % V) return false;
     for (int64_t ld : lds)
         if (ld % V) return false;
@@ -368,11 +441,18 @@ bool packs(const ScanShape& s, std::initializer_list<const void*> ptrs, std::ini
 }
 
 // Up to this many steps a chain is walked by one thread, without tiles.
-constexpr int kFewSteps = 16;
+constexpr int kFewSteps = 8;
 
-template <class T, int V, int GATE>
+// Whether a tile's rows may lie 2^32 bytes apart, which its 32-bit distances do not
+// reach: such a call walks each chain in one thread too. (512: steps of the longest tile.)
+template <class T>
+bool far_apart(const ScanShape& s, const std::initializer_list<int64_t>& lds) {
+    return 512.0 * (s.time_major ? s.batch : 1) * sizeof(T) * (double)std::max(std::max(lds), (int64_t)s.channels) >= 0x1p32;
+}
+
+template <class T, int V, int WV, int GATE>
 int fwd_v(const ScanShape& s, const ScanFwd& a, hipStream_t st) {
-    if (s.time <= kFewSteps) {
+    if (s.time <= kFewSteps || far_apart<T>(s, {a.ldx, a.ldf})) {
         const int64_t items = (int64_t)s.batch * (s.channels / V), blocks = (items + 255) / 256;
         if (blocks > kMaxGridX) return fail(SEERA_ERR_INVALID_ARGUMENT, "gated_scan: batch * channels is too large");
         hipLaunchKernelGGL((scan_fwd_steps<T, V, GATE>), dim3((unsigned)blocks), dim3(256), 0, st, a, s, items);
@@ -380,12 +460,12 @@ int fwd_v(const ScanShape& s, const ScanFwd& a, hipStream_t st) {
         return SEERA_OK;
     }
     const ScanPtrs p{a.x, a.f, nullptr, nullptr, a.h, nullptr, nullptr, a.h0, a.hT, a.lengths, a.ldx, a.ldf, s.channels, 0};
-    return launch_tiles<T, V, 128 / (V * (int)sizeof(T)), 16, GATE, 0>(s, p, st);
+    return choose_tiles<T, V, WV, GATE, 0>(s, p, st);
 }
 
-template <class T, int V, int GATE>
+template <class T, int V, int WV, int GATE>
 int bwd_v(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
-    if (s.time <= kFewSteps) {
+    if (s.time <= kFewSteps || far_apart<T>(s, {a.ldx, a.ldf, a.lddx, a.lddf})) {
         const int64_t items = (int64_t)s.batch * (s.channels / V), blocks = (items + 255) / 256;
         if (blocks > kMaxGridX) return fail(SEERA_ERR_INVALID_ARGUMENT, "gated_scan: batch * channels is too large");
         hipLaunchKernelGGL((scan_bwd_steps<T, V, GATE>), dim3((unsigned)blocks), dim3(256), 0, st, a, s, items);
@@ -393,32 +473,44 @@ int bwd_v(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
         return SEERA_OK;
     }
     const ScanPtrs p{a.x, a.f, a.h, a.dh, a.dx, a.df, a.h0, a.dhT, a.dh0, a.lengths, a.ldx, a.ldf, a.lddx, a.lddf};
-    return launch_tiles<T, V, 128 / (V * (int)sizeof(T)), 8, GATE, 1>(s, p, st);
+    return choose_tiles<T, V, WV, GATE, 1>(s, p, st);
 }
 
-// Two 16-bit values a lane where everything is aligned to pairs, one otherwise.
-template <class T>
+// The widest of 8 and 4 bytes a lane that everything is aligned to, or one value.
+template <class T, int GATE>
 int fwd_t(const ScanShape& s, const ScanFwd& a, hipStream_t st) {
-    const bool linear = s.gate == SEERA_GATE_LINEAR;
-    if (sizeof(T) == 2 && packs<T, 2>(s, {a.x, a.f, a.h}, {a.ldx, a.ldf}))
-        return linear ? fwd_v<T, sizeof(T) == 2 ? 2 : 1, SEERA_GATE_LINEAR>(s, a, st) : fwd_v<T, sizeof(T) == 2 ? 2 : 1, SEERA_GATE_SIGMOID>(s, a, st);
-    return linear ? fwd_v<T, 1, SEERA_GATE_LINEAR>(s, a, st) : fwd_v<T, 1, SEERA_GATE_SIGMOID>(s, a, st);
+    constexpr int E = (int)sizeof(T);
+    const auto ptrs = {a.x, a.f, (const void*)a.h};
+    const auto lds = {a.ldx, a.ldf};
+    if (packs<T, 8 / E>(s, ptrs, lds)) return fwd_v<T, 4 / E, 8 / E, GATE>(s, a, st);
+    if (E == 2 && packs<T, 4 / E>(s, ptrs, lds)) return fwd_v<T, 4 / E, 4 / E, GATE>(s, a, st);
+    return fwd_v<T, 1, 1, GATE>(s, a, st);
+}
+template <class T, int GATE>
+int bwd_t(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
+    constexpr int E = (int)sizeof(T);
+    const auto ptrs = {GATE == SEERA_GATE_LINEAR ? a.f : a.x, a.f, a.h, a.dh, (const void*)a.dx, (const void*)a.df};
+    const auto lds = {GATE == SEERA_GATE_LINEAR ? a.ldf : a.ldx, a.ldf, a.lddx, a.lddf};
+    if (packs<T, 8 / E>(s, ptrs, lds)) return bwd_v<T, 4 / E, 8 / E, GATE>(s, a, st);
+    if (E == 2 && packs<T, 4 / E>(s, ptrs, lds)) return bwd_v<T, 4 / E, 4 / E, GATE>(s, a, st);
+    return bwd_v<T, 1, 1, GATE>(s, a, st);
 }
 template <class T>
-int bwd_t(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
-    const bool linear = s.gate == SEERA_GATE_LINEAR;
-    if (sizeof(T) == 2 && packs<T, 2>(s, {linear ? a.f : a.x, a.f, a.h, a.dh, a.dx, a.df}, {linear ? a.ldf : a.ldx, a.ldf, a.lddx, a.lddf}))
-        return linear ? bwd_v<T, sizeof(T) == 2 ? 2 : 1, SEERA_GATE_LINEAR>(s, a, st) : bwd_v<T, sizeof(T) == 2 ? 2 : 1, SEERA_GATE_SIGMOID>(s, a, st);
-    return linear ? bwd_v<T, 1, SEERA_GATE_LINEAR>(s, a, st) : bwd_v<T, 1, SEERA_GATE_SIGMOID>(s, a, st);
+int fwd_gate(const ScanShape& s, const ScanFwd& a, hipStream_t st) {
+    return s.gate == SEERA_GATE_LINEAR ? fwd_t<T, SEERA_GATE_LINEAR>(s, a, st) : fwd_t<T, SEERA_GATE_SIGMOID>(s, a, st);
+}
+template <class T>
+int bwd_gate(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
+    return s.gate == SEERA_GATE_LINEAR ? bwd_t<T, SEERA_GATE_LINEAR>(s, a, st) : bwd_t<T, SEERA_GATE_SIGMOID>(s, a, st);
 }
 
 }  // namespace
 
 int gated_scan_fwd(const ScanShape& s, const ScanFwd& a, hipStream_t st) {
-    return s.dtype == SEERA_DTYPE_F32 ? fwd_t<float>(s, a, st) : s.dtype == SEERA_DTYPE_F16 ? fwd_t<f16_t>(s, a, st) : fwd_t<bf16_t>(s, a, st);
+    return s.dtype == SEERA_DTYPE_F32 ? fwd_gate<float>(s, a, st) : s.dtype == SEERA_DTYPE_F16 ? fwd_gate<f16_t>(s, a, st) : fwd_gate<bf16_t>(s, a, st);
 }
 int gated_scan_bwd(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
-    return s.dtype == SEERA_DTYPE_F32 ? bwd_t<float>(s, a, st) : s.dtype == SEERA_DTYPE_F16 ? bwd_t<f16_t>(s, a, st) : bwd_t<bf16_t>(s, a, st);
+    return s.dtype == SEERA_DTYPE_F32 ? bwd_gate<float>(s, a, st) : s.dtype == SEERA_DTYPE_F16 ? bwd_gate<f16_t>(s, a, st) : bwd_gate<bf16_t>(s, a, st);
 }
 
 }  // namespace seera

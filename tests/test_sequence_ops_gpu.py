@@ -159,7 +159,8 @@ def _check_scan(lib, batch, time, channels, dtype, sigmoid, seed=1, lengths=None
 
 @pytest.mark.parametrize("sigmoid", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("batch,time,channels", [(1, 1, 1), (3, 1, 64), (2, 2, 33), (1, 7, 130), (2, 31, 64), (3, 129, 65), (2, 300, 96), (1, 1025, 40), (5, 640, 8)])
+@pytest.mark.parametrize("batch,time,channels", [(1, 1, 1), (3, 1, 64), (2, 2, 33), (1, 7, 130), (2, 31, 64), (3, 129, 65), (2, 300, 96), (1, 1025, 40), (5, 640, 8),
+                                                 (2, 8, 34), (2, 9, 34), (3, 32, 200), (1, 33, 200), (2, 128, 36), (2, 256, 20), (1, 511, 70)])
 def test_scan_sizes(lib, batch, time, channels, dtype, sigmoid):
     _check_scan(lib, batch, time, channels, dtype, sigmoid)
 
@@ -262,6 +263,27 @@ def test_scan_gradient_against_differences(lib, time, channels):
     slope = (loss_f(step) - loss_f(-step)) / (2 * step)
     want = (got["df"] * w).sum()
     assert abs(slope - want) <= step**2 * np.abs(got["df"] * w).sum() * 8 + 64 * q.U * size * np.sqrt(time) / step
+
+
+def test_scan_rows_far_apart(lib):
+    """Rows 8 MiB and more apart: a tile's rows would lie further from each other
+    than 32 bits of address reach. x and f are two slices of the same wide rows."""
+    time, c, ld = 40, 24, (1 << 21) + 3
+    d = _scan_data(1, time, c, q.F32, True, 12)
+    whole = np.zeros(time * ld, np.float32)
+    rows = whole.reshape(time, ld)
+    rows[:, :c], rows[:, c:2 * c] = d["x"][0], d["f"][0]
+    xf, h0, h = DeviceBuffer.from_array(whole), DeviceBuffer.from_array(d["h0"]), Rows((1, time, c), q.F32)
+    capi.call("seera_hip_gated_scan_fwd", xf.ptr, xf.ptr + 4 * c, h0.ptr, None, h.ptr, None, 1, time, c, ld, ld, 1, 0, 0)
+    ref, _, bound, _ = q.scan_fwd(d["x"], d["f"], d["h0"].astype(np.float64))
+    got = h.values()
+    _close(got, ref, bound, q.F32, "h")
+    kept, dh = Rows((1, time, c), q.F32, data=ref), Rows((1, time, c), q.F32, data=d["dh"])
+    refs, bounds = q.scan_bwd(d["x"], d["f"], _seen(ref, q.F32), d["dh"], d["h0"].astype(np.float64))
+    dx, df = (Rows((1, time, c), q.F32) for _ in range(2))
+    capi.call("seera_hip_gated_scan_bwd", xf.ptr, xf.ptr + 4 * c, h0.ptr, None, kept.ptr, dh.ptr, None, dx.ptr, df.ptr, None, 1, time, c, ld, ld, c, c, 1, 0, 0)
+    _close(dx.values(), refs["dx"], bounds["dx"], q.F32, "dx")
+    _close(df.values(), refs["df"], bounds["df"], q.F32, "df")
 
 
 # ---- block norm ----
