@@ -41,8 +41,8 @@ __device__ __forceinline__ uint32_t shared_exponent(uint32_t largest) { return l
 
 // What a launch works on: up to kMost tensors in the kernel's arguments, so that
 // a step needs no copy to the device and may be captured in a graph. Thread block
-// b works on values [(b - first) * kChunk, ...) of the last tensor with first <= b.
-constexpr int kMost = 48, kChunk = 4096, kThreads = 256;
+// b works on values [(b - first) * chunk, ...) of the last tensor with first <= b.
+constexpr int kMost = 48, kThreads = 256;
 struct Slot {
     float* param;      // adamw_values: where m's values go
     const void* grad;  // adamw_values: where v's values go
@@ -57,7 +57,7 @@ struct Batch {
     Slot slot[kMost];
     unsigned first[kMost];
     uint8_t bits[kMost], grad_dtype[kMost], copy[kMost];
-    int count;
+    int count, chunk;  // chunk: a multiple of kThreads * 8
 };
 
 // The block's slot, by one comparison in each of 48 lanes.
@@ -68,12 +68,19 @@ __device__ __forceinline__ int slot_of(const Batch& b) {
 }
 
 // N consecutive values; the cut ones at the tensor's end one by one. Whole ones are
-// one access at any alignment of T.
-template <class T, int N>
+// one access at any alignment of T (the hardware takes unaligned addresses).
+// STREAM: past the cache, for what this step alone touches.
+template <bool STREAM, class T, int N>
 __device__ __forceinline__ void load_some(T (&to)[N], const void* from, int64_t i, int live) {
     const T* p = (const T*)from + i;
     if (live == N) {
-        __builtin_memcpy(to, p, sizeof(to));
+        if constexpr (STREAM) {
+            typedef uint32_t Bits __attribute__((ext_vector_type(sizeof(to) / 4), aligned(2), may_alias));
+            const Bits w = __builtin_nontemporal_load((const Bits*)p);
+            __builtin_memcpy(to, &w, sizeof(to));
+        } else {
+            __builtin_memcpy(to, p, sizeof(to));
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < N; ++k) to[k] = k < live ? p[k] : (T)0;
@@ -83,25 +90,32 @@ template <class T, int N>
 __device__ __forceinline__ void store_some(void* to, int64_t i, const T (&from)[N], int live) {
     T* p = (T*)to + i;
     if (live == N) {
-        __builtin_memcpy(p, from, sizeof(from));
+        if constexpr (sizeof(from) >= 8) {
+            typedef uint32_t Bits __attribute__((ext_vector_type(sizeof(from) / 4), aligned(1), may_alias));
+            Bits w;
+            __builtin_memcpy(&w, from, sizeof(from));
+            __builtin_nontemporal_store(w, (Bits*)p);
+        } else {
+            __builtin_memcpy(p, from, sizeof(from));
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < N; ++k)
             if (k < live) p[k] = from[k];
     }
 }
-template <class T, int N>
+template <class T, bool STREAM, int N>
 __device__ __forceinline__ void load_as_f32(float (&to)[N], const void* from, int64_t i, int live) {
     T raw[N];
-    load_some(raw, from, i, live);
+    load_some<STREAM>(raw, from, i, live);
 #pragma unroll
     for (int k = 0; k < N; ++k) to[k] = to_f32(raw[k]);
 }
-template <int N>
+template <bool STREAM, int N>
 __device__ __forceinline__ void load_grads(float (&to)[N], const void* from, int dtype, int64_t i, int live) {
-    if (dtype == SEERA_DTYPE_F32) load_as_f32<float>(to, from, i, live);
-    else if (dtype == SEERA_DTYPE_F16) load_as_f32<f16_t>(to, from, i, live);
-    else load_as_f32<bf16_t>(to, from, i, live);
+    if (dtype == SEERA_DTYPE_F32) load_as_f32<float, STREAM>(to, from, i, live);
+    else if (dtype == SEERA_DTYPE_F16) load_as_f32<f16_t, STREAM>(to, from, i, live);
+    else load_as_f32<bf16_t, STREAM>(to, from, i, live);
 }
 template <class T, int N>
 __device__ __forceinline__ void store_rounded(void* to, int64_t i, const float (&from)[N], int live) {
@@ -142,8 +156,8 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
     const int at = slot_of(b);
     const Slot t = b.slot[at];
     const int bits = b.bits[at], dtype = b.grad_dtype[at], copy = b.copy[at];
-    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * kChunk;
-    const int64_t end = min(begin + kChunk, t.count);
+    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * b.chunk;
+    const int64_t end = min(begin + b.chunk, t.count);
     const float scale = s.grad_scale ? *s.grad_scale : 1.f;
     if (bits == 32) {
         constexpr int N = 4;
@@ -151,10 +165,10 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
         for (int64_t i = begin + threadIdx.x * N; i < end; i += kThreads * N) {
             const int live = (int)min((int64_t)N, t.count - i);
             float g[N], m[N], v[N], p[N];
-            load_grads(g, t.grad, dtype, i, live);
-            load_some(m, t.m, i, live);
-            load_some(v, t.v, i, live);
-            load_some(p, t.param, i, live);
+            load_grads<true>(g, t.grad, dtype, i, live);
+            load_some<true>(m, t.m, i, live);
+            load_some<true>(v, t.v, i, live);
+            load_some<true>(p, t.param, i, live);
             update(s, t.keep, scale, g, m, v, p);
             store_some(t.m, i, m, live);
             store_some(t.v, i, v, live);
@@ -169,10 +183,10 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
         const int64_t block = i / kBlock;
         float g[N], m[N], v[N], p[N];
         uint8_t cm[N], cv[N];
-        load_grads(g, t.grad, dtype, i, live);
-        load_some(cm, t.m, i, live);
-        load_some(cv, t.v, i, live);
-        load_some(p, t.param, i, live);
+        load_grads<false>(g, t.grad, dtype, i, live);
+        load_some<false>(cm, t.m, i, live);
+        load_some<false>(cv, t.v, i, live);
+        load_some<false>(p, t.param, i, live);
         uint32_t em = t.m_exp[block], ev = t.v_exp[block];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
@@ -211,35 +225,50 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
 __global__ __launch_bounds__(kThreads) void adamw_values(Batch b) {
     const int at = slot_of(b);
     const Slot t = b.slot[at];
-    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * kChunk;
-    const int64_t end = min(begin + kChunk, t.count);
+    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * b.chunk;
+    const int64_t end = min(begin + b.chunk, t.count);
     float *m_out = t.param, *v_out = (float*)t.grad;
-    constexpr int N = 4;
-    for (int64_t i = begin + threadIdx.x * N; i < end; i += kThreads * N) {
-        const int live = (int)min((int64_t)N, t.count - i);
-        float x[N];
-        uint8_t c[N];
-        if (b.bits[at] == 32) {
-            if (m_out) load_some(x, t.m, i, live), store_some(m_out, i, x, live);
-            if (v_out) load_some(x, t.v, i, live), store_some(v_out, i, x, live);
-            continue;
+    if (b.bits[at] == 32) {
+        constexpr int N = 4;
+        for (int64_t i = begin + threadIdx.x * N; i < end; i += kThreads * N) {
+            const int live = (int)min((int64_t)N, t.count - i);
+            float x[N];
+            if (m_out) load_some<false>(x, t.m, i, live), store_some(m_out, i, x, live);
+            if (v_out) load_some<false>(x, t.v, i, live), store_some(v_out, i, x, live);
         }
-        if (m_out) {
-            load_some(c, t.m, i, live);
-            const uint32_t e = t.m_exp[i / kBlock];
+        return;
+    }
+    // four values a lane and store, so that a wave writes 1 KB in one piece; two of
+    // them in flight
+    constexpr int N = 4, K = 2;
+    for (int64_t i0 = begin + threadIdx.x * N; i0 < end; i0 += kThreads * N * K) {
+        uint8_t cm[K][N], cv[K][N];
+        uint32_t em[K], ev[K];
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                x[k] = decode(c[k] & 127, e, 15);
-                if (c[k] & 128) x[k] = -x[k];
+        for (int k = 0; k < K; ++k) {
+            const int64_t i = i0 + k * kThreads * N;
+            if (i >= end) break;
+            const int live = (int)min((int64_t)N, t.count - i);
+            load_some<false>(cm[k], t.m, i, live);
+            load_some<false>(cv[k], t.v, i, live);
+            em[k] = t.m_exp[i / kBlock];
+            ev[k] = t.v_exp[i / kBlock];
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int64_t i = i0 + k * kThreads * N;
+            if (i >= end) break;
+            const int live = (int)min((int64_t)N, t.count - i);
+            float x[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                x[j] = decode(cm[k][j] & 127, em[k], 15);
+                if (cm[k][j] & 128) x[j] = -x[j];
             }
-            store_some(m_out, i, x, live);
-        }
-        if (v_out) {
-            load_some(c, t.v, i, live);
-            const uint32_t e = t.v_exp[i / kBlock];
+            if (m_out) store_some(m_out, i, x, live);
 #pragma unroll
-            for (int k = 0; k < N; ++k) x[k] = decode(c[k], e, 31);
-            store_some(v_out, i, x, live);
+            for (int j = 0; j < N; ++j) x[j] = decode(cv[k][j], ev[k], 31);
+            if (v_out) store_some(v_out, i, x, live);
         }
     }
 }
@@ -249,12 +278,15 @@ __global__ __launch_bounds__(kThreads) void adamw_values(Batch b) {
 template <class Fill, class Launch>
 int batches(const seera_adamw_tensor* tensors, int n, Fill&& fill, Launch&& launch) {
     Batch b;
-    int64_t blocks = 0;
+    int64_t blocks = 0, total = 0;
+    for (int i = 0; i < n; ++i) total += tensors[i].count;
     b.count = 0;
+    // small models: smaller shares, so that every compute unit has one
+    b.chunk = total < 16384 * (int64_t)device_cus() ? 2048 : 4096;
     for (int i = 0; i < n; ++i) {
         const seera_adamw_tensor& t = tensors[i];
         if (t.count == 0) continue;
-        const int64_t more = (t.count + kChunk - 1) / kChunk;
+        const int64_t more = (t.count + b.chunk - 1) / b.chunk;
         if (more > kMaxGridX) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: tensor %d is too large", i);
         if (b.count == kMost || blocks + more > kMaxGridX) {
             launch(b, (unsigned)blocks);

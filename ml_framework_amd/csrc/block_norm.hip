@@ -63,58 +63,73 @@ __device__ __forceinline__ float slope_of(int act, float g) {
 }
 
 // 16 bytes of a row, moved as one access at any alignment of T (the hardware
-// takes unaligned addresses). CUT: the row's last pack may be cut, and goes value
-// by value. A pack past the row's end is zeros and is not stored.
+// takes unaligned addresses) and without a branch, so that nothing waits for a
+// load before its values are used. The pack at column `want` lies at `c`: moved
+// back where it would pass the row's end, so that some of its values belong to
+// the pack before it, or all of them. Values lo <= i < hi are its own: only they
+// enter sums and are stored. With CUT false (cols is a multiple of N) a pack is
+// whole or has no value.
 template <class T>
 struct Wide {
     static constexpr int N = 16 / sizeof(T);
     T v[N];
 };
-template <bool CUT, class T>
-__device__ __forceinline__ void load_wide(Wide<T>& to, const T* row, int c, int cols) {
-    constexpr int N = Wide<T>::N;
-    if (!CUT) {
-        // no branch: lanes past the end load the last pack and drop it
-        uint32_t bits[4];
-        __builtin_memcpy(bits, row + min(c, cols - N), 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bits[i] = c < cols ? bits[i] : 0u;
-        __builtin_memcpy(&to, bits, 16);
-    } else if (c + N <= cols) {
-        __builtin_memcpy(&to, row + c, 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) to.v[i] = c + i < cols ? row[c + i] : from_f32<T>(0.f);
+template <int N, bool CUT>
+struct Place {
+    int c, lo, hi;
+    __device__ Place(int want, int cols) {
+        c = max(min(want, cols - N), 0);
+        lo = CUT ? min(want - c, N) : want < cols ? 0 : N;
+        hi = CUT ? min(N, cols - c) : N;
     }
+    __device__ bool whole() const { return lo == 0 && (!CUT || hi == N); }
+    __device__ bool own(int i) const { return CUT ? i >= lo && i < hi : lo == 0; }
+    // x in a sum: 0 where value i is not the pack's own
+    __device__ float mine(int i, float x) const { return !CUT || own(i) ? x : 0.f; }
+    // a pack's part of a sum
+    __device__ float part(float x) const { return CUT || lo == 0 ? x : 0.f; }
+};
+template <class T, bool CUT>
+__device__ __forceinline__ void load_wide(Wide<T>& to, const T* row, const Place<Wide<T>::N, CUT>& at, int cols) {
+    typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));
+    if (CUT && cols < Wide<T>::N) {
+#pragma unroll
+        for (int i = 0; i < Wide<T>::N; ++i) to.v[i] = i < at.hi ? row[i] : from_f32<T>(0.f);
+        return;
+    }
+    // streamed past the cache where rows share no line of it
+    const Bits w = CUT ? *(const Bits*)(row + at.c) : __builtin_nontemporal_load((const Bits*)(row + at.c));
+    __builtin_memcpy(&to, &w, 16);
 }
-template <bool CUT, class T>
-__device__ __forceinline__ void store_wide(T* row, int c, int cols, const Wide<T>& from) {
-    constexpr int N = Wide<T>::N;
-    if (c + N <= cols) {
-        __builtin_memcpy(row + c, &from, sizeof(from));
+template <class T, bool CUT>
+__device__ __forceinline__ void store_wide(T* row, const Place<Wide<T>::N, CUT>& at, const Wide<T>& from) {
+    typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));
+    if (at.whole()) {
+        Bits w;
+        __builtin_memcpy(&w, &from, 16);
+        __builtin_nontemporal_store(w, (Bits*)(row + at.c));
     } else if (CUT) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (c + i < cols) row[c + i] = from.v[i];
+        for (int i = 0; i < Wide<T>::N; ++i)
+            if (at.own(i)) row[at.c + i] = from.v[i];
     }
 }
-// N fp32 weights from column c on; what lies past the end is of no effect.
-template <bool CUT, int N>
-__device__ __forceinline__ void load_weights(float (&to)[N], const float* w, int c, int cols) {
-    if (!CUT) {
-        __builtin_memcpy(to, w + min(c, cols - N), sizeof(to));
-    } else if (c + N <= cols) {
-        __builtin_memcpy(to, w + c, sizeof(to));
-    } else {
+// The N fp32 weights of a pack.
+template <int N, bool CUT>
+__device__ __forceinline__ void load_weights(float (&to)[N], const float* w, const Place<N, CUT>& at, int cols) {
+    if (CUT && cols < N) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) to[i] = c + i < cols ? w[c + i] : 0.f;
+        for (int i = 0; i < N; ++i) to[i] = i < at.hi ? w[i] : 0.f;
+        return;
     }
+    __builtin_memcpy(to, w + at.c, sizeof(to));
 }
 
 // A row in the registers of NT threads, K wide packs each; ROWS rows a block.
 template <class T, int K, int NT, int ROWS, bool CUT>
 __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape s) {
     constexpr int N = Wide<T>::N;
+    typedef Place<N, CUT> At;
     __shared__ float part[2 * (NT / 64) * ROWS];
     const int tid = threadIdx.x % NT;
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT;
@@ -122,34 +137,39 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
     const T* yr = (const T*)p.y + row * p.ldy;
     const T* gr = (const T*)p.g + row * p.ldg;
     const T* rr = (const T*)p.r + row * s.cols;
+    auto place = [&](int k) { return At((k * NT + tid) * N, s.cols); };
     Wide<T> y[K], g[K], r[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) load_wide<CUT>(y[k], yr, (k * NT + tid) * N, s.cols);
+    for (int k = 0; k < K; ++k) load_wide(y[k], yr, place(k), s.cols);
     if (p.g)
 #pragma unroll
-        for (int k = 0; k < K; ++k) load_wide<CUT>(g[k], gr, (k * NT + tid) * N, s.cols);
+        for (int k = 0; k < K; ++k) load_wide(g[k], gr, place(k), s.cols);
     if (p.r)
 #pragma unroll
-        for (int k = 0; k < K; ++k) load_wide<CUT>(r[k], rr, (k * NT + tid) * N, s.cols);
+        for (int k = 0; k < K; ++k) load_wide(r[k], rr, place(k), s.cols);
     float rstd1 = 1.f;
     if (p.w1) {
         float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            const At at = place(k);
+            float own = 0.f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum = fmaf(to_f32(y[k].v[i]), to_f32(y[k].v[i]), sum);
+            for (int i = 0; i < N; ++i) own = fmaf(to_f32(y[k].v[i]), at.mine(i, to_f32(y[k].v[i])), own);
+            sum += at.part(own);
+        }
         rstd1 = rsqrtf(row_sum<NT>(sum, part, 0) / s.cols + p.eps);
         if (p.rstd1 && tid == 0) p.rstd1[row] = rstd1;
     }
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int c = (k * NT + tid) * N;
+        const At at = place(k);
         float u[N], w[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) u[i] = to_f32(y[k].v[i]);
         if (p.w1) {
-            load_weights<CUT>(w, p.w1, c, s.cols);
+            load_weights(w, p.w1, at, s.cols);
 #pragma unroll
             for (int i = 0; i < N; ++i) u[i] = u[i] * rstd1 * w[i];
         }
@@ -157,31 +177,37 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
 #pragma unroll
             for (int i = 0; i < N; ++i) u[i] *= act_of(s.act, to_f32(g[k].v[i]));
         if (p.s) {
-            load_weights<CUT>(w, p.s, c, s.cols);
+            load_weights(w, p.s, at, s.cols);
 #pragma unroll
             for (int i = 0; i < N; ++i) u[i] *= w[i];
         }
         if (p.r)
 #pragma unroll
             for (int i = 0; i < N; ++i) u[i] += to_f32(r[k].v[i]);
+        float own = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             y[k].v[i] = from_f32<T>(u[i]);  // as it is kept
-            sum = fmaf(to_f32(y[k].v[i]), to_f32(y[k].v[i]), sum);
+            own = fmaf(to_f32(y[k].v[i]), at.mine(i, to_f32(y[k].v[i])), own);
         }
-        if (p.r_out) store_wide<CUT>((T*)p.r_out + row * s.cols, c, s.cols, y[k]);
+        sum += at.part(own);
     }
+    // a row's packs may reach into each other: all of it is read before any is written
+    if (CUT && NT > 64 && !p.w1) __syncthreads();
+    if (p.r_out)
+#pragma unroll
+        for (int k = 0; k < K; ++k) store_wide((T*)p.r_out + row * s.cols, place(k), y[k]);
     if (!p.w2) return;
     const float rstd2 = rsqrtf(row_sum<NT>(sum, part, 1) / s.cols + p.eps);
     if (p.rstd2 && tid == 0) p.rstd2[row] = rstd2;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int c = (k * NT + tid) * N;
+        const At at = place(k);
         float w[N];
-        load_weights<CUT>(w, p.w2, c, s.cols);
+        load_weights(w, p.w2, at, s.cols);
 #pragma unroll
         for (int i = 0; i < N; ++i) y[k].v[i] = from_f32<T>(to_f32(y[k].v[i]) * rstd2 * w[i]);
-        store_wide<CUT>((T*)p.n_out + row * s.cols, c, s.cols, y[k]);
+        store_wide((T*)p.n_out + row * s.cols, at, y[k]);
     }
 }
 
@@ -197,10 +223,11 @@ struct NormRow {
 template <class T, int K, int NT, bool NEXT, bool HOLD, bool CUT>
 __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, float* partial) {
     constexpr int N = Wide<T>::N;
+    typedef Place<N, CUT> At;
     __shared__ float part[2 * (NT / 64)];
     const bool inner = p.w1 || p.g || p.s;
     float h1[K][N], hs[K][N], h2[K][N], sum1[K][N], sums[K][N], sum2[K][N];
-    auto column = [](int k) { return (int)(k * NT + threadIdx.x) * N; };
+    auto place = [&](int k) { return At((int)(k * NT + threadIdx.x) * N, s.cols); };
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -212,23 +239,23 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int i = 0; i < N; ++i) to[k][i] = 1.f;
-            int c = column(k);
-            if (!HOLD) asm volatile("" : "+v"(c));  // an address of this row's own: the loads stay in the loop
-            if (w) load_weights<CUT>(to[k], w, c, s.cols);
+            At at = place(k);
+            if (!HOLD) asm volatile("" : "+v"(at.c));  // an address of this row's own: the loads stay in the loop
+            if (w) load_weights(to[k], w, at, s.cols);
         }
     };
     if (HOLD) weights(h1, p.w1), weights(hs, p.s), weights(h2, p.w2);
     auto load = [&](NormRow<T, K>& to, int64_t row) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int c = column(k);
-            if (inner) load_wide<CUT>(to.y[k], (const T*)p.y + row * p.ldy, c, s.cols);
-            if (p.g) load_wide<CUT>(to.g[k], (const T*)p.g + row * p.ldg, c, s.cols);
+            const At c = place(k);
+            if (inner) load_wide(to.y[k], (const T*)p.y + row * p.ldy, c, s.cols);
+            if (p.g) load_wide(to.g[k], (const T*)p.g + row * p.ldg, c, s.cols);
             if (p.w2) {
-                load_wide<CUT>(to.r[k], (const T*)p.r_out + row * s.cols, c, s.cols);
-                load_wide<CUT>(to.n[k], (const T*)p.dn + row * s.cols, c, s.cols);
+                load_wide(to.r[k], (const T*)p.r_out + row * s.cols, c, s.cols);
+                load_wide(to.n[k], (const T*)p.dn + row * s.cols, c, s.cols);
             }
-            if (p.dr_out) load_wide<CUT>(to.d[k], (const T*)p.dr_out + row * s.cols, c, s.cols);
+            if (p.dr_out) load_wide(to.d[k], (const T*)p.dr_out + row * s.cols, c, s.cols);
         }
         to.rstd1 = p.w1 ? p.rstd1[row] : 1.f;
         if (p.w2) to.rstd2 = p.rstd2[row];
@@ -249,13 +276,17 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
             if (!HOLD) weights(h2, p.w2);
             float dot = 0.f;
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k) {
+                const At at = place(k);
+                float own = 0.f;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float hat = to_f32(now.r[k].v[i]) * now.rstd2, dn = to_f32(now.n[k].v[i]);
                     sum2[k][i] = fmaf(dn, hat, sum2[k][i]);
-                    dot = fmaf(dn * h2[k][i], hat, dot);
+                    own = fmaf(dn * h2[k][i], at.mine(i, hat), own);
                 }
+                dot += at.part(own);
+            }
             dot = row_sum<NT>(dot, part, 0) * inv;
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -266,6 +297,8 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
                 }
         }
         if (!HOLD) weights(h1, p.w1), weights(hs, p.s);
+        // a row's packs may reach into each other: all of it is read before any is written
+        if (CUT && NT > 64 && !p.w2) __syncthreads();
         float dot = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -273,7 +306,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
             if (p.dr) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) out.v[i] = from_f32<T>(d[k][i]);
-                store_wide<CUT>((T*)p.dr + row * s.cols, column(k), s.cols, out);
+                store_wide((T*)p.dr + row * s.cols, place(k), out);
             }
             if (p.g) {
 #pragma unroll
@@ -285,7 +318,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
                     out.v[i] = from_f32<T>(d[k][i] * z * (s.act == SEERA_GATE_ACT_SILU ? fmaf(g, slope, q) : slope));
                     d[k][i] *= act;
                 }
-                store_wide<CUT>((T*)p.dg + row * p.lddg, column(k), s.cols, out);
+                store_wide((T*)p.dg + row * p.lddg, place(k), out);
             } else if (p.s) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -294,13 +327,16 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
                 }
             }
             if (p.w1) {
+                const At at = place(k);
+                float own = 0.f;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float hat = to_f32(now.y[k].v[i]) * now.rstd1;
                     sum1[k][i] = fmaf(d[k][i], hat, sum1[k][i]);
                     d[k][i] *= h1[k][i];
-                    dot = fmaf(d[k][i], hat, dot);
+                    own = fmaf(d[k][i], at.mine(i, hat), own);
                 }
+                dot += at.part(own);
             }
         }
         if (p.w1) {
@@ -315,7 +351,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
             Wide<T> out;
 #pragma unroll
             for (int i = 0; i < N; ++i) out.v[i] = from_f32<T>(d[k][i]);
-            store_wide<CUT>((T*)p.dy + row * p.lddy, column(k), s.cols, out);
+            store_wide((T*)p.dy + row * p.lddy, place(k), out);
         }
         if (NEXT) now = next;
     }
@@ -324,8 +360,9 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = column(k) + i;
-            if (c >= s.cols) continue;
+            const At at = place(k);
+            const int c = at.c + i;
+            if (!at.own(i)) continue;
             if (p.w1) to[c] = sum1[k][i];
             if (p.s) to[s.cols + c] = sums[k][i];
             if (p.w2) to[2 * s.cols + c] = sum2[k][i];
@@ -454,8 +491,10 @@ template <class T>
 int bwd_t(const NormShape& s, const NormBwd& a, hipStream_t st) {
     constexpr int N = Wide<T>::N;
     const int packs = (s.cols + N - 1) / N;
-    const int threads = packs <= 64 ? 64 : packs <= 128 ? 128 : packs <= 256 ? 256 : 512;
-    const int blocks = (int)std::min<int64_t>(s.rows, (int64_t)device_cus() * std::max(1, 512 / threads));
+    const int threads = packs <= 64 ? 64 : packs <= 128 ? 128 : packs <= 512 ? 256 : 512;
+    // 512 threads a compute unit, and four rows a block before there are that many
+    const int64_t cus = device_cus(), most = cus * (512 / threads);
+    const int blocks = (int)(s.rows <= cus ? s.rows : std::min(most, std::max<int64_t>(cus, s.rows / 4)));
     void* ws = nullptr;
     SEERA_TRY(workspace((size_t)std::max(blocks, 1) * 3 * s.cols * sizeof(float), &ws, st));
     if (blocks) {
@@ -463,7 +502,7 @@ int bwd_t(const NormShape& s, const NormBwd& a, hipStream_t st) {
         if (packs <= 64) bwd_launch<T, 1, 64, true, true>(s, a, blocks, to, st);
         else if (packs <= 128) bwd_launch<T, 1, 128, true, true>(s, a, blocks, to, st);
         else if (packs <= 256) bwd_launch<T, 1, 256, true, true>(s, a, blocks, to, st);
-        else if (packs <= 512) bwd_launch<T, 1, 512, true, true>(s, a, blocks, to, st);
+        else if (packs <= 512) bwd_launch<T, 2, 256, false, true>(s, a, blocks, to, st);
         else if (packs <= 1024) bwd_launch<T, 2, 512, N == 4, false>(s, a, blocks, to, st);
         else bwd_wide<T>(s, a, blocks, to, st);
         SEERA_HIP_TRY(hipGetLastError());

@@ -163,6 +163,7 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
     constexpr int W = NT / 64, SL = 64 / CL, kSteps = W * SL * L;
     typedef Pack<T, V> P;
     typedef Steps<T, V, L> S;
+    typedef std::conditional_t<sizeof(P) == 8, uint64_t, std::conditional_t<sizeof(P) == 4, uint32_t, uint16_t>> Bits __attribute__((may_alias));
     __shared__ float2 totals[2][W][CL][V];
     // neighbouring channel groups on one die: they share lines of memory
     const unsigned chunk = (blocks + 7) / 8, id = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
@@ -194,7 +195,10 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
             const char* q = (const char*)base + (low_row(u0) - shift * step) * ld * (int64_t)sizeof(T);
             const unsigned mine = from_low * (unsigned)(step * ld * (int64_t)sizeof(T)) + c * (unsigned)sizeof(T);
 #pragma unroll
-            for (int i = 0; i < L; ++i, q += stride) to.v[i] = *(const P*)(q + mine);
+            for (int i = 0; i < L; ++i, q += stride) {
+                const Bits w = __builtin_nontemporal_load((const Bits*)(q + mine));
+                __builtin_memcpy(&to.v[i], &w, sizeof(w));
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < L; ++i) to.v[i] = P{};
