@@ -357,6 +357,99 @@ PYBIND11_MODULE(seera_cuda, m) {
           },
           "Broadcast mul 4D (GPU ptrs)");
 
+    // ---- sequence models (no counterpart in the reference) ----
+    m.attr("DTYPE_F32") = (int)SEERA_DTYPE_F32;
+    m.attr("DTYPE_F16") = (int)SEERA_DTYPE_F16;
+    m.attr("DTYPE_BF16") = (int)SEERA_DTYPE_BF16;
+    m.attr("GATE_LINEAR") = (int)SEERA_GATE_LINEAR;
+    m.attr("GATE_SIGMOID") = (int)SEERA_GATE_SIGMOID;
+    m.attr("GATE_ACT_SILU") = (int)SEERA_GATE_ACT_SILU;
+    m.attr("GATE_ACT_SIGMOID") = (int)SEERA_GATE_ACT_SIGMOID;
+    m.def("cuda_gated_scan_fwd",
+          [](uintptr_t x, uintptr_t f, uintptr_t h0, uintptr_t lengths, uintptr_t h, uintptr_t hT,
+             int batch, int time, int channels, int64_t ldx, int64_t ldf, int gate, int time_major,
+             int dtype) {
+              check(seera_hip_gated_scan_fwd(dev<const void>(x), dev<const void>(f),
+                                             dev<const float>(h0), dev<const int>(lengths),
+                                             dev<void>(h), dev<float>(hT), batch, time, channels,
+                                             ldx, ldf, gate, time_major, dtype));
+          },
+          "Gated linear recurrence over time (GPU ptrs; 0 for an optional one)");
+    m.def("cuda_gated_scan_bwd",
+          [](uintptr_t x, uintptr_t f, uintptr_t h0, uintptr_t lengths, uintptr_t h, uintptr_t dh,
+             uintptr_t dhT, uintptr_t dx, uintptr_t df, uintptr_t dh0, int batch, int time,
+             int channels, int64_t ldx, int64_t ldf, int64_t lddx, int64_t lddf, int gate,
+             int time_major, int dtype) {
+              check(seera_hip_gated_scan_bwd(
+                  dev<const void>(x), dev<const void>(f), dev<const float>(h0),
+                  dev<const int>(lengths), dev<const void>(h), dev<const void>(dh),
+                  dev<const float>(dhT), dev<void>(dx), dev<void>(df), dev<float>(dh0), batch, time,
+                  channels, ldx, ldf, lddx, lddf, gate, time_major, dtype));
+          },
+          "Gated linear recurrence backward (GPU ptrs; 0 for an optional one)");
+    m.def("cuda_block_norm_fwd",
+          [](uintptr_t y, uintptr_t g, uintptr_t r, uintptr_t w1, uintptr_t s, uintptr_t w2,
+             uintptr_t r_out, uintptr_t n_out, uintptr_t rstd1, uintptr_t rstd2, int rows, int cols,
+             int64_t ldy, int64_t ldg, float eps, int act, int dtype) {
+              check(seera_hip_block_norm_fwd(
+                  dev<const void>(y), dev<const void>(g), dev<const void>(r), dev<const float>(w1),
+                  dev<const float>(s), dev<const float>(w2), dev<void>(r_out), dev<void>(n_out),
+                  dev<float>(rstd1), dev<float>(rstd2), rows, cols, ldy, ldg, eps, act, dtype));
+          },
+          "Norms after and before a block, gate, scale and residual (GPU ptrs; 0 for an optional one)");
+    m.def("cuda_block_norm_bwd",
+          [](uintptr_t y, uintptr_t g, uintptr_t r_out, uintptr_t w1, uintptr_t s, uintptr_t w2,
+             uintptr_t rstd1, uintptr_t rstd2, uintptr_t dr_out, uintptr_t dn, uintptr_t dy,
+             uintptr_t dg, uintptr_t dr, uintptr_t dw1, uintptr_t ds, uintptr_t dw2, int rows,
+             int cols, int64_t ldy, int64_t ldg, int64_t lddy, int64_t lddg, int act, int dtype) {
+              check(seera_hip_block_norm_bwd(
+                  dev<const void>(y), dev<const void>(g), dev<const void>(r_out),
+                  dev<const float>(w1), dev<const float>(s), dev<const float>(w2),
+                  dev<const float>(rstd1), dev<const float>(rstd2), dev<const void>(dr_out),
+                  dev<const void>(dn), dev<void>(dy), dev<void>(dg), dev<void>(dr), dev<float>(dw1),
+                  dev<float>(ds), dev<float>(dw2), rows, cols, ldy, ldg, lddy, lddg, act, dtype));
+          },
+          "Block norm backward (GPU ptrs; 0 for an optional one)");
+    // One tensor of an AdamW step; pointers as ints, like everywhere here.
+    py::class_<seera_adamw_tensor> tensor(m, "AdamwTensor");
+    tensor.def(py::init([] { return seera_adamw_tensor{}; }))
+        .def_readwrite("count", &seera_adamw_tensor::count)
+        .def_readwrite("weight_decay", &seera_adamw_tensor::weight_decay)
+        .def_readwrite("grad_dtype", &seera_adamw_tensor::grad_dtype)
+        .def_readwrite("param16_dtype", &seera_adamw_tensor::param16_dtype)
+        .def_readwrite("state_bits", &seera_adamw_tensor::state_bits);
+#define SEERA_POINTER(field, type)                                                                  \
+    tensor.def_property(                                                                            \
+        #field, [](const seera_adamw_tensor& t) { return reinterpret_cast<uintptr_t>(t.field); },   \
+        [](seera_adamw_tensor& t, uintptr_t p) { t.field = dev<type>(p); })
+    SEERA_POINTER(param, float);
+    SEERA_POINTER(grad, const void);
+    SEERA_POINTER(m, void);
+    SEERA_POINTER(v, void);
+    SEERA_POINTER(m_exp, uint8_t);
+    SEERA_POINTER(v_exp, uint8_t);
+    SEERA_POINTER(param16, void);
+#undef SEERA_POINTER
+    m.def("cuda_adamw_step",
+          [](const std::vector<seera_adamw_tensor>& tensors, double lr, double beta1, double beta2,
+             double eps, int64_t step, uint32_t seed, uintptr_t grad_scale) {
+              check(seera_hip_adamw_step(tensors.data(), (int)tensors.size(), lr, beta1, beta2, eps,
+                                         step, seed, dev<const float>(grad_scale)));
+          },
+          "AdamW step over a list of AdamwTensor, in place (grad_scale: GPU ptr or 0)");
+    m.def("cuda_adamw_state_values",
+          [](const std::vector<seera_adamw_tensor>& tensors, const std::vector<uintptr_t>& m_values,
+             const std::vector<uintptr_t>& v_values) {
+              if (m_values.size() != tensors.size() || v_values.size() != tensors.size())
+                  throw std::invalid_argument("seera_cuda: one pointer for each tensor is needed");
+              std::vector<float*> pm, pv;
+              for (uintptr_t p : m_values) pm.push_back(dev<float>(p));
+              for (uintptr_t p : v_values) pv.push_back(dev<float>(p));
+              check(seera_hip_adamw_state_values(tensors.data(), (int)tensors.size(), pm.data(),
+                                                 pv.data()));
+          },
+          "The moments of a list of AdamwTensor as fp32 (lists of GPU ptrs, 0 to skip one)");
+
     // ---- transfers (cuda_bindings.cpp:73-170) ----
     m.def("to_device_f16", [](arr_f a) { return upload<float>(a); },
           "Upload float32 numpy -> float32 GPU buffer (reference name)");
