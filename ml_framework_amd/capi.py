@@ -174,7 +174,9 @@ def check(status: int) -> None:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise on failure."""
-    check(getattr(load(), name)(*args))
+    status = getattr(_lib or load(), name)(*args)
+    if status != SEERA_OK:
+        check(status)
 
 
 def gpu_available() -> bool:

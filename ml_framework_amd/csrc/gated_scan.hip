@@ -177,7 +177,8 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
     const int n = steps_of(p.lengths, b, s.time);
     const int channel = (group * CL + cl) * V;
     const bool active = channel < s.channels;
-    const int c = active ? channel : s.channels - V;  // loads stay inside the row
+    // lanes past the last channel do that channel's work again: same loads, same values, same stores
+    const int c = active ? channel : s.channels - V;
     const int64_t step = s.time_major ? s.batch : 1, row0 = s.time_major ? b : (int64_t)b * s.time;
     const int64_t state = (int64_t)b * s.channels + c, states = (int64_t)s.batch * s.channels;
     const int first = (wave * SL + slot) * L;  // of the thread's steps in a tile
@@ -189,9 +190,9 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
     const int64_t dir = DIR == 0 ? 1 : -1;
     auto low_row = [&](int u0) { return row0 + (int64_t)(DIR == 0 ? begin + u0 : end - u0 - kSteps) * step; };
     const unsigned from_low = DIR == 0 ? first : kSteps - 1 - first;
-    auto load = [&](const void* base, int64_t ld, int u0, int shift, auto whole, S& to) {
-        const int64_t stride = dir * step * ld * (int64_t)sizeof(T);
-        if (decltype(whole)::value) {
+    auto load = [&](const void* base, int64_t ld, int u0, int shift, bool whole, S& to) {
+        if (whole) {
+            const int64_t stride = dir * step * ld * (int64_t)sizeof(T);
             const char* q = (const char*)base + (low_row(u0) - shift * step) * ld * (int64_t)sizeof(T);
             const unsigned mine = from_low * (unsigned)(step * ld * (int64_t)sizeof(T)) + c * (unsigned)sizeof(T);
 #pragma unroll
@@ -211,20 +212,17 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
         }
     };
     constexpr bool kNeedX = DIR == 0 || (!MAPS && GATE == SEERA_GATE_SIGMOID), kNeedH = DIR == 1 && !MAPS;
-    auto load_all = [&](int u0, auto whole, S& x, S& f, S& d, S& h) {
-        load(p.f, p.ldf, u0, 0, whole, f);
-        if (kNeedX) load(p.x, p.ldx, u0, 0, whole, x);
-        if (DIR == 1) load(p.dh, s.channels, u0, 0, whole, d);
-        if (kNeedH) load(p.h, s.channels, u0, 1, whole, h);
-    };
     // inside the segment, the sequence, and (for h one step before) past its first step
     auto is_whole = [&](int u0) {
         if (u0 + kSteps > length) return false;
         return DIR == 0 ? begin + u0 + kSteps <= n : end - u0 <= n && end - u0 - kSteps > 0;
     };
     auto load_tile = [&](int u0, S& x, S& f, S& d, S& h) {
-        if (is_whole(u0)) load_all(u0, std::true_type{}, x, f, d, h);
-        else load_all(u0, std::false_type{}, x, f, d, h);
+        const bool whole = is_whole(u0);
+        load(p.f, p.ldf, u0, 0, whole, f);
+        if (kNeedX) load(p.x, p.ldx, u0, 0, whole, x);
+        if (DIR == 1) load(p.dh, s.channels, u0, 0, whole, d);
+        if (kNeedH) load(p.h, s.channels, u0, 1, whole, h);
     };
 
     float carry[V], h0[V];
@@ -278,8 +276,21 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
             }
     };
     S rx, rf, rd, rh, nx, nf, nd, nh;
-    auto compute = [&](int u0, auto whole_tile) {
-        constexpr bool kWhole = decltype(whole_tile)::value;
+    auto compute = [&](int u0) {
+        const bool cut = !is_whole(u0);
+        if (cut) {
+            // steps outside: a = 1 and nothing added
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int u = u0 + first + i;
+                if (u < length && (DIR == 0 ? begin + u : end - 1 - u) < n) continue;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    rf.v[i].v[v] = from_f32<T>(GATE == SEERA_GATE_LINEAR ? 1.f : __builtin_inff());
+                    (DIR == 0 ? rx : rd).v[i].v[v] = from_f32<T>(0.f);
+                }
+            }
+        }
         // kept for the second run: a and b; backward the gates' small sides (f and dh
         // are in registers as they came)
         float a[DIR == 0 ? L : 1][V], m[L][V];
@@ -288,15 +299,6 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
         for (int v = 0; v < V; ++v) A[v] = 1.f, B[v] = 0.f;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int u = u0 + first + i;
-            if (!kWhole && !(u < length && (DIR == 0 ? begin + u : end - 1 - u) < n)) {
-                // a step outside: a = 1, nothing added
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    rf.v[i].v[v] = from_f32<T>(GATE == SEERA_GATE_LINEAR ? 1.f : __builtin_inff());
-                    (DIR == 0 ? rx : rd).v[i].v[v] = from_f32<T>(0.f);
-                }
-            }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float f = to_f32(rf.v[i].v[v]), small = GATE == SEERA_GATE_LINEAR ? 0.f : small_side(f);
@@ -316,40 +318,47 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
         float z[V];
         compose(A, B, z);
         if (MAPS) return;
-        auto run = [&](int i, P& o, P& o2) {
-            const int u = u0 + first + i, t = DIR == 0 ? begin + u : end - 1 - u;
-            const bool live = kWhole || t < n;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (DIR == 0) {
-                    z[v] = fmaf(a[i][v], z[v], m[i][v]);
-                    o.v[v] = from_f32<T>(live ? z[v] : 0.f);
-                } else {
-                    float ai, rest;
-                    sides<GATE>(to_f32(rf.v[i].v[v]), m[i][v], ai, rest);
-                    const float g = to_f32(rd.v[i].v[v]) + z[v];
-                    z[v] = ai * g;
-                    const float before = kWhole || t > 0 ? to_f32(rh.v[i].v[v]) : h0[v];
-                    const float one = g * rest;
-                    const float two = GATE == SEERA_GATE_SIGMOID ? one * (before - to_f32(rx.v[i].v[v])) * ai : g * before;
-                    o.v[v] = from_f32<T>(live ? one : 0.f);
-                    o2.v[v] = from_f32<T>(live ? two : 0.f);
-                }
-            }
-        };
         const int64_t stride = dir * step * p.ldo * (int64_t)sizeof(T), stride2 = dir * step * p.ldo2 * (int64_t)sizeof(T);
         char* q = (char*)p.out + low_row(u0) * p.ldo * (int64_t)sizeof(T);
         char* q2 = (char*)p.out2 + low_row(u0) * p.ldo2 * (int64_t)sizeof(T);
         const unsigned mine = from_low * (unsigned)(step * p.ldo * (int64_t)sizeof(T)) + c * (unsigned)sizeof(T);
         const unsigned mine2 = from_low * (unsigned)(step * p.ldo2 * (int64_t)sizeof(T)) + c * (unsigned)sizeof(T);
+        auto second = [&](auto whole_tile) {
+            constexpr bool kWhole = decltype(whole_tile)::value;
 #pragma unroll
-        for (int i = 0; i < L; ++i, q += stride, q2 += stride2) {
-            P o, o2;
-            run(i, o, o2);
-            if (active && (kWhole || u0 + first + i < length)) {
-                *(P*)(q + mine) = o;
-                if (DIR == 1) *(P*)(q2 + mine2) = o2;
+            for (int i = 0; i < L; ++i, q += stride, q2 += stride2) {
+                const int u = u0 + first + i, t = DIR == 0 ? begin + u : end - 1 - u;
+                P o, o2;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float one, two = 0.f;
+                    if (DIR == 0) {
+                        one = z[v] = fmaf(a[i][v], z[v], m[i][v]);
+                    } else {
+                        float ai, rest;
+                        sides<GATE>(to_f32(rf.v[i].v[v]), m[i][v], ai, rest);
+                        const float g = to_f32(rd.v[i].v[v]) + z[v];
+                        z[v] = ai * g;
+                        const float before = kWhole || t > 0 ? to_f32(rh.v[i].v[v]) : h0[v];
+                        one = g * rest;
+                        two = GATE == SEERA_GATE_SIGMOID ? one * (before - to_f32(rx.v[i].v[v])) * ai : g * before;
+                    }
+                    o.v[v] = from_f32<T>(kWhole || t < n ? one : 0.f);
+                    o2.v[v] = from_f32<T>(kWhole || t < n ? two : 0.f);
+                }
+                if (kWhole || u < length) {
+                    *(P*)(q + mine) = o;
+                    if (DIR == 1) *(P*)(q2 + mine2) = o2;
+                }
             }
+        };
+        if (cut) {
+            second(std::false_type{});
+            // waits for all loads and stores: after this path, whose number of stores varies, the
+            // next tile's values would else be waited for together with the stores in every path
+            __builtin_amdgcn_s_waitcnt(0x0f70);
+        } else {
+            second(std::true_type{});
         }
     };
     load_tile(0, rx, rf, rd, rh);
@@ -369,10 +378,13 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
             }
         compose(A, B, z);
     }
+    // The values loaded before the loop are waited for here: in it, a wait for them
+    // would be one for the next tile's loads too.
+#pragma unroll
+    for (int v = 0; v < V; ++v) asm volatile("" : "+v"(carry[v]), "+v"(h0[v]));
     for (int u0 = 0; u0 < length; u0 += kSteps) {
         if (u0 + kSteps < length) load_tile(u0 + kSteps, nx, nf, nd, nh);
-        if (is_whole(u0)) compute(u0, std::true_type{});
-        else compute(u0, std::false_type{});
+        compute(u0);
         rx = nx, rf = nf, rd = nd, rh = nh;
     }
     if (!active || wave || slot) return;
@@ -385,11 +397,14 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
     }
 }
 
+constexpr int kLongestTile = 1024;  // steps
+
 // Launches the tiles; parts > 1 splits time (where it is long enough) for a second
 // pass over x, f (f, dh), in exchange for that many times the blocks.
 template <class T, int V, int CL, int NT, int L, int GATE, int DIR>
 int launch_tiles(const ScanShape& s, const ScanPtrs& p, int64_t parts, hipStream_t st) {
     constexpr int kSteps = NT / CL * L;
+    static_assert(kSteps <= kLongestTile, "far_apart() counts on it");
     const unsigned groups = (s.channels + CL * V - 1) / (CL * V);
     const int64_t chains = (int64_t)groups * s.batch, states = (int64_t)s.batch * s.channels;
     const int tiles = (s.time + kSteps - 1) / kSteps;
@@ -422,13 +437,12 @@ template <class T, int V, int WV, int GATE, int DIR>
 int choose_tiles(const ScanShape& s, const ScanPtrs& p, hipStream_t st) {
     constexpr int E = (int)sizeof(T);
     constexpr int kFull = 128 / (V * E), kHalf = std::min(64, 64 / (V * E));  // lanes over 128 and 64 bytes of channels
-    constexpr int kValues = DIR == 0 ? 16 : 8;                                // a thread's, of x, f (and dh, h)
     const int64_t cus = device_cus();
     auto chains = [&](int bytes) { return (int64_t)s.batch * ((s.channels * (int64_t)E + bytes - 1) / bytes); };
     if (s.time <= 32) return launch_tiles<T, V, kFull, 128, 8 / V, GATE, DIR>(s, p, 1, st);
     if (s.time <= 128) return launch_tiles<T, V, kFull, 256, 8 / V, GATE, DIR>(s, p, 1, st);
-    if (chains(128) >= 2 * cus) return launch_tiles<T, V, kFull, 512, kValues / V, GATE, DIR>(s, p, 1, st);
-    if (chains(64) * 4 >= cus * (DIR == 0 ? 2 : 3)) return launch_tiles<T, V, kHalf, 512, kValues / V, GATE, DIR>(s, p, 1, st);
+    if (chains(128) * 4 >= cus * 3) return launch_tiles<T, V, kFull, 512, (DIR == 0 ? 16 : 8) / V, GATE, DIR>(s, p, 1, st);
+    if (chains(64) * 4 >= cus * (DIR == 0 ? 2 : 3)) return launch_tiles<T, V, kHalf, 512, (DIR == 0 ? 32 : 8) / V, GATE, DIR>(s, p, 1, st);
     const int64_t wide = chains(64 * WV * E);
     return launch_tiles<T, WV, 64, 512, 16 / WV, GATE, DIR>(s, p, (2 * cus + wide - 1) / wide, st);
 }
@@ -448,10 +462,10 @@ bool packs(const ScanShape& s, const std::initializer_list<const void*>& ptrs, c
 constexpr int kFewSteps = 8;
 
 // Whether a tile's rows may lie 2^32 bytes apart, which its 32-bit distances do not
-// reach: such a call walks each chain in one thread too. (512: steps of the longest tile.)
+// reach: such a call walks each chain in one thread too.
 template <class T>
 bool far_apart(const ScanShape& s, const std::initializer_list<int64_t>& lds) {
-    return 512.0 * (s.time_major ? s.batch : 1) * sizeof(T) * (double)std::max(std::max(lds), (int64_t)s.channels) >= 0x1p32;
+    return (double)kLongestTile * (s.time_major ? s.batch : 1) * sizeof(T) * (double)std::max(std::max(lds), (int64_t)s.channels) >= 0x1p32;
 }
 
 template <class T, int V, int WV, int GATE>
