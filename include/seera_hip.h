@@ -448,9 +448,11 @@ int seera_hip_broadcast_mul_4d(const float *A, const float *B, float *C,
  * statistics and the gradients of weights are fp32. Arithmetic, states, sums
  * and statistics are fp32; a 16-bit output is rounded once, when it is stored.
  * Pointers marked "optional" may be NULL. Pointers must be aligned to their
- * type; every other alignment, row distance and size is taken (the widest
- * loads need 16-byte aligned pointers and row distances). Outputs are
- * overwritten. The _async forms follow the workspace rule of HIP graphs
+ * type; no more alignment, and no multiple in a size or row distance, is needed
+ * (the scan moves 8 or 4 bytes a lane where pointers, row distances and channels
+ * are multiples of that, else single values). Outputs are overwritten and may
+ * not overlap inputs but where it says so. Results do not depend on timing: sums
+ * are taken in a fixed order. The _async forms follow the workspace rule of HIP graphs
  * (below): one eager call of the same sizes before a capture. */
 enum {
     SEERA_DTYPE_F32 = 0,
@@ -472,7 +474,9 @@ enum {
  *   hT       [batch, channels] fp32, the state after the last step; optional. It
  *            may be h0 itself, so that one buffer carries a generation's state
  * time == 1 is the step of a model that generates token by token; time == 0
- * copies h0 to hT. A gate of exactly 0 (f = -inf under SIGMOID) starts anew. */
+ * copies h0 to hT. A gate of exactly 0 (f = -inf under SIGMOID) starts anew.
+ * time is at most 2^30. Steps are composed before the state is known, so under
+ * LINEAR the product of the gates of a span must not overflow fp32. */
 enum { SEERA_GATE_LINEAR = 0, SEERA_GATE_SIGMOID = 1 };
 int seera_hip_gated_scan_fwd(const void *x, const void *f, const float *h0,
                              const int *lengths, void *h, float *hT, int batch,

@@ -5,8 +5,15 @@
 //   c_t = a_t (dh_t + c_{t+1}),  g_t = dh_t + c_{t+1}   (backward; dh0 = c_0)
 //
 // Both are chains of affine maps c -> A c + B, one chain per (sequence,
-// channel). The forward reads x, f and writes h; the backward reads x, f, h,
-// dh and writes dx, df: memory bound.
+// channel). The forward reads x, f and writes h (3 values an element, about 25
+// vector instructions of a lane); the backward reads x, f, h, dh and writes dx,
+// df (6 values): bytes bound both, and the problem is to have enough of them in
+// flight while a chain is serial. Measured (bf16, sigmoid, x and f slices of one
+// matrix; floors at 5.35 TB/s, a large copy's rate): 8 x 2048 x 1024 forward 27
+// us (floor 19), backward 52 (38); 16 x 2048 x 1024 44 and 88 (38, 75).
+//
+// df could be had from h_{t-1} - h_t without reading x, but that difference
+// cancels for a near 1, with a 16-bit h altogether.
 #include <algorithm>
 #include <type_traits>
 
@@ -44,7 +51,9 @@ __device__ __forceinline__ int steps_of(const int* lengths, int b, int time) {
     return lengths ? min(max(lengths[b], 0), time) : time;
 }
 
-// One thread per sequence and V channels, step by step.
+// One thread per sequence and V channels, step by step: a generation's single
+// token (64 x 1024 channels in 3 us, of which the launch is most), and the calls
+// that the tiles do not reach.
 template <class T, int V, int GATE>
 __global__ __launch_bounds__(256) void scan_fwd_steps(ScanFwd p, ScanShape s, int64_t items) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -133,7 +142,11 @@ __global__ __launch_bounds__(256) void scan_bwd_steps(ScanBwd p, ScanShape s, in
 // wave's slots (shuffles), then over the waves (shared memory), always in the
 // order of time, so a result does not depend on timing. With its carry each
 // thread then runs its steps again from registers: x, f (dh, h) are read once.
-// The next tile's loads are issued before the present one is computed.
+// The next tile's loads are issued before the present one is computed, and pass
+// the cache by (non-temporal: backward 8 x 2048 x 1024 57 -> 53 us). Two tiles
+// ahead, or more waves, gained nothing: with 256 blocks the pattern of memory (64
+// bytes of each row a block) holds it at 3.7 TB/s, where 1024 blocks of 128 bytes
+// reach 5.
 //
 // DIR 0 runs forward (maps a, b), 1 backward in time (maps a, a dh). A step's
 // place in the walk is u, from 0 at the segment's first step of the walk.
@@ -431,8 +444,20 @@ int launch_tiles(const ScanShape& s, const ScanPtrs& p, int64_t parts, hipStream
     return SEERA_OK;
 }
 
-// V: values that may be moved as one in a narrow tile (4 bytes, or one value where
-// nothing is aligned to that), WV: in a wide one.
+// Which tiles a call gets. V: values that may be moved as one in a narrow tile (4
+// bytes, or one value where nothing is aligned to that), WV: in a wide one.
+//
+//   time <= 32, 128  small blocks: 64 x 32 x 1024 forward 5.1 us, with 512 threads 11.3;
+//                    64 x 128 x 1024 12.5, with 128 threads 13.9
+//   else, by the number of blocks that whole chains give:
+//   128 bytes of channels a block from 3 blocks on 4 compute units: fp32 8 x 2048 x 1024
+//                    40 us, with 64 bytes 56; below that 64 bytes: bf16 8 x 2048 x 1024 27
+//                    us, with 128 bytes (128 blocks) 39
+//   64 bytes from 2 blocks on 4 (backward 3): at 2 on 4 the forward takes 44 us whole and
+//                    47 split, the backward 92 and 70; at 3 on 4 38 and 48, 71 and 87
+//   else time is split over about two blocks a compute unit. That reads x, f (f, dh)
+//                    twice, so the rows are as wide as lanes allow (512 bytes: fp32 1 x 65536
+//                    x 512 117 us; 128 bytes 148); whole it would take 590
 template <class T, int V, int WV, int GATE, int DIR>
 int choose_tiles(const ScanShape& s, const ScanPtrs& p, hipStream_t st) {
     constexpr int E = (int)sizeof(T);

@@ -574,6 +574,26 @@ def test_adamw_from_nothing(lib):
     assert np.array_equal(*out) and np.all(np.isfinite(out[0])) and np.array_equal(out[0][::7], p[::7])
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-12, 1e-6])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_small_eps(lib, eps, bits):
+    """Gradients down to where their squares are denormal, with an eps that keeps them
+    from mattering and without one."""
+    n = 512
+    r = np.random.default_rng(14)
+    size = np.repeat(10.0 ** np.array([-19.5, -18, -12, -3]), 128)
+    p, g = (0.1 * r.standard_normal(n)).astype(np.float32), (size * (0.5 + r.random(n)) * np.sign(r.standard_normal(n))).astype(np.float32)
+    dp, dg = DeviceBuffer.from_array(p), DeviceBuffer.from_array(g)
+    zero = [DeviceBuffer.from_array(np.zeros(4 * n, np.uint8)) for _ in range(4)]
+    t = capi.AdamwTensor(param=dp.ptr, grad=dg.ptr, m=zero[0].ptr, v=zero[1].ptr, m_exp=zero[2].ptr, v_exp=zero[3].ptr, count=n, state_bits=bits)
+    capi.call("seera_hip_adamw_step", ctypes.byref(t), 1, 1e-3, 0.9, 0.999, eps, 1, 0, None)
+    # v as fp32 holds it: a denormal has fewer bits, which the reference follows
+    m32, v32 = q.adamw_moments(np.zeros(n, np.float32), np.zeros(n, np.float32), g, 1.0, 0.9, 0.999)
+    update = 1e-3 * (m32.astype(np.float64) / (1 - 0.9)) / (np.sqrt(v32.astype(np.float64) / (1 - 0.999)) + eps)
+    got = dp.to_array(n).astype(np.float64)
+    assert np.all(np.abs(got - (p - update)) <= 16 * q.U * (np.abs(p) + np.abs(update)))
+
+
 def test_adamw_not_finite_gradients(lib):
     """Infinity and NaN reach their own parameter at once; an 8-bit block that held
     one is NaN from then on, other blocks are untouched."""
