@@ -308,8 +308,8 @@ int batches(const seera_adamw_tensor* tensors, int n, Fill&& fill, Launch&& laun
         const seera_adamw_tensor& t = tensors[i];
         if (t.count == 0) continue;
         const int64_t more = (t.count + b.chunk - 1) / b.chunk;
-        if (more > kMaxGridX) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: tensor %d is too large", i);
-        if (b.count == kMost || blocks + more > kMaxGridX) {
+        if (more >= kMaxThreads / kThreads) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: tensor %d is too large", i);
+        if (b.count == kMost || blocks + more >= kMaxThreads / kThreads) {
             launch(b, (unsigned)blocks);
             SEERA_HIP_TRY(hipGetLastError());
             b.count = 0;

@@ -441,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_rows(NormBwd p, NormShape s
 
 // out[k][c] = sum over blocks of partial[block][k][c], in a fixed order: 16
 // interleaved chains, then their sum. 32 columns a block.
-constexpr int kSumCols = 32, kSumRows = 16;
+constexpr int kSumCols = 32, kSumRows = 16, kFlight = 16;
 __global__ __launch_bounds__(kSumCols * kSumRows) void norm_bwd_sums(const float* partial, int blocks, int cols, float* dw1, float* ds, float* dw2) {
     __shared__ float part[kSumRows][kSumCols + 1];
     const int k = blockIdx.y, lane = threadIdx.x % kSumCols, chain = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + lane;
@@ -449,8 +449,14 @@ __global__ __launch_bounds__(kSumCols * kSumRows) void norm_bwd_sums(const float
     if (!out) return;
     float sum = 0.f;
     if (c < cols) {
-#pragma unroll 8
-        for (int b = chain; b < blocks; b += kSumRows) sum += partial[((int64_t)b * 3 + k) * cols + c];
+        // past the last block the last one again, not added
+        for (int b = chain; b < blocks; b += kSumRows * kFlight) {
+            float x[kFlight];
+#pragma unroll
+            for (int i = 0; i < kFlight; ++i) x[i] = partial[((int64_t)min(b + i * kSumRows, blocks - 1) * 3 + k) * cols + c];
+#pragma unroll
+            for (int i = 0; i < kFlight; ++i) sum += b + i * kSumRows < blocks ? x[i] : 0.f;
+        }
     }
     part[chain][lane] = sum;
     __syncthreads();
@@ -461,11 +467,22 @@ __global__ __launch_bounds__(kSumCols * kSumRows) void norm_bwd_sums(const float
 }
 
 template <class T, int K, int NT, int ROWS>
-int fwd_launch(const NormShape& s, const NormFwd& a, hipStream_t st) {
-    const dim3 grid((s.rows + ROWS - 1) / ROWS), block(NT * ROWS);
-    if (s.cols % Wide<T>::N) hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, true>), grid, block, 0, st, a, s);
-    else hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, false>), grid, block, 0, st, a, s);
-    SEERA_HIP_TRY(hipGetLastError());
+int fwd_launch(NormShape s, NormFwd a, hipStream_t st) {
+    // as many rows at once as a launch may have threads for
+    constexpr int kMost = (int)std::min<int64_t>(kMaxThreads / NT / 2, 1 << 30);
+    for (int left = s.rows; left > 0; left -= kMost) {
+        s.rows = std::min(left, kMost);
+        const dim3 grid((s.rows + ROWS - 1) / ROWS), block(NT * ROWS);
+        if (s.cols % Wide<T>::N) hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, true>), grid, block, 0, st, a, s);
+        else hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, false>), grid, block, 0, st, a, s);
+        SEERA_HIP_TRY(hipGetLastError());
+        auto on = [&](auto& p, int64_t ld) {
+            if (p) p = (std::decay_t<decltype(p)>)((char*)p + s.rows * ld);
+        };
+        on(a.y, a.ldy * sizeof(T)), on(a.g, a.ldg * sizeof(T));
+        on(a.r, s.cols * sizeof(T)), on(a.r_out, s.cols * sizeof(T)), on(a.n_out, s.cols * sizeof(T));
+        on(a.rstd1, sizeof(float)), on(a.rstd2, sizeof(float));
+    }
     return SEERA_OK;
 }
 

@@ -11,6 +11,9 @@
 
 namespace seera {
 
+// Threads that one launch may have along an axis.
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;
+
 // Rows of a [batch, time] matrix of `channels` values, `ld` elements apart;
 // row (b, t) is b * time + t, or t * batch + b where time_major.
 struct ScanShape {
