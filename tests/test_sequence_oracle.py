@@ -232,6 +232,14 @@ def test_adamw_values_refusals():
     _refused("seera_hip_adamw_state_values", (_tensor(), 1, two, (ctypes.c_void_p * 1)(P + 2)), "aligned")
 
 
+def test_sizes_that_no_launch_reaches_are_refused():
+    for time in (1, 20, 500):
+        _refused("seera_hip_gated_scan_fwd_async", (P, P, P, None, P, P, 1 << 30, time, 2048, 2048, 2048, 1, 0, 0, None), "too large")
+        _refused("seera_hip_gated_scan_bwd_async", (P, P, P, None, P, P, P, P, P, P, 1 << 30, time, 2048, *[2048] * 4, 1, 0, 0, None), "too large")
+    _refused("seera_hip_gated_scan_fwd_async", (P, P, P, None, P, P, 2, (1 << 30) + 1, 8, 8, 8, 1, 0, 0, None), "time")
+    _refused("seera_hip_adamw_step_async", (_tensor(count=1 << 50), 1, 1e-3, 0.9, 0.999, 1e-8, 1, 0, None, None), "too large")
+
+
 def test_nothing_to_do_needs_no_pointers():
     lib = capi.load()
     for dims in ((0, 3, 8), (2, 3, 0)):
