@@ -449,11 +449,11 @@ int launch_tiles(const ScanShape& s, const ScanPtrs& p, int64_t parts, hipStream
 //   128 bytes of channels a block from 3 blocks on 4 compute units: fp32 8 x 2048 x 1024
 //                    40 us, with 64 bytes 56; below that 64 bytes: bf16 8 x 2048 x 1024 27
 //                    us, with 128 bytes (128 blocks) 39
-//   64 bytes from 2 blocks on 4 (backward 3): at 2 on 4 the forward takes 44 us whole and
-//                    47 split, the backward 92 and 70; at 3 on 4 38 and 48, 71 and 87
-//   else time is split over about two blocks a compute unit. That reads x, f (f, dh)
-//                    twice, so the rows are as wide as lanes allow (512 bytes: fp32 1 x 65536
-//                    x 512 117 us; 128 bytes 148); whole it would take 590
+//   64 bytes from 5 blocks on 8, and for short chains: bf16 5 x 4096 x 1024 46 and 92 us,
+//                    split 56 and 97; 4 x 300 x 1024 7.8 and 9.4, split 10.4 and 11.7
+//   else time is split over about two blocks a compute unit: 4 x 4096 x 1024 40 and 61 us,
+//                    whole 45 and 88. That reads x, f (f, dh) twice, in rows of 64 lanes
+//                    (bf16 256 bytes: 1 x 4096 x 1024 16.6 us, of four values a lane 21.5)
 template <class T, int V, int WV, int GATE, int DIR>
 int choose_tiles(const ScanShape& s, const ScanPtrs& p, hipStream_t st) {
     constexpr int E = (int)sizeof(T);
@@ -463,9 +463,10 @@ int choose_tiles(const ScanShape& s, const ScanPtrs& p, hipStream_t st) {
     if (s.time <= 32) return launch_tiles<T, V, kFull, 128, 8 / V, GATE, DIR>(s, p, 1, st);
     if (s.time <= 128) return launch_tiles<T, V, kFull, 256, 8 / V, GATE, DIR>(s, p, 1, st);
     if (chains(128) * 4 >= cus * 3) return launch_tiles<T, V, kFull, 512, (DIR == 0 ? 16 : 8) / V, GATE, DIR>(s, p, 1, st);
-    if (chains(64) * 4 >= cus * (DIR == 0 ? 2 : 3)) return launch_tiles<T, V, kHalf, 512, (DIR == 0 ? 32 : 8) / V, GATE, DIR>(s, p, 1, st);
+    if (s.time <= 512 || chains(64) * 8 >= cus * 5) return launch_tiles<T, V, kHalf, 512, (DIR == 0 ? 32 : 8) / V, GATE, DIR>(s, p, 1, st);
     const int64_t wide = chains(64 * WV * E);
-    return launch_tiles<T, WV, 64, 512, 16 / WV, GATE, DIR>(s, p, (2 * cus + wide - 1) / wide, st);
+    constexpr int kValues = DIR == 0 && E == 2 ? 16 : 8;
+    return launch_tiles<T, WV, 64, 512, kValues / WV, GATE, DIR>(s, p, (2 * cus + wide - 1) / wide, st);
 }
 
 // Whether V values of T may be moved as one: sizes, row distances and addresses.
@@ -515,14 +516,13 @@ int bwd_v(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
     return choose_tiles<T, V, WV, GATE, 1>(s, p, st);
 }
 
-// The widest of 8 and 4 bytes a lane that everything is aligned to, or one value.
+// Two values a lane where everything is aligned to pairs (fp32 narrow tiles take one).
 template <class T, int GATE>
 int fwd_t(const ScanShape& s, const ScanFwd& a, hipStream_t st) {
     constexpr int E = (int)sizeof(T);
     const auto ptrs = {a.x, a.f, (const void*)a.h};
     const auto lds = {a.ldx, a.ldf};
-    if (packs<T, 8 / E>(s, ptrs, lds)) return fwd_v<T, 4 / E, 8 / E, GATE>(s, a, st);
-    if (E == 2 && packs<T, 4 / E>(s, ptrs, lds)) return fwd_v<T, 4 / E, 4 / E, GATE>(s, a, st);
+    if (packs<T, 2>(s, ptrs, lds)) return fwd_v<T, 4 / E, 2, GATE>(s, a, st);
     return fwd_v<T, 1, 1, GATE>(s, a, st);
 }
 template <class T, int GATE>
@@ -530,8 +530,7 @@ int bwd_t(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
     constexpr int E = (int)sizeof(T);
     const auto ptrs = {GATE == SEERA_GATE_LINEAR ? a.f : a.x, a.f, a.h, a.dh, (const void*)a.dx, (const void*)a.df};
     const auto lds = {GATE == SEERA_GATE_LINEAR ? a.ldf : a.ldx, a.ldf, a.lddx, a.lddf};
-    if (packs<T, 8 / E>(s, ptrs, lds)) return bwd_v<T, 4 / E, 8 / E, GATE>(s, a, st);
-    if (E == 2 && packs<T, 4 / E>(s, ptrs, lds)) return bwd_v<T, 4 / E, 4 / E, GATE>(s, a, st);
+    if (packs<T, 2>(s, ptrs, lds)) return bwd_v<T, 4 / E, 2, GATE>(s, a, st);
     return bwd_v<T, 1, 1, GATE>(s, a, st);
 }
 template <class T>
