@@ -449,8 +449,8 @@ int seera_hip_broadcast_mul_4d(const float *A, const float *B, float *C,
  * and statistics are fp32; a 16-bit output is rounded once, when it is stored.
  * Pointers marked "optional" may be NULL. Pointers must be aligned to their
  * type; no more alignment, and no multiple in a size or row distance, is needed
- * (the scan moves 8 or 4 bytes a lane where pointers, row distances and channels
- * are multiples of that, else single values). Outputs are overwritten and may
+ * (the scan moves two values a lane where pointers, row distances and channels
+ * are multiples of two values, else one). Outputs are overwritten and may
  * not overlap inputs but where it says so. Results do not depend on timing: sums
  * are taken in a fixed order. The _async forms follow the workspace rule of HIP graphs
  * (below): one eager call of the same sizes before a capture. */

@@ -6,8 +6,8 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 //
 // Bytes bound: 28 a value with fp32 states and gradients, 16 with 8-bit states,
-// bf16 gradients and a bf16 copy. 97 tensors of 97.6 M values: 496 us (5.7 TB/s; a
-// large copy makes 5.35); with 8 bits, and the values read out (10 bytes), 474 us.
+// bf16 gradients and a bf16 copy. 97 tensors of 97.6 M values: 490 us (5.8 TB/s; a
+// large copy makes 5.35); with 8 bits, and the values read out (10 bytes), 463 us.
 //
 // Codes. v moves by a thousandth of itself in a step and a code's place is an
 // eighth: rounded to nearest, v would never fall (a run on a noisy quadratic left
@@ -55,8 +55,9 @@ __device__ __forceinline__ uint32_t shared_exponent(uint32_t largest) { return l
 
 // What a launch works on: up to kMost tensors (3.9 of the 4 KB that arguments may take) in the kernel's arguments, so that
 // a step needs no copy to the device and may be captured in a graph. Thread block
-// b works on values [(b - first) * chunk, ...) of the last tensor with first <= b.
-constexpr int kMost = 48, kThreads = 256;
+// b works on values [(b - first) * kChunk, ...) of the last tensor with first <= b:
+// 2048 values (0.54 M values 7.5 us, in shares of 4096 8.7; 97.6 M with 8 bits 475, 491).
+constexpr int kMost = 48, kThreads = 256, kChunk = kThreads * 8;
 struct Slot {
     float* param;      // adamw_values: where m's values go
     const void* grad;  // adamw_values: where v's values go
@@ -71,7 +72,7 @@ struct Batch {
     Slot slot[kMost];
     unsigned first[kMost];
     uint8_t bits[kMost], grad_dtype[kMost], copy[kMost];
-    int count, chunk;  // chunk: a multiple of kThreads * 8
+    int count;
 };
 
 // The block's slot, by one comparison in each of 48 lanes.
@@ -177,8 +178,8 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
     const int at = slot_of(b);
     const Slot t = b.slot[at];
     const int bits = b.bits[at], dtype = b.grad_dtype[at], copy = b.copy[at];
-    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * b.chunk;
-    const int64_t end = min(begin + b.chunk, t.count);
+    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * kChunk;
+    const int64_t end = min(begin + kChunk, t.count);
     const float scale = s.grad_scale ? *s.grad_scale : 1.f;
     if (bits == 32) {
         constexpr int N = 4;
@@ -246,8 +247,8 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
 __global__ __launch_bounds__(kThreads) void adamw_values(Batch b) {
     const int at = slot_of(b);
     const Slot t = b.slot[at];
-    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * b.chunk;
-    const int64_t end = min(begin + b.chunk, t.count);
+    const int64_t begin = (int64_t)(blockIdx.x - b.first[at]) * kChunk;
+    const int64_t end = min(begin + kChunk, t.count);
     float *m_out = t.param, *v_out = (float*)t.grad;
     if (b.bits[at] == 32) {
         constexpr int N = 4;
@@ -299,15 +300,12 @@ __global__ __launch_bounds__(kThreads) void adamw_values(Batch b) {
 template <class Fill, class Launch>
 int batches(const seera_adamw_tensor* tensors, int n, Fill&& fill, Launch&& launch) {
     Batch b;
-    int64_t blocks = 0, total = 0;
-    for (int i = 0; i < n; ++i) total += tensors[i].count;
+    int64_t blocks = 0;
     b.count = 0;
-    // small models: smaller shares, so that every compute unit has one (0.54 M values 7.5 us, 8.7 in shares of 4096)
-    b.chunk = total < 16384 * (int64_t)device_cus() ? 2048 : 4096;
     for (int i = 0; i < n; ++i) {
         const seera_adamw_tensor& t = tensors[i];
         if (t.count == 0) continue;
-        const int64_t more = (t.count + b.chunk - 1) / b.chunk;
+        const int64_t more = (t.count + kChunk - 1) / kChunk;
         if (more >= kMaxThreads / kThreads) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: tensor %d is too large", i);
         if (b.count == kMost || blocks + more >= kMaxThreads / kThreads) {
             launch(b, (unsigned)blocks);
