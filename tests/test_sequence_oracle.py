@@ -226,6 +226,16 @@ def test_adamw_refuses_constants(change, what):
     _refused("seera_hip_adamw_step_async", list({**base, **change}.values()) + [None], what)
 
 
+def test_adamw_tensor_layout():
+    """The ctypes structure, field by field, against the header's (natural alignment,
+    no padding): a host buffer of the same layout may stand for an array of them."""
+    names = ["param", "grad", "m", "v", "m_exp", "v_exp", "param16", "count", "weight_decay", "grad_dtype", "param16_dtype", "state_bits", "reserved"]
+    offsets = [8 * i for i in range(9)] + [72, 76, 80, 84]
+    assert [getattr(capi.AdamwTensor, n).offset for n in names] == offsets and ctypes.sizeof(capi.AdamwTensor) == 88
+    body = open(capi.HEADER).read().split("typedef struct seera_adamw_tensor {")[1].split("}")[0]
+    assert [line.split()[-1].strip("*;") for line in body.strip().splitlines()] == names
+
+
 def test_adamw_values_refusals():
     two = (ctypes.c_void_p * 1)(P)
     _refused("seera_hip_adamw_state_values", (_tensor(), 1, None, two), "null array")
