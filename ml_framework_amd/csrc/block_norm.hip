@@ -17,6 +17,7 @@
 #include "io_types.h"
 #include "runtime.h"
 #include "sequence.h"
+#include "sequence_rules.h"
 
 namespace seera {
 namespace {
@@ -38,14 +39,14 @@ __device__ __forceinline__ float wave_sum(float v) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// The sum over the NT threads of a row. Consecutive calls use alternating halves
-// of `part`, so one barrier each is enough.
+// The sum over the NT threads of a row, with one barrier: `halves` is the block's
+// own, kept over all of its sums.
 template <int NT>
-__device__ __forceinline__ float row_sum(float v, float* part, int half) {
+__device__ __forceinline__ float row_sum(float v, float* part, Halves& halves) {
     v = wave_sum(v);
     if (NT == 64) return v;
     constexpr int W = NT / 64;
-    float* at = part + half * W;
+    float* at = part + halves.next() * W;
     if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = 0.f;
@@ -143,6 +144,7 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
     constexpr int N = Wide<T>::N;
     typedef Place<N, CUT> At;
     __shared__ float part[2 * (NT / 64) * ROWS];
+    Halves halves;
     const int tid = threadIdx.x % NT;
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT;
     if (ROWS > 1 && row >= s.rows) return;  // whole waves: such rows take no barrier
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
             for (int i = 0; i < N; ++i) own = fmaf(to_f32(y[k].v[i]), at.mine(i, to_f32(y[k].v[i])), own);
             sum += at.part(own);
         }
-        rstd1 = rsqrtf(row_sum<NT>(sum, part, 0) / s.cols + p.eps);
+        rstd1 = rsqrtf(row_sum<NT>(sum, part, halves) / s.cols + p.eps);
         if (p.rstd1 && tid == 0) p.rstd1[row] = rstd1;
     }
     float sum = 0.f;
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
 #pragma unroll
         for (int k = 0; k < K; ++k) store_wide((T*)p.r_out + row * s.cols, place(k), y[k]);
     if (!p.w2) return;
-    const float rstd2 = rsqrtf(row_sum<NT>(sum, part, 1) / s.cols + p.eps);
+    const float rstd2 = rsqrtf(row_sum<NT>(sum, part, halves) / s.cols + p.eps);
     if (p.rstd2 && tid == 0) p.rstd2[row] = rstd2;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -237,6 +239,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
     constexpr int N = Wide<T>::N;
     typedef Place<N, CUT> At;
     __shared__ float part[2 * (NT / 64)];
+    Halves halves;  // over the rows: a row may have one sum or two
     const bool inner = p.w1 || p.g || p.s;
     float h1[K][N], hs[K][N], h2[K][N], sum1[K][N], sums[K][N], sum2[K][N];
     auto place = [&](int k) { return At((int)(k * NT + threadIdx.x) * N, s.cols); };
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
                 }
                 dot += at.part(own);
             }
-            dot = row_sum<NT>(dot, part, 0) * inv;
+            dot = row_sum<NT>(dot, part, halves) * inv;
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
             }
         }
         if (p.w1) {
-            dot = row_sum<NT>(dot, part, 1) * inv;
+            dot = row_sum<NT>(dot, part, halves) * inv;
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll

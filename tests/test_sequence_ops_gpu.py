@@ -393,6 +393,15 @@ def test_norm_sizes(lib, dtype, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("parts", ["w2", "r w2", "g w1", "s r", "g r s w2"])
+@pytest.mark.parametrize("rows,cols", [(1500, 2048), (700, 1024), (700, 1502), (600, 5002)])
+def test_norm_parts_over_many_rows(lib, dtype, parts, rows, cols):
+    """Several rows a block and several waves a row, with one of the two norms or
+    none: the sums of consecutive rows share memory."""
+    _check_norm(lib, rows, cols, dtype, parts, silu=cols != 1024, seed=cols)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("gap,shift", [(0, 1), (1, 0), (2, 2), (8, 0), (64, 4)])
 def test_norm_layouts(lib, dtype, gap, shift):
     _check_norm(lib, 6, 264, dtype, "g r w1 s w2", gap=gap, shift=shift)
