@@ -20,6 +20,7 @@
 #include "io_types.h"
 #include "runtime.h"
 #include "sequence.h"
+#include "sequence_rules.h"
 
 namespace seera {
 namespace {
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, cl = lane % CL, slot = lane / CL;
     const int segment = DIR == 0 ? (int)part : seg.count - 1 - (int)part;
     const int begin = segment * seg.steps, end = min(begin + seg.steps, s.time), length = end - begin;
-    const int n = steps_of(p.lengths, b, s.time);
+    const Walk walk = walk_of(DIR == 1, begin, end, steps_of(p.lengths, b, s.time));
     const int channel = (group * CL + cl) * V;
     const bool active = channel < s.channels;
     // lanes past the last channel do that channel's work again: same loads, same values, same stores
@@ -197,9 +198,9 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
     const int first = (wave * SL + slot) * L;  // of the thread's steps in a tile
 
     // Addresses: the row of a tile's step i is uniform but for the thread's first
-    // step, whose distance is 32 bits (launch_tiles sees to it). In a tile that is
-    // not whole, steps past the segment's end repeat its last, or are not loaded where
-    // a thread has none before it.
+    // step, whose distance is 32 bits (far_apart sees to it). In a tile that is not
+    // whole, a thread's steps outside of the sequence repeat its live one next to them,
+    // and a thread without a live step loads nothing.
     const int64_t dir = DIR == 0 ? 1 : -1;
     auto low_row = [&](int u0) { return row0 + (int64_t)(DIR == 0 ? begin + u0 : end - u0 - kSteps) * step; };
     const unsigned from_low = DIR == 0 ? first : kSteps - 1 - first;
@@ -216,22 +217,17 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
         } else {
 #pragma unroll
             for (int i = 0; i < L; ++i) to.v[i] = P{};
-            if (u0 + first >= length) return;
+            if (!walk.any(u0 + first, L)) return;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const int u = min(u0 + first + i, length - 1), t = max((DIR == 0 ? begin + u : end - 1 - u) - shift, 0);
+                const int t = max(walk.time_of(walk.nearest(u0 + first + i)) - shift, 0);
                 to.v[i] = *(const P*)((const char*)base + ((row0 + t * step) * ld + c) * (int64_t)sizeof(T));
             }
         }
     };
     constexpr bool kNeedX = DIR == 0 || (!MAPS && GATE == SEERA_GATE_SIGMOID), kNeedH = DIR == 1 && !MAPS;
-    // inside the segment, the sequence, and (for h one step before) past its first step
-    auto is_whole = [&](int u0) {
-        if (u0 + kSteps > length) return false;
-        return DIR == 0 ? begin + u0 + kSteps <= n : end - u0 <= n && end - u0 - kSteps > 0;
-    };
     auto load_tile = [&](int u0, S& x, S& f, S& d, S& h) {
-        const bool whole = is_whole(u0);
+        const bool whole = walk.whole(u0, kSteps);
         load(p.f, p.ldf, u0, 0, whole, f);
         if (kNeedX) load(p.x, p.ldx, u0, 0, whole, x);
         if (DIR == 1) load(p.dh, s.channels, u0, 0, whole, d);
@@ -290,13 +286,12 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
     };
     S rx, rf, rd, rh, nx, nf, nd, nh;
     auto compute = [&](int u0) {
-        const bool cut = !is_whole(u0);
+        const bool cut = !walk.whole(u0, kSteps);
         if (cut) {
             // steps outside: a = 1 and nothing added
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const int u = u0 + first + i;
-                if (u < length && (DIR == 0 ? begin + u : end - 1 - u) < n) continue;
+                if (walk.live(u0 + first + i)) continue;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     rf.v[i].v[v] = from_f32<T>(GATE == SEERA_GATE_LINEAR ? 1.f : __builtin_inff());
@@ -340,7 +335,7 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
             constexpr bool kWhole = decltype(whole_tile)::value;
 #pragma unroll
             for (int i = 0; i < L; ++i, q += stride, q2 += stride2) {
-                const int u = u0 + first + i, t = DIR == 0 ? begin + u : end - 1 - u;
+                const int u = u0 + first + i;
                 P o, o2;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
@@ -352,12 +347,12 @@ __global__ __launch_bounds__(NT) void scan_tiles(ScanPtrs p, ScanShape s, Segmen
                         sides<GATE>(to_f32(rf.v[i].v[v]), m[i][v], ai, rest);
                         const float g = to_f32(rd.v[i].v[v]) + z[v];
                         z[v] = ai * g;
-                        const float before = kWhole || t > 0 ? to_f32(rh.v[i].v[v]) : h0[v];
+                        const float before = kWhole || walk.time_of(u) > 0 ? to_f32(rh.v[i].v[v]) : h0[v];
                         one = g * rest;
                         two = GATE == SEERA_GATE_SIGMOID ? one * (before - to_f32(rx.v[i].v[v])) * ai : g * before;
                     }
-                    o.v[v] = from_f32<T>(kWhole || t < n ? one : 0.f);
-                    o2.v[v] = from_f32<T>(kWhole || t < n ? two : 0.f);
+                    o.v[v] = from_f32<T>(kWhole || walk.live(u) ? one : 0.f);
+                    o2.v[v] = from_f32<T>(kWhole || walk.live(u) ? two : 0.f);
                 }
                 if (kWhole || u < length) {
                     *(P*)(q + mine) = o;

@@ -47,8 +47,46 @@ static void sums_of_a_row() {
         }
 }
 
+// The rows that a block's threads load, as scan_tiles asks for them: tiles of
+// threads * per steps, in a whole tile each step's own row, else the nearest live
+// step's; and, with shift 1 (backward, h), the row before it.
+static void rows_of_a_walk() {
+    // planted: bounds by the segment alone load rows that a length leaves out
+    const Walk planted = walk_of(false, 0, 64, 64);
+    if (planted.time_of(planted.nearest(40)) < 20) ++bad, std::printf("a planted bound by the segment is not seen\n");
+    struct Tile {
+        int threads, per;
+    };
+    for (const Tile tile : {Tile{4, 8}, Tile{32, 4}, Tile{1, 16}, Tile{16, 1}})
+        for (int time : {1, 2, 31, 32, 33, 100, 257})
+            for (int steps : {time, 32, 64})  // of a segment
+                for (int begin = 0; begin < time; begin += steps)
+                    for (int n = 0; n <= time; ++n)
+                        for (int back = 0; back < 2; ++back) {
+                            const int end = begin + steps < time ? begin + steps : time, k = tile.threads * tile.per;
+                            const Walk walk = walk_of(back, begin, end, n);
+                            for (int u0 = 0; u0 < walk.length(); u0 += k)
+                                for (int first = u0; first < u0 + k; first += tile.per)
+                                    for (int u = first; u < first + tile.per; ++u) {
+                                        const int own = back ? end - 1 - u : begin + u;
+                                        const bool inside = own >= begin && own < end && own < n, whole = walk.whole(u0, k);
+                                        bool right = walk.live(u) == inside && (!whole || inside);
+                                        if (whole || walk.any(first, tile.per)) {
+                                            const int at = whole ? own : walk.time_of(walk.nearest(u)), before = whole ? at - 1 : at > 0 ? at - 1 : 0;
+                                            right = right && at >= begin && at < end && at < n && (!inside || at == own);
+                                            right = right && (!back || (before >= 0 && before < n));
+                                        } else {
+                                            right = right && !inside;
+                                        }
+                                        if (!right && bad++ < 5)
+                                            std::printf("walk: time %d segment %d..%d n %d back %d u0 %d first %d u %d\n", time, begin, end, n, back, u0, first, u);
+                                    }
+                        }
+}
+
 int main() {
     sums_of_a_row();
+    rows_of_a_walk();
     if (!bad) std::puts("all checks passed");
     return bad != 0;
 }
