@@ -96,8 +96,9 @@ struct Place {
     }
     __device__ bool whole() const { return lo == 0 && (!CUT || hi == N); }
     __device__ bool own(int i) const { return CUT ? i >= lo && i < hi : lo == 0; }
-    // x in a sum: 0 where value i is not the pack's own
-    __device__ float mine(int i, float x) const { return !CUT || own(i) ? x : 0.f; }
+    // sum + a b, of value i: not added where it is not the pack's own (a factor of 0 would
+    // make an infinity there a NaN)
+    __device__ float add(int i, float a, float b, float sum) const { return !CUT || own(i) ? fmaf(a, b, sum) : sum; }
     // a pack's part of a sum
     __device__ float part(float x) const { return CUT || lo == 0 ? x : 0.f; }
 };
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
             const At at = place(k);
             float own = 0.f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) own = fmaf(to_f32(y[k].v[i]), at.mine(i, to_f32(y[k].v[i])), own);
+            for (int i = 0; i < N; ++i) own = at.add(i, to_f32(y[k].v[i]), to_f32(y[k].v[i]), own);
             sum += at.part(own);
         }
         rstd1 = rsqrtf(row_sum<NT>(sum, part, halves) / s.cols + p.eps);
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             y[k].v[i] = from_f32<T>(u[i]);  // as it is kept
-            own = fmaf(to_f32(y[k].v[i]), at.mine(i, to_f32(y[k].v[i])), own);
+            own = at.add(i, to_f32(y[k].v[i]), to_f32(y[k].v[i]), own);
         }
         sum += at.part(own);
     }
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
                 for (int i = 0; i < N; ++i) {
                     const float hat = to_f32(now.r[k].v[i]) * now.rstd2, dn = to_f32(now.n[k].v[i]);
                     sum2[k][i] = fmaf(dn, hat, sum2[k][i]);
-                    own = fmaf(dn * h2[k][i], at.mine(i, hat), own);
+                    own = at.add(i, dn * h2[k][i], hat, own);
                 }
                 dot += at.part(own);
             }
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
                     const float hat = to_f32(now.y[k].v[i]) * now.rstd1;
                     sum1[k][i] = fmaf(d[k][i], hat, sum1[k][i]);
                     d[k][i] *= h1[k][i];
-                    own = fmaf(d[k][i], at.mine(i, hat), own);
+                    own = at.add(i, d[k][i], hat, own);
                 }
                 dot += at.part(own);
             }

@@ -456,6 +456,39 @@ def test_norm_nan_stays_in_its_row(lib):
         assert np.all(np.isnan(got[k][2])) and np.all(np.isfinite(np.delete(got[k], 2, 0)))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [8, 9, 77, 203, 1501, 2051, 5001, 9003])
+def test_norm_infinities_at_a_rows_end(lib, dtype, cols):
+    """An infinity in one of the last columns, where a row's last loads reach into
+    each other at an odd width: the row's norm is 1 / infinity, so that its other
+    values are 0; backward its mean is infinite and the row's gradients with it."""
+    rows = 12
+    at = [cols - 1 - min(i, cols - 1) for i in range(rows - 3)]  # three rows without
+    for parts, forward, backward in (("r w2", "y", "dn"), ("g w1", "y", "dr_out")):
+        d = _norm_data(rows, cols, dtype, parts, cols)
+        for row, c in enumerate(at):
+            d[forward][row, c] = np.inf if row % 2 else -np.inf
+        with np.errstate(invalid="ignore"):
+            ref, bound = q.norm_fwd(**{k: d[k] for k in ("y", "g", "r", "w1") if k in d})
+            got = _norm_forward(lib, d, dtype, True)
+            if "w2" in d:
+                more, more_bound = q.norm_next(got["r_out"], d["w2"])
+                ref.update(more)
+                bound.update(more_bound)
+        for k in got:
+            _close(got[k], ref[k], bound[k], dtype if k in ("r_out", "n_out") else q.F32, k)
+        d = _norm_data(rows, cols, dtype, parts, cols)
+        kept = _norm_forward(lib, d, dtype, True)
+        for row, c in enumerate(at):
+            d[backward][row, c] = np.inf if row % 2 else -np.inf
+        with np.errstate(invalid="ignore"):
+            refs, bounds = q.norm_bwd(d["y"], d.get("g"), kept["r_out"], d.get("w1"), None, d.get("w2"), kept.get("rstd1"), kept.get("rstd2"),
+                                      d["dr_out"], d["dn"] if "w2" in d else None)
+        gots = _norm_backward(lib, d, kept, dtype, True)
+        for k in gots:
+            _close(gots[k], refs[k], bounds[k], q.F32 if k[1:] in ("w1", "s", "w2") else dtype, k)
+
+
 def test_norm_in_place(lib):
     """r_out over r, dr over dr_out: the results of separate buffers."""
     rows, cols = 40, 512
