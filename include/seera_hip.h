@@ -593,7 +593,10 @@ typedef struct seera_adamw_tensor {
  *   m = beta1 m + (1 - beta1) g      v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr weight_decay)
  *           - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
- * param takes m and v as computed, before they are rounded to 8 bits. */
+ * param takes m and v as computed, before they are rounded to 8 bits. The update
+ * is of fp32 operations, each rounded correctly, in the order written here with
+ * lr / (1 - beta1^t) and 1 / sqrt(1 - beta2^t) as factors (with 8-bit states a root
+ * of v or a quotient of lr m below 2^-101 may be off by a unit in the last place). */
 int seera_hip_adamw_step(const seera_adamw_tensor *tensors, int n, double lr,
                          double beta1, double beta2, double eps, int64_t step,
                          uint32_t seed, const float *grad_scale);

@@ -150,10 +150,32 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
 }
 
-// N values of the step: the moments and the parameter. PLAIN: correctly rounded
-// square root and quotient; else the hardware's, off by a unit in the last place
-// of the update: with 8-bit states the instructions count (99 a value, three
-// quarters of the step's 335 us for 97.6 M values; so 75 a value and 295 us).
+// The square root, rounded correctly from v = 2^-101 on: the hardware's is off by a
+// unit at most, and the residuals of its two neighbours say which is nearest (all
+// 2^24 values of [1, 4) checked). 0, infinity and NaN pass through; below 2^-101 the
+// residuals lose bits, and the hardware takes denormals for 0.
+__device__ __forceinline__ float root_of(float v) {
+    const float s = __builtin_amdgcn_sqrtf(v);
+    const float down = __uint_as_float(__float_as_uint(s) - 1), up = __uint_as_float(__float_as_uint(s) + 1);
+    const float below = fmaf(-down, s, v), above = fmaf(-up, s, v);
+    const float r = below <= 0.f ? down : s;
+    return above > 0.f ? up : r;
+}
+// a / b, rounded correctly for a b whose reciprocal is normal and an a of 0 or from
+// 2^-101 on: with a correctly rounded reciprocal (one Newton step on the hardware's;
+// all 2^23 fractions checked) one step on the quotient rounds it correctly (Markstein
+// 1990).
+__device__ __forceinline__ float quotient_of(float a, float b) {
+    float r = __builtin_amdgcn_rcpf(b);
+    r = fmaf(fmaf(-b, r, 1.f), r, r);
+    const float q = a * r;
+    return __builtin_amdgcn_div_fixupf(fmaf(fmaf(-b, q, a), r, q), b, a);
+}
+
+// N values of the step: the moments and the parameter, each operation rounded
+// correctly. PLAIN: for every v and eps; else root_of and quotient_of, for the 8-bit
+// states, whose instructions count (97.6 M values with their reading out 472 us,
+// PLAIN 484; the hardware's root and reciprocal alone, off by a unit, 465).
 template <bool PLAIN, int N>
 __device__ __forceinline__ void update(const AdamwStep& s, float keep, float scale, const float (&g)[N], float (&m)[N], float (&v)[N], float (&p)[N]) {
 #pragma unroll
@@ -161,8 +183,9 @@ __device__ __forceinline__ void update(const AdamwStep& s, float keep, float sca
         const float gk = g[k] * scale;
         m[k] = m[k] * s.beta1 + gk * s.one_minus_beta1;
         v[k] = v[k] * s.beta2 + (gk * gk) * s.one_minus_beta2;
-        if (PLAIN) p[k] = p[k] * keep - s.step_size * m[k] / (sqrtf(v[k]) * s.inv_sqrt_corr2 + s.eps);
-        else p[k] = p[k] * keep - s.step_size * m[k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[k]) * s.inv_sqrt_corr2 + s.eps);
+        const float size = s.step_size * m[k];
+        if (PLAIN) p[k] = p[k] * keep - size / (sqrtf(v[k]) * s.inv_sqrt_corr2 + s.eps);
+        else p[k] = p[k] * keep - quotient_of(size, root_of(v[k]) * s.inv_sqrt_corr2 + s.eps);
     }
 }
 
@@ -173,7 +196,8 @@ __device__ __forceinline__ void store_params(const Slot& t, int copy, int64_t i,
     else if (copy == SEERA_DTYPE_BF16) store_rounded<bf16_t>(t.param16, i, p, live);
 }
 
-template <bool PLAIN>
+// PLAIN8: update's PLAIN for the 8-bit states.
+template <bool PLAIN8>
 __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
     const int at = slot_of(b);
     const Slot t = b.slot[at];
@@ -191,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
             load_some<true>(m, t.m, i, live);
             load_some<true>(v, t.v, i, live);
             load_some<true>(p, t.param, i, live);
-            update<PLAIN>(s, t.keep, scale, g, m, v, p);
+            update<true>(s, t.keep, scale, g, m, v, p);
             store_some(t.m, i, m, live);
             store_some(t.v, i, v, live);
             store_params(t, copy, i, p, live);
@@ -216,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void adamw_many(Batch b, AdamwStep s) {
             if (cm[k] & 128) m[k] = -m[k];
             v[k] = decode(cv[k], ev, 31);
         }
-        update<PLAIN>(s, t.keep, scale, g, m, v, p);
+        update<PLAIN8>(s, t.keep, scale, g, m, v, p);
         store_params(t, copy, i, p, live);
         uint32_t am = 0, av = 0;
 #pragma unroll
@@ -340,9 +364,9 @@ int adamw_step(const seera_adamw_tensor* tensors, int n, const AdamwStep& step, 
             s.key = mix((uint32_t)i * 0x9E3779B9u + step.seed);
         },
         [&](const Batch& b, unsigned blocks) {
-            // the hardware's square root takes denormals (below 1.2e-38) for 0: that is lost in
-            // an eps from 1e-10 on, and would divide by 0 without one
-            if (step.eps >= 1e-10f) hipLaunchKernelGGL(adamw_many<false>, dim3(blocks), dim3(kThreads), 0, st, b, step);
+            // root_of takes denormals (roots below 1.1e-19) for 0: rounded away where they are added
+            // to an eps of 2^25 times that
+            if (step.eps >= 3.7e-12f * step.inv_sqrt_corr2) hipLaunchKernelGGL(adamw_many<false>, dim3(blocks), dim3(kThreads), 0, st, b, step);
             else hipLaunchKernelGGL(adamw_many<true>, dim3(blocks), dim3(kThreads), 0, st, b, step);
         });
 }

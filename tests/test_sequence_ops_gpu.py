@@ -590,6 +590,32 @@ def test_adamw_tensors(lib, bits, grad_dtype, copy, shift):
         t.check(0.37, **CONSTANTS, step=step, seed=77 + step)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("grad_dtype", DTYPES)
+@pytest.mark.parametrize("eps", [1e-8, 1e-30])
+@pytest.mark.parametrize("decay", [0.0, 0.01])
+def test_adamw_rounds_correctly(lib, bits, grad_dtype, eps, decay):
+    """The parameter is that of fp32 operations, each rounded correctly, bit for bit,
+    with states of either kind."""
+    one = np.float32
+    n, lr, beta1, beta2, scale = 20000, 3e-3, 0.9, 0.999, one(0.37)
+    t = Tensors([n], bits, grad_dtype, 0, 21, decay=decay)
+    device_scale = DeviceBuffer.from_array(np.array([scale], np.float32))
+    for step in (1, 2, 50):
+        h, d = t.host[0], t.dev[0]
+        g = q.load(h["g"], grad_dtype).astype(np.float32)
+        capi.call("seera_hip_adamw_step", t.table, 1, lr, beta1, beta2, eps, step, step, device_scale.ptr)
+        m, v = q.adamw_moments(h["m"], h["v"], g, scale, beta1, beta2)
+        size, root = one(lr / (1 - beta1**step)), one(1 / np.sqrt(1 - beta2**step))
+        want = h["p"] * one(1 - lr * h["decay"]) - size * m / (np.sqrt(v) * root + one(eps))
+        assert want.dtype == np.float32
+        assert np.array_equal(d["p"].raw()[0].view(np.uint32), want.view(np.uint32))
+        h["p"], h["m"], h["v"] = want, m, v
+        if bits == 8:  # the next step starts from what the codes hold
+            for k, top in (("m", 15), ("v", 31)):
+                h[k] = q.decode(d[k].to_array(n, np.uint8), d[k + "_exp"].to_array(-(-n // q.BLOCK), np.uint8), top)
+
+
 def test_adamw_many_tensors_of_both_kinds(lib, stream):
     """More tensors than one launch describes, 8 and 32 bits mixed, no gradient scale."""
     r = np.random.default_rng(2)
