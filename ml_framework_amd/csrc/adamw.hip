@@ -320,9 +320,12 @@ __global__ __launch_bounds__(kThreads) void adamw_values(Batch b) {
 }
 
 // Launches `kernel` over all tensors, kMost at a time (fewer where the grid of
-// those would pass its limit).
+// those would pass its limit). Nothing is launched where a tensor is refused.
 template <class Fill, class Launch>
 int batches(const seera_adamw_tensor* tensors, int n, Fill&& fill, Launch&& launch) {
+    constexpr int64_t kMostBlocks = kMaxThreads / kThreads - 1;
+    for (int i = 0; i < n; ++i)
+        if (tensors[i].count > kMostBlocks * kChunk) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: tensor %d is too large", i);
     Batch b;
     int64_t blocks = 0;
     b.count = 0;
@@ -330,8 +333,7 @@ int batches(const seera_adamw_tensor* tensors, int n, Fill&& fill, Launch&& laun
         const seera_adamw_tensor& t = tensors[i];
         if (t.count == 0) continue;
         const int64_t more = (t.count + kChunk - 1) / kChunk;
-        if (more >= kMaxThreads / kThreads) return fail(SEERA_ERR_INVALID_ARGUMENT, "adamw: tensor %d is too large", i);
-        if (b.count == kMost || blocks + more >= kMaxThreads / kThreads) {
+        if (b.count == kMost || blocks + more > kMostBlocks) {
             launch(b, (unsigned)blocks);
             SEERA_HIP_TRY(hipGetLastError());
             b.count = 0;

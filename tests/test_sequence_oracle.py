@@ -250,6 +250,15 @@ def test_sizes_that_no_launch_reaches_are_refused():
     _refused("seera_hip_adamw_step_async", (_tensor(count=1 << 50), 1, 1e-3, 0.9, 0.999, 1e-8, 1, 0, None, None), "too large")
 
 
+def test_a_refused_step_has_moved_no_tensor():
+    """The last of more tensors than one launch takes is too large: the call is
+    refused before any launch (here, without a device, a launch is another error)."""
+    many = (capi.AdamwTensor * 60)(*[_tensor()[0]] * 59, _tensor(count=1 << 50)[0])
+    _refused("seera_hip_adamw_step_async", (many, 60, 1e-3, 0.9, 0.999, 1e-8, 1, 0, None, None), "tensor 59 is too large")
+    outs = (ctypes.c_void_p * 60)(*[P] * 60)
+    _refused("seera_hip_adamw_state_values_async", (many, 60, outs, outs, None), "tensor 59 is too large")
+
+
 def test_nothing_to_do_needs_no_pointers():
     lib = capi.load()
     for dims in ((0, 3, 8), (2, 3, 0)):
