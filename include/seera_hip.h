@@ -490,7 +490,7 @@ int seera_hip_gated_scan_fwd_async(const void *x, const void *f,
 /* Its gradients. h is the forward's output, dh [batch, time] rows (contiguous)
  * and dhT [batch, channels] fp32 (optional, zeros) the gradients of h and hT.
  * With g_t = dh_t + a_{t+1} g_{t+1} (dhT at the last step):
- *   LINEAR   dx = g            df = g h_{t-1}          (x is not read, may be NULL)
+ *   LINEAR   dx = g            df = g h_{t-1}          (x is not read: NULL, any ldx)
  *   SIGMOID  dx = g (1 - a)    df = g (h_{t-1} - x) a (1 - a)
  * and dh0 = a_0 g_0 (optional; it may be dhT itself). dx and df are 0 in rows
  * t >= length. */

@@ -76,9 +76,10 @@ int scan_fwd(const ScanShape& s, const ScanFwd& a, hipStream_t st) {
     return gated_scan_fwd(s, a, st);
 }
 
-int scan_bwd(const ScanShape& s, const ScanBwd& a, hipStream_t st) {
+int scan_bwd(const ScanShape& s, ScanBwd a, hipStream_t st) {
     const char* op = "gated_scan";
     bool work;
+    if (s.gate == SEERA_GATE_LINEAR) a.x = nullptr, a.ldx = s.channels;  // not read
     SEERA_TRY(scan_shape(s, {a.ldx, a.ldf, a.lddx, a.lddf}, &work));
     if (s.batch == 0 || s.channels == 0) return SEERA_OK;
     const size_t e = dtype_bytes(s.dtype);

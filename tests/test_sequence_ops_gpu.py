@@ -265,6 +265,22 @@ def test_scan_gradient_against_differences(lib, time, channels):
     assert abs(slope - want) <= step**2 * np.abs(got["df"] * w).sum() * 8 + 64 * q.U * size * np.sqrt(time) / step
 
 
+@pytest.mark.parametrize("time", [3, 100, 2500])
+def test_scan_linear_backward_without_x(lib, time):
+    """No x and no row distance of one: the result of a call that gives both."""
+    batch, c = 2, 40
+    d = _scan_data(batch, time, c, q.F32, False, 13)
+    h, _ = _scan_forward(lib, d, q.F32, False)
+    want = _scan_backward(lib, d, h, q.F32, False)
+    f, kept, dh = (Rows((batch, time, c), q.F32, data=a) for a in (d["f"], h, d["dh"]))
+    dx, df = (Rows((batch, time, c), q.F32) for _ in range(2))
+    h0, dhT, dh0 = DeviceBuffer.from_array(d["h0"]), DeviceBuffer.from_array(d["dhT"]), DeviceBuffer(d["h0"].nbytes)
+    capi.call("seera_hip_gated_scan_bwd", None, f.ptr, h0.ptr, None, kept.ptr, dh.ptr, dhT.ptr, dx.ptr, df.ptr, dh0.ptr, batch, time, c, 0, c, c, c,
+              capi.SEERA_GATE_LINEAR, 0, q.F32)
+    assert np.array_equal(dx.values(), want["dx"]) and np.array_equal(df.values(), want["df"])
+    assert np.array_equal(dh0.to_array(d["h0"].shape).astype(np.float64), want["dh0"])
+
+
 def test_scan_rows_far_apart(lib):
     """Rows 8 MiB and more apart: a tile's rows would lie further from each other
     than 32 bits of address reach. x and f are two slices of the same wide rows."""

@@ -259,6 +259,14 @@ def test_a_refused_step_has_moved_no_tensor():
     _refused("seera_hip_adamw_state_values_async", (many, 60, outs, outs, None), "tensor 59 is too large")
 
 
+def test_a_linear_scans_backward_asks_nothing_of_x():
+    """x is not read there, so that its row distance is not looked at either."""
+    for ldx in (0, -1, 1 << 62):
+        args = (None, P, None, None, P, P, None, P, P, None, 0, 3, 8, ldx, 8, 8, 8)
+        assert capi.load().seera_hip_gated_scan_bwd_async(*args, capi.SEERA_GATE_LINEAR, 0, 0, None) == capi.SEERA_OK
+        _refused("seera_hip_gated_scan_bwd_async", (*args, capi.SEERA_GATE_SIGMOID, 0, 0, None), "row distance")
+
+
 def test_nothing_to_do_needs_no_pointers():
     lib = capi.load()
     for dims in ((0, 3, 8), (2, 3, 0)):
