@@ -419,7 +419,8 @@ int launch_tiles(const ScanShape& s, const ScanPtrs& p, int64_t parts, hipStream
         seg.steps = per * kSteps;
     }
     const int64_t blocks = chains * seg.count;
-    if (blocks >= kMaxThreads / NT) return fail(SEERA_ERR_INVALID_ARGUMENT, "gated_scan: batch * channels is too large");
+    if (blocks > kMaxThreads / NT - 8) return fail(SEERA_ERR_INVALID_ARGUMENT, "gated_scan: batch * channels is too large");
+    // a whole number of blocks for each of the eight dies
     auto grid = [](int64_t n) { return dim3((unsigned)((n + 7) / 8 * 8)); };
     if (seg.count > 1) {
         void* ws = nullptr;

@@ -250,6 +250,13 @@ def test_sizes_that_no_launch_reaches_are_refused():
     _refused("seera_hip_adamw_step_async", (_tensor(count=1 << 50), 1, 1e-3, 0.9, 0.999, 1e-8, 1, 0, None, None), "too large")
 
 
+def test_a_grid_that_rounds_up_to_the_limit_is_refused():
+    """A scan's grid is a multiple of eight blocks: the last few counts below a
+    launch's limit round up to it."""
+    for batch in ((1 << 25) - 1, (1 << 25) - 7):
+        _refused("seera_hip_gated_scan_fwd_async", (P, P, P, None, P, P, batch, 20, 2, 2, 2, 1, 0, 2, None), "too large")
+
+
 def test_a_refused_step_has_moved_no_tensor():
     """The last of more tensors than one launch takes is too large: the call is
     refused before any launch (here, without a device, a launch is another error)."""
