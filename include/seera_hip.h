@@ -571,8 +571,12 @@ int seera_hip_block_norm_bwd_async(const void *y, const void *g,
  * the bits c << 20, times 2^(E - 31); of m that of the low seven bits, times
  * 2^(E - 15), negative with the top bit. E = 255 marks a block that held an
  * infinity or NaN: its values are NaN. Rounding is up or down with the remainder
- * as its probability, from a hash of (seed, place in the list, index): unbiased,
- * and the same in every run. A positive v keeps a code of at least 1. */
+ * as its probability, from a hash of (seed, place in the list, index): the same in
+ * every run, and unbiased over the steps as long as each step has another seed (the
+ * step's number will do). With one seed for all steps a value meets the same
+ * threshold in each, and v, which falls by a small part of a code's place, stays
+ * where it is. A captured graph replays one seed, step and lr: replay no step with
+ * 8-bit states. A positive v keeps a code of at least 1. */
 typedef struct seera_adamw_tensor {
     float *param;
     const void *grad;

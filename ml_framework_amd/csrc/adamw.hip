@@ -12,9 +12,10 @@
 // Codes. v moves by a thousandth of itself in a step and a code's place is an
 // eighth: rounded to nearest, v would never fall (a run on a noisy quadratic left
 // it at a quarter of its value). So a value is rounded up or down with the
-// remainder as probability, by bits of a hash, which leaves the mean right. And
-// the shared exponent is a power of two: a scale that followed the largest value
-// exactly would move every code off its place in every step, and round it again.
+// remainder as probability, by bits of a hash, which leaves the mean right where
+// each step has a seed of its own. And the shared exponent is a power of two: a
+// scale that followed the largest value exactly would move every code off its place
+// in every step, and round it again.
 #include <algorithm>
 
 #include "io_types.h"
