@@ -66,12 +66,20 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     return s;
 }
 
-// 1 / (1 + e^-g) and its slope; the activation and its slope from them.
-__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
-__device__ __forceinline__ float act_of(int act, float g) { return act == SEERA_GATE_ACT_SILU ? g * sigmoid(g) : sigmoid(g); }
-__device__ __forceinline__ float slope_of(int act, float g) {
-    const float q = sigmoid(g), d = q * (1.f - q);
-    return act == SEERA_GATE_ACT_SILU ? fmaf(g, d, q) : d;
+// The activation of a gate.
+__device__ __forceinline__ float act_of(int act, float g) {
+    const float q = __builtin_amdgcn_rcpf(1.f + __expf(-g));
+    return act == SEERA_GATE_ACT_SILU ? g * q : q;
+}
+// The activation and its slope. The sigmoid's slope is the product of its two sides,
+// both from e^-|g|: 1 minus the larger one has no digit left where that is near 1.
+struct Act {
+    float of, slope;
+};
+__device__ __forceinline__ Act act_and_slope(int act, float g) {
+    const float e = __expf(-fabsf(g)), large = __builtin_amdgcn_rcpf(1.f + e), small = e * large;
+    const float q = g >= 0.f ? large : small, d = small * large;
+    return act == SEERA_GATE_ACT_SILU ? Act{g * q, fmaf(g, d, q)} : Act{q, d};
 }
 
 // 16 bytes of a row, moved as one access at any alignment of T (the hardware
@@ -327,12 +335,12 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
             if (p.g) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float g = to_f32(now.g[k].v[i]), q = sigmoid(g), slope = q * (1.f - q);
-                    const float act = s.act == SEERA_GATE_ACT_SILU ? g * q : q, z = to_f32(now.y[k].v[i]) * now.rstd1 * h1[k][i];
-                    sums[k][i] = fmaf(d[k][i] * z, act, sums[k][i]);
+                    const Act act = act_and_slope(s.act, to_f32(now.g[k].v[i]));
+                    const float z = to_f32(now.y[k].v[i]) * now.rstd1 * h1[k][i];
+                    sums[k][i] = fmaf(d[k][i] * z, act.of, sums[k][i]);
                     d[k][i] *= hs[k][i];
-                    out.v[i] = from_f32<T>(d[k][i] * z * (s.act == SEERA_GATE_ACT_SILU ? fmaf(g, slope, q) : slope));
-                    d[k][i] *= act;
+                    out.v[i] = from_f32<T>(d[k][i] * z * act.slope);
+                    d[k][i] *= act.of;
                 }
                 store_wide((T*)p.dg + row * p.lddg, place(k), out);
             } else if (p.s) {
@@ -416,15 +424,16 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_rows(NormBwd p, NormShape s
             }
             if (p.dr) ((T*)p.dr)[at + c] = from_f32<T>(d);
             const bool inner = p.w1 || p.g || p.s;
-            const float yv = inner ? to_f32(y[c]) : 0.f, gv = p.g ? to_f32(g[c]) : 0.f;
-            const float hat = yv * rstd1, z = p.w1 ? hat * p.w1[c] : yv, act = p.g ? act_of(s.act, gv) : 1.f;
+            const float yv = inner ? to_f32(y[c]) : 0.f;
+            const float hat = yv * rstd1, z = p.w1 ? hat * p.w1[c] : yv;
+            const Act act = p.g ? act_and_slope(s.act, to_f32(g[c])) : Act{1.f, 0.f};
             if (p.s) {
-                sums[s.cols + c] += d * z * act;
+                sums[s.cols + c] += d * z * act.of;
                 d *= p.s[c];
             }
             if (p.g) {
-                ((T*)p.dg)[row * p.lddg + c] = from_f32<T>(d * z * slope_of(s.act, gv));
-                d *= act;
+                ((T*)p.dg)[row * p.lddg + c] = from_f32<T>(d * z * act.slope);
+                d *= act.of;
             }
             if (p.w1) {
                 sums[c] += d * hat;

@@ -439,6 +439,22 @@ def test_norm_optional_outputs(lib, stream):
         _close(alone[k], refs[k], bounds[k], q.F32 if k[1:] in ("w1", "s", "w2") else q.BF16, k)
 
 
+@pytest.mark.parametrize("cols", [200, 1501, 9000])
+def test_norm_slope_of_a_saturated_gate(lib, cols):
+    """The gradient of a sigmoid gate far from 0, against sigma(g) sigma(-g): each of
+    the two by an exponential whose argument is rounded (|g| u), a sum, a reciprocal
+    and products, so that the relative error stays (16 + 2 |g|) u where 1 - sigma(g)
+    has no digit left."""
+    rows = 3
+    d = _norm_data(rows, cols, q.F32, "g", 31)
+    d["g"] = _seen(np.linspace(-80, 80, rows * cols).reshape(rows, cols), q.F32)
+    got = _norm_backward(lib, d, {}, q.F32, False)
+    with np.errstate(over="ignore"):
+        slope = 1 / (1 + np.exp(d["g"])) / (1 + np.exp(-d["g"]))
+    want = d["dr_out"] * d["y"] * slope
+    assert np.all(np.abs(got["dg"] - want) <= np.abs(want) * (16 + 2 * np.abs(d["g"])) * q.U + 2.0**-126)
+
+
 def test_norm_of_no_rows(lib):
     """No rows: the sums over them are zero."""
     w, out = DeviceBuffer.from_array(np.ones(40, np.float32)), [DeviceBuffer.from_array(np.full(40, 7, np.float32)) for _ in range(3)]
