@@ -542,6 +542,52 @@ def test_norm_in_place(lib):
         assert np.array_equal(dw[k].values()[0], back["d" + k]), k
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("parts", ["g r w1 s w2", "w2", "r w2", "g w1", "s r", "g r s w2"])
+@pytest.mark.parametrize("rows,cols", [(300, 1501), (40, 1500), (270, 5003), (300, 9001)])
+def test_norm_in_place_over_several_waves(lib, dtype, parts, rows, cols):
+    """Every overlap that is allowed, at widths of several waves whose last loads
+    reach into the pack before them: the results of separate buffers, bit for bit."""
+    d = _norm_data(rows, cols, dtype, parts, rows + cols)
+    want = _norm_forward(lib, d, dtype, True)
+    w = {k: Rows((1, cols), q.F32, data=d[k][None]) if k in d else None for k in ("w1", "s", "w2")}
+    p = lambda m: m.ptr if m is not None else None  # noqa: E731
+    weights = [p(w[k]) for k in ("w1", "s", "w2")]
+    for r_over, n_over in (("r", "y"), ("y", "r"), ("g", "y"), ("r", "g"), ("y", None), (None, "y")):
+        names = {r_over, n_over} - {None}
+        if not names <= set(d) or (n_over and "w2" not in d):
+            continue
+        m = {k: Rows((rows, cols), dtype, data=d[k]) if k in d else None for k in ("y", "g", "r")}
+        r_out = m[r_over] if r_over else Rows((rows, cols), dtype)
+        n_out = (m[n_over] if n_over else Rows((rows, cols), dtype)) if "w2" in d else None
+        capi.call("seera_hip_block_norm_fwd", m["y"].ptr, p(m["g"]), p(m["r"]), *weights, r_out.ptr, p(n_out), None, None, rows, cols, cols, cols, 1e-6, 0, dtype)
+        assert np.array_equal(r_out.values(), want["r_out"]), (r_over, n_over)
+        assert n_out is None or np.array_equal(n_out.values(), want["n_out"]), (r_over, n_over)
+    back = _norm_backward(lib, d, want, dtype, True)
+    inner = any(k in d for k in ("w1", "g", "s"))
+    for dr_over in ("dr_out", "dn"):
+        if dr_over == "dn" and "w2" not in d:
+            continue
+        m = {k: Rows((rows, cols), dtype, data=d[k]) if k in d else None for k in ("y", "g", "dr_out")}
+        m["dn"] = Rows((rows, cols), dtype, data=d["dn"]) if "w2" in d else None
+        kept = Rows((rows, cols), dtype, data=want["r_out"]) if "w2" in d else None
+        s1, s2 = (Rows((1, rows), q.F32, data=want[k][None]) if k in want else None for k in ("rstd1", "rstd2"))
+        dw = {k: Rows((1, cols), q.F32) if k in d else None for k in w}
+        capi.call("seera_hip_block_norm_bwd", m["y"].ptr if inner else None, p(m["g"]), p(kept), *weights, p(s1), p(s2), m["dr_out"].ptr, p(m["dn"]),
+                  m["y"].ptr, p(m["g"]), m[dr_over].ptr, *[p(dw[k]) for k in w], rows, cols, cols, cols, cols, cols, 0, dtype)
+        for k, v in (("dy", m["y"]), ("dg", m["g"]), ("dr", m[dr_over])):
+            assert v is None or np.array_equal(v.values(), back[k]), (k, dr_over)
+        for k in dw:
+            assert dw[k] is None or np.array_equal(dw[k].values()[0], back["d" + k]), (k, dr_over)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("parts", ["g r w1 s w2", "w2", "g w1"])
+def test_norm_wide_rows_over_many_rows(lib, dtype, parts):
+    """Rows beyond the widths whose backward stays in registers, several a block."""
+    _check_norm(lib, 520, 9002, dtype, parts, seed=77)
+
+
 # ---- AdamW ----
 
 
