@@ -71,14 +71,14 @@ __device__ __forceinline__ float act_of(int act, float g) {
     const float q = __builtin_amdgcn_rcpf(1.f + __expf(-g));
     return act == SEERA_GATE_ACT_SILU ? g * q : q;
 }
-// The activation and its slope. The sigmoid's slope is the product of its two sides,
-// both from e^-|g|: 1 minus the larger one has no digit left where that is near 1.
+// The activation and its slope. The sigmoid's slope is the product of its two sides
+// q and e^-g q: 1 - q has no digit left where q is near 1. (Below g = -88 that is
+// infinity times 0, and the side is 1.)
 struct Act {
     float of, slope;
 };
 __device__ __forceinline__ Act act_and_slope(int act, float g) {
-    const float e = __expf(-fabsf(g)), large = __builtin_amdgcn_rcpf(1.f + e), small = e * large;
-    const float q = g >= 0.f ? large : small, d = small * large;
+    const float e = __expf(-g), q = __builtin_amdgcn_rcpf(1.f + e), d = q * fminf(e * q, 1.f);
     return act == SEERA_GATE_ACT_SILU ? Act{g * q, fmaf(g, d, q)} : Act{q, d};
 }
 
@@ -272,7 +272,8 @@ __global__ __launch_bounds__(NT) void norm_bwd_regs(NormBwd p, NormShape s, floa
     auto load = [&](NormRow<T, K>& to, int64_t row) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const At c = place(k);
+            At c = place(k);
+            if (!HOLD) asm volatile("" : "+v"(c.c));  // as for the weights: 5 K addresses held over the rows would spill
             if (inner) load_wide(to.y[k], (const T*)p.y + row * p.ldy, c, s.cols);
             if (p.g) load_wide(to.g[k], (const T*)p.g + row * p.ldg, c, s.cols);
             if (p.w2) {
