@@ -6,8 +6,8 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 //
 // Bytes bound: 28 a value with fp32 states and gradients, 16 with 8-bit states,
-// bf16 gradients and a bf16 copy. 97 tensors of 97.6 M values: 490 us (5.8 TB/s; a
-// large copy makes 5.35); with 8 bits, and the values read out (10 bytes), 463 us.
+// bf16 gradients and a bf16 copy. 97 tensors of 97.6 M values: 501 us (5.5 TB/s; a
+// large copy makes 5.35); with 8 bits, and the values read out (10 bytes), 472 us.
 //
 // Codes. v moves by a thousandth of itself in a step and a code's place is an
 // eighth: rounded to nearest, v would never fall (a run on a noisy quadratic left
