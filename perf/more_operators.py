@@ -322,7 +322,7 @@ def _sample(case, t):
     """In 64 bits: a cut and a draw both compare a sum of many terms with a border."""
     z, index = torch.sort(t["logits"].float(), dim=1, descending=True, stable=True)
     greedy = t["temperature"] <= 0
-    z = (z - z[:, :1]).double() / torch.where(greedy, 1.0, t["temperature"]).double()[:, None]
+    z = (z.double() - z[:, :1].double()) / torch.where(greedy, 1.0, t["temperature"]).double()[:, None]
     w = torch.exp(z)
     keep = torch.ones_like(w, dtype=torch.bool)
     if "top_k" in t:
