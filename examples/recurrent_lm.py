@@ -13,6 +13,13 @@ Each block is
 
 and the step is cuda_adamw_step over all tensors: the products' weights with
 8-bit states, the norms' with 32-bit ones.
+
+The trained model then answers in 8 bits, on the GPU from one token to the next:
+
+    weights     cuda_quantize_weights_f8, once
+    n           cuda_block_norm_fwd_f8: the same norms, their output in 8 bits
+    products    cuda_matmul_f8
+    next token  cuda_sample: temperature, top-k, top-p
 """
 from __future__ import annotations
 
@@ -175,9 +182,64 @@ class RecurrentLM:
             self.sc.cuda_free(p)
         return out
 
+    def to_8_bits(self):
+        """Puts the products' weights into 8 bits, for answer(); anew after each training."""
+        for name in [f"{part}{i}" for i in range(self.blocks) for part in ("in", "out")] + ["head"]:
+            k, n = self.weights.shape[name]
+            # a fp32 buffer of a quarter as many values holds the codes
+            codes = self.weights.new("f8_" + name, (n, padded(k) // 4))
+            scales = self.weights.new("f8_scales_" + name, (padded(n) // 128, padded(k) // 128))
+            self.sc.cuda_quantize_weights_f8(self.weights[name], codes, scales, n, k, n, 0, self.sc.DTYPE_F32)
+
+    def answer(self, prompt, count, temperature=0.7, top_k=0, top_p=0.95, seed=0):
+        """Sampled continuation of a prompt with the weights in 8 bits."""
+        sc, w, c, v = self.sc, self.weights, self.width, self.vocab
+        b = Buffers(sc)
+        f32, nothing = sc.DTYPE_F32, 0
+        try:
+            for name, size in (("r", c), ("proj", 3 * c), ("h", c), ("y", c), ("logits", v), ("n", padded(c) // 4), ("n_scales", padded(c) // 128), ("token", 1), ("logp", 1)):
+                b.new(name, (size,))
+            for i in range(self.blocks):
+                b.new(f"state{i}", (c,))
+            b.new("temperature", (1,), [temperature])
+            b.new("top_p", (1,), [top_p])
+            b.new("uniform", (count,), np.random.default_rng(seed).random(count, np.float32))
+            b.ptr["top_k"] = sc.to_device_i32(np.array([top_k], np.int32))
+
+            def product(name, to):
+                k, n = w.shape[name]
+                sc.cuda_matmul_f8(b["n"], b["n_scales"], w["f8_" + name], w["f8_scales_" + name], nothing, to, 1, n, k, n, f32)
+
+            def norm(y, g, r, w1, s, w2, r_out):
+                sc.cuda_block_norm_fwd_f8(y, g, r, w1, s, w2, r_out, b["n"], b["n_scales"], 1, c, c, c, EPS, sc.GATE_ACT_SILU, f32)
+
+            out = list(prompt)
+            for at in range(len(prompt) + count - 1):
+                sc.cuda_memcopy_devicetodevice(b["r"], w["embed"] + 4 * c * out[at], c)
+                norm(b["r"], nothing, nothing, nothing, nothing, w["first"], nothing)
+                for i in range(self.blocks):
+                    product(f"in{i}", b["proj"])
+                    sc.cuda_gated_scan_fwd(b["proj"], b["proj"] + 4 * c, b[f"state{i}"], 0, b["h"], b[f"state{i}"], 1, 1, c, 3 * c, 3 * c, sc.GATE_SIGMOID, 0, f32)
+                    norm(b["h"], nothing, nothing, nothing, nothing, nothing, nothing)  # into 8 bits as it is
+                    product(f"out{i}", b["y"])
+                    norm(b["y"], b["proj"] + 8 * c, b["r"], w[f"after{i}"], w[f"scale{i}"], w[f"before{i}"], b["r"])
+                if at + 1 < len(prompt):
+                    continue
+                product("head", b["logits"])
+                sc.cuda_sample(b["logits"], b["uniform"] + 4 * (at + 1 - len(prompt)), b["temperature"], b["top_k"], b["top_p"], nothing, b["token"], b["logp"], 1, v, v, f32)
+                out.append(int(sc.to_host_i32(b["token"], (1,))[0]))
+            return out
+        finally:
+            b.close()
+
     def close(self):
         self.weights.close()
         self.work.close()
+
+
+def padded(k):
+    """The length of a row of k codes."""
+    return -(-k // 128) * 128
 
 
 def batches(text, batch, time, seed=0):
@@ -200,6 +262,8 @@ def main(steps=250):
                 print(f"step {i:4d}  loss {loss:.4f}", flush=True)
         start = [letters.index(ch) for ch in TEXT[:12]]
         print("".join(letters[k] for k in model.generate(start, 160)))
+        model.to_8_bits()
+        print("in 8 bits: " + "".join(letters[k] for k in model.answer(start, 160)))
     finally:
         model.close()
 

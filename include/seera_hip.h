@@ -618,6 +618,89 @@ int seera_hip_adamw_state_values_async(const seera_adamw_tensor *tensors, int n,
                                        float *const *m_values,
                                        float *const *v_values, void *stream);
 
+/* ---- models that answer in 8 bits (no counterpart in the reference) ----
+ *
+ * An 8-bit operand is a matrix of e4m3 codes (sign, 4 bits of exponent, 3 of
+ * mantissa; 0x7e = 448 is the largest, 0x7f and 0xff are NaN) with fp32 scales; a
+ * value is code times scale.
+ *   codes   [rows][kp], kp = K rounded up to 128: row after row, 16-byte aligned, the
+ *           codes from K on 0. The entry points below write them so, and what a
+ *           caller brings of its own has to be so (zeros need one operand only)
+ *   scales  of activations [rows][kp / 128]: one for 128 values of a row;
+ *           of weights [N rounded up to 128, / 128][kp / 128]: one for 128 x 128
+ * They are made with scale = max|v| / 448 (fp32) and code = v / scale, rounded to
+ * nearest, ties to even. A block of zeros has scale 0, one that holds an infinity or NaN
+ * scale NaN: its values are NaN. Pointers other than codes must be aligned to
+ * their type; sizes may be any. Results do not depend on timing. The entry points
+ * take no workspace, so a captured call needs no eager one before it. */
+
+/* seera_hip_block_norm_fwd with its output in 8 bits, K = cols (at most 16384):
+ *   z = rms(y) w1,  u = z act(g) s,  r_out = r + u,  n = rms(r_out) w2
+ * each factor or term that is NULL left out, n = r_out without w2. n is of r_out as
+ * it is stored (rounded to dtype, also where r_out is NULL) and is not rounded to dtype itself.
+ * So y and w2 alone are a plain norm, y alone is put into 8 bits. r_out may be r, or y or g
+ * where that has contiguous rows. No statistics are kept: this form has no backward. */
+int seera_hip_block_norm_fwd_f8(const void *y, const void *g, const void *r,
+                                const float *w1, const float *s,
+                                const float *w2, void *r_out, uint8_t *codes,
+                                float *scales, int rows, int cols, int64_t ldy,
+                                int64_t ldg, float eps, int act, int dtype);
+int seera_hip_block_norm_fwd_f8_async(const void *y, const void *g,
+                                      const void *r, const float *w1,
+                                      const float *s, const float *w2,
+                                      void *r_out, uint8_t *codes,
+                                      float *scales, int rows, int cols,
+                                      int64_t ldy, int64_t ldg, float eps,
+                                      int act, int dtype, void *stream);
+/* A weight matrix in 8 bits. w is [k, n] as the B of seera_hip_matmul, rows ldw
+ * elements apart, or with transposed != 0 [n, k]. Writes codes [n][kp] and scales
+ * [n rounded up to 128, / 128][kp / 128]. */
+int seera_hip_quantize_weights_f8(const void *w, uint8_t *codes, float *scales,
+                                  int n, int k, int64_t ldw, int transposed,
+                                  int dtype);
+int seera_hip_quantize_weights_f8_async(const void *w, uint8_t *codes,
+                                        float *scales, int n, int k,
+                                        int64_t ldw, int transposed, int dtype,
+                                        void *stream);
+/* C[M, N] = A W^T + bias of A [M][kp] with the scales of activations and W [N][kp]
+ * with those of weights. Each block of 128 along K is summed in fp32, multiplied by
+ * its two scales and added in fp32; bias ([N] fp32, optional) is added and the result
+ * rounded to dtype once. Rows of C are ldc elements apart. K == 0 gives the bias. */
+int seera_hip_matmul_f8(const uint8_t *a, const float *a_scales,
+                        const uint8_t *w, const float *w_scales,
+                        const float *bias, void *C, int M, int N, int K,
+                        int64_t ldc, int dtype);
+int seera_hip_matmul_f8_async(const uint8_t *a, const float *a_scales,
+                              const uint8_t *w, const float *w_scales,
+                              const float *bias, void *C, int M, int N, int K,
+                              int64_t ldc, int dtype, void *stream);
+/* A token for each row of logits ([rows, vocab], ld elements apart, vocab at most
+ * 2^22). uniform, temperature, top_k, top_p, min_p, tokens, logp hold [rows] values on the
+ * device; all but uniform and tokens are optional.
+ *   weight   exp((l - max l) / temperature)   (1 without); a temperature that is not
+ *            above 0 takes the largest logit's token, the lowest of several
+ *   order    by logit, largest first, equal ones by index
+ *   top_k    keeps the first top_k (all where it is below 1)
+ *   top_p    keeps of those the fewest, at least one, whose weights reach top_p of
+ *            their sum (all where it is not below 1)
+ *   min_p    keeps weights of at least min_p (of the largest's, which is 1)
+ *   token    the first, by index, where the sum of the kept weights up to and with it
+ *            is above uniform (in [0, 1); a NaN counts as 0, others as the nearer end) of their total
+ *   logp     the logarithm of its weight's share of that total; 0 where it was not drawn
+ * Weights are whole multiples of 2^-40, so that sums do not depend on their order; one
+ * below half of that is none. A logit of -infinity or NaN is never drawn, of several
+ * +infinities each has weight 1. A row with nothing to draw gives token -1 and
+ * logp -infinity. */
+int seera_hip_sample(const void *logits, const float *uniform,
+                     const float *temperature, const int *top_k,
+                     const float *top_p, const float *min_p, int *tokens,
+                     float *logp, int rows, int vocab, int64_t ld, int dtype);
+int seera_hip_sample_async(const void *logits, const float *uniform,
+                           const float *temperature, const int *top_k,
+                           const float *top_p, const float *min_p, int *tokens,
+                           float *logp, int rows, int vocab, int64_t ld,
+                           int dtype, void *stream);
+
 /* ---- timing (no reference counterpart; used by bench.py) ---- */
 
 /* Events on `stream`: create / record / elapsed milliseconds / destroy. */

@@ -31,6 +31,10 @@ _scan_fwd = [_vp] * 6 + [_i] * 3 + [_i64] * 2 + [_i] * 3
 _scan_bwd = [_vp] * 10 + [_i] * 3 + [_i64] * 4 + [_i] * 3
 _norm_fwd = [_vp] * 10 + [_i] * 2 + [_i64] * 2 + [_f] + [_i] * 2
 _norm_bwd = [_vp] * 16 + [_i] * 2 + [_i64] * 4 + [_i] * 2
+_norm_f8 = [_vp] * 9 + [_i] * 2 + [_i64] * 2 + [_f] + [_i] * 2
+_quantize_f8 = [_vp] * 3 + [_i] * 2 + [_i64] + [_i] * 2
+_matmul_f8 = [_vp] * 6 + [_i] * 3 + [_i64, _i]
+_sample = [_vp] * 8 + [_i] * 2 + [_i64, _i]
 _adamw = [_vp, _i, _d, _d, _d, _d, _i64, ctypes.c_uint32, _vp]
 
 
@@ -140,6 +144,15 @@ PROTOTYPES: dict[str, tuple[list, object]] = {
     "seera_hip_adamw_step_async": (_adamw + [_vp], _i),
     "seera_hip_adamw_state_values": ([_vp, _i, _vp, _vp], _i),
     "seera_hip_adamw_state_values_async": ([_vp, _i, _vp, _vp, _vp], _i),
+    # models that answer in 8 bits: block norm, weights, products, sampling
+    "seera_hip_block_norm_fwd_f8": (_norm_f8, _i),
+    "seera_hip_block_norm_fwd_f8_async": (_norm_f8 + [_vp], _i),
+    "seera_hip_quantize_weights_f8": (_quantize_f8, _i),
+    "seera_hip_quantize_weights_f8_async": (_quantize_f8 + [_vp], _i),
+    "seera_hip_matmul_f8": (_matmul_f8, _i),
+    "seera_hip_matmul_f8_async": (_matmul_f8 + [_vp], _i),
+    "seera_hip_sample": (_sample, _i),
+    "seera_hip_sample_async": (_sample + [_vp], _i),
 }
 
 _lib = None

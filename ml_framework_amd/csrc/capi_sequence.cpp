@@ -4,46 +4,13 @@
 // and synchronize, the _async forms enqueue on the caller's stream.
 #include <math.h>
 
+#include "capi_args.h"
 #include "io_types.h"
-#include "runtime.h"
 #include "sequence.h"
 
 using namespace seera;
 
 namespace {
-
-template <class F>
-int now(F&& f) {
-    clear_error();
-    SEERA_TRY(f(nullptr));
-    SEERA_HIP_TRY(hipDeviceSynchronize());
-    note_device_synchronized();
-    return SEERA_OK;
-}
-template <class F>
-int later(void* stream, F&& f) {
-    clear_error();
-    SEERA_TRY(f(reinterpret_cast<hipStream_t>(stream)));
-    note_async_work();
-    return SEERA_OK;
-}
-
-int bad(const char* op, const char* what) { return fail(SEERA_ERR_INVALID_ARGUMENT, "%s: %s", op, what); }
-
-// Each of `ptrs` must not be null and must be aligned to a value of `bytes`.
-int required(const char* op, size_t bytes, std::initializer_list<const void*> ptrs) {
-    for (const void* p : ptrs) {
-        if (!p) return bad(op, "null device pointer");
-        if (!aligned_to(p, bytes)) return bad(op, "a pointer is not aligned to its type");
-    }
-    return SEERA_OK;
-}
-// The same where a pointer is given.
-int optional(const char* op, size_t bytes, std::initializer_list<const void*> ptrs) {
-    for (const void* p : ptrs)
-        if (!aligned_to(p, bytes)) return bad(op, "a pointer is not aligned to its type");
-    return SEERA_OK;
-}
 
 // ---- gated scan ----
 

@@ -450,6 +450,43 @@ PYBIND11_MODULE(seera_cuda, m) {
           },
           "The moments of a list of AdamwTensor as fp32 (lists of GPU ptrs, 0 to skip one)");
 
+    // ---- models that answer in 8 bits (no counterpart in the reference) ----
+    m.def("cuda_block_norm_fwd_f8",
+          [](uintptr_t y, uintptr_t g, uintptr_t r, uintptr_t w1, uintptr_t s, uintptr_t w2,
+             uintptr_t r_out, uintptr_t codes, uintptr_t scales, int rows, int cols, int64_t ldy,
+             int64_t ldg, float eps, int act, int dtype) {
+              check(seera_hip_block_norm_fwd_f8(
+                  dev<const void>(y), dev<const void>(g), dev<const void>(r), dev<const float>(w1),
+                  dev<const float>(s), dev<const float>(w2), dev<void>(r_out), dev<uint8_t>(codes),
+                  dev<float>(scales), rows, cols, ldy, ldg, eps, act, dtype));
+          },
+          "Block norm with its output in e4m3 codes and scales (GPU ptrs; 0 for an optional one)");
+    m.def("cuda_quantize_weights_f8",
+          [](uintptr_t w, uintptr_t codes, uintptr_t scales, int n, int k, int64_t ldw,
+             int transposed, int dtype) {
+              check(seera_hip_quantize_weights_f8(dev<const void>(w), dev<uint8_t>(codes),
+                                                  dev<float>(scales), n, k, ldw, transposed, dtype));
+          },
+          "Weights [k, n] (or [n, k]) in e4m3 codes and scales (GPU ptrs)");
+    m.def("cuda_matmul_f8",
+          [](uintptr_t a, uintptr_t a_scales, uintptr_t w, uintptr_t w_scales, uintptr_t bias,
+             uintptr_t C, int M, int N, int K, int64_t ldc, int dtype) {
+              check(seera_hip_matmul_f8(dev<const uint8_t>(a), dev<const float>(a_scales),
+                                        dev<const uint8_t>(w), dev<const float>(w_scales),
+                                        dev<const float>(bias), dev<void>(C), M, N, K, ldc, dtype));
+          },
+          "C = A W^T + bias of operands in e4m3 codes and scales (GPU ptrs; 0 for no bias)");
+    m.def("cuda_sample",
+          [](uintptr_t logits, uintptr_t uniform, uintptr_t temperature, uintptr_t top_k,
+             uintptr_t top_p, uintptr_t min_p, uintptr_t tokens, uintptr_t logp, int rows,
+             int vocab, int64_t ld, int dtype) {
+              check(seera_hip_sample(dev<const void>(logits), dev<const float>(uniform),
+                                     dev<const float>(temperature), dev<const int>(top_k),
+                                     dev<const float>(top_p), dev<const float>(min_p),
+                                     dev<int>(tokens), dev<float>(logp), rows, vocab, ld, dtype));
+          },
+          "A token for each row of logits (GPU ptrs; 0 for an optional one)");
+
     // ---- transfers (cuda_bindings.cpp:73-170) ----
     m.def("to_device_f16", [](arr_f a) { return upload<float>(a); },
           "Upload float32 numpy -> float32 GPU buffer (reference name)");

@@ -1,0 +1,588 @@
+"""The block norm in 8 bits, weights in 8 bits, their product and sampling on the
+GPU against oracle/inference.py, at the sizes, layouts and values where they can go
+wrong. Tolerances are the oracle's, derived before the first run: codes of given
+fp32 values and tokens have to be equal. Outputs lie in buffers of a byte pattern
+with room around them, which has to be intact afterwards."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from ml_framework_amd import capi
+from ml_framework_amd.capi import DeviceBuffer
+from oracle import inference as q
+from oracle import sequence as s
+from tests.test_sequence_ops_gpu import Rows, _close, _seen
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [s.F32, s.F16, s.BF16]
+FILL = 0xA5
+
+
+@pytest.fixture(scope="module")
+def lib():
+    assert capi.gpu_available(), "no HIP device visible"
+    return capi.load()
+
+
+@pytest.fixture
+def stream(lib):
+    st = ctypes.c_void_p()
+    capi.check(lib.seera_hip_stream_create(ctypes.byref(st)))
+    yield st.value
+    lib.seera_hip_stream_destroy(st.value)
+
+
+class Bytes:
+    """A device array in the middle of a byte pattern, 16-byte aligned."""
+
+    def __init__(self, shape, dtype=np.uint8, data=None):
+        self.shape, self.dtype = shape, np.dtype(dtype)
+        self.size = int(np.prod(shape)) * self.dtype.itemsize
+        whole = np.full(self.size + 512, FILL, np.uint8)
+        if data is not None:
+            whole[256:256 + self.size] = np.ascontiguousarray(data, self.dtype).view(np.uint8).reshape(-1)
+        self.buf = DeviceBuffer.from_array(whole)
+        self.ptr = self.buf.ptr + 256
+
+    def values(self):
+        whole = self.buf.to_array(self.size + 512, np.uint8)
+        assert np.all(whole[:256] == FILL) and np.all(whole[256 + self.size:] == FILL), "written outside of the array"
+        return whole[256:256 + self.size].copy().view(self.dtype).reshape(self.shape)
+
+
+def _call(lib, name, args, stream=None):
+    if stream is None:
+        return capi.call(name, *args)
+    capi.call(name + "_async", *args, stream)
+    capi.check(lib.seera_hip_stream_synchronize(stream))
+
+
+# ---- block norm ----
+
+
+def _norm_data(rows, cols, dtype, parts, seed):
+    r = np.random.default_rng(seed)
+    d = {"y": _seen(r.standard_normal((rows, cols)) * np.exp(r.standard_normal((rows, 1))), dtype)}
+    for k in parts.split():
+        if k in "gr":
+            d[k] = _seen(r.standard_normal((rows, cols)) * 2, dtype)
+        else:
+            d[k] = (1 + 0.3 * r.standard_normal(cols)).astype(np.float32).astype(np.float64)
+    return d
+
+
+def _norm(lib, d, dtype, silu=True, gap=0, shift=0, r_out=True, stream=None, eps=1e-6):
+    rows, cols = d["y"].shape
+    y = Rows((rows, cols), dtype, cols + gap, shift, d["y"], hole=np.nan)
+    g = Rows((rows, cols), dtype, cols + gap, shift, d["g"], hole=np.nan) if "g" in d else None
+    r = Rows((rows, cols), dtype, None, shift, d["r"]) if "r" in d else None
+    w = {k: Rows((1, cols), s.F32, None, shift, d[k][None]) if k in d else None for k in ("w1", "s", "w2")}
+    out, codes, scales = Rows((rows, cols), dtype, None, shift), Bytes((rows, q.padded(cols))), Bytes((rows, q.padded(cols) // 128), np.float32)
+    p = lambda m, on=True: m.ptr if m is not None and on else None  # noqa: E731
+    _call(lib, "seera_hip_block_norm_fwd_f8", (y.ptr, p(g), p(r), p(w["w1"]), p(w["s"]), p(w["w2"]), p(out, r_out), codes.ptr, scales.ptr, rows, cols,
+                                               cols + gap, cols + gap, eps, 0 if silu else 1, dtype), stream)
+    return out.values() if r_out else None, codes.values(), scales.values()
+
+
+def _check_norm(lib, rows, cols, dtype, parts, silu=True, seed=1, d=None, **kw):
+    d = d or _norm_data(rows, cols, dtype, parts, seed)
+    kept, codes, scales = _norm(lib, d, dtype, silu, **kw)
+    ref, bound = s.norm_fwd(**{k: d[k] for k in ("y", "g", "r", "w1", "s") if k in d}, silu=silu)
+    _close(kept, ref["r_out"], bound["r_out"], dtype, "r_out")
+    if "w2" not in d:  # what is put into 8 bits is r_out itself: the same bits
+        want, want_scales = q.quantize_rows(kept.astype(np.float32))
+        assert np.array_equal(scales, want_scales) and np.array_equal(codes, want)
+    q.check_codes(codes, scales, *q.norm_values(kept, d.get("w2"), 1e-6))
+
+
+PARTS = ["", "w2", "r w2", "g w1", "g r w1 s w2", "r", "s r"]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("parts", PARTS)
+def test_norm_parts(lib, dtype, parts):
+    _check_norm(lib, 9, 200, dtype, parts)
+    _check_norm(lib, 5, 77, dtype, parts, silu=False)
+    _check_norm(lib, 3, 1501, dtype, parts)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 3), (2, 7), (1, 64), (2, 63), (3, 127), (3, 128), (3, 129), (2, 255), (3, 512), (1, 1024), (700, 66), (4, 2048), (3, 1921),
+                                       (2, 2050), (2, 4096), (5, 4098), (2, 8192), (3, 8001), (2, 16384), (1, 16383), (2, 16257), (1500, 256), (2100, 1000)])
+def test_norm_sizes(lib, dtype, rows, cols):
+    _check_norm(lib, rows, cols, dtype, "g r w1 s w2", seed=rows)
+    _check_norm(lib, rows, cols, dtype, "", seed=cols)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap,shift", [(0, 1), (1, 0), (2, 2), (8, 0), (64, 4)])
+def test_norm_layouts(lib, dtype, gap, shift, stream):
+    _check_norm(lib, 6, 264, dtype, "g r w1 s w2", gap=gap, shift=shift)
+    _check_norm(lib, 6, 1200, dtype, "g w1", gap=gap, shift=shift, silu=False, stream=stream)
+    _check_norm(lib, 4, 5002, dtype, "r w2", gap=gap, shift=shift)
+
+
+def test_norm_without_r_out(lib):
+    d = _norm_data(4, 300, s.BF16, "g r w1 s w2", 3)
+    full, less = _norm(lib, d, s.BF16), _norm(lib, d, s.BF16, r_out=False)
+    assert np.array_equal(full[1], less[1]) and np.array_equal(full[2], less[2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [300, 1501, 4100])
+def test_norm_in_place(lib, dtype, cols):
+    """The residual stream is moved on in its own buffer."""
+    d = _norm_data(5, cols, dtype, "r w2", 4)
+    want, codes, scales = _norm(lib, d, dtype)
+    y, r, w2 = Rows((5, cols), dtype, data=d["y"]), Rows((5, cols), dtype, data=d["r"]), Rows((1, cols), s.F32, data=d["w2"][None])
+    c, sc = Bytes(codes.shape), Bytes(scales.shape, np.float32)
+    capi.call("seera_hip_block_norm_fwd_f8", y.ptr, None, r.ptr, None, None, w2.ptr, r.ptr, c.ptr, sc.ptr, 5, cols, cols, cols, 1e-6, 0, dtype)
+    assert np.array_equal(r.values(), want) and np.array_equal(c.values(), codes) and np.array_equal(sc.values(), scales)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [256, 301, 4100])
+def test_norm_blocks_of_zeros_and_of_what_is_not_finite(lib, dtype, cols):
+    """A block of zeros has scale 0; one with an infinity or NaN scale NaN, and no other."""
+    d = _norm_data(4, cols, dtype, "", 5)
+    d["y"][0] = 0
+    d["y"][1, 128:] = 0
+    d["y"][2, 130], d["y"][3, cols - 1] = np.inf, np.nan
+    kept, codes, scales = _norm(lib, d, dtype)
+    want, want_scales = q.quantize_rows(np.nan_to_num(kept, nan=0, posinf=0).astype(np.float32))
+    want_scales[2, 1] = want_scales[3, (cols - 1) // 128] = np.nan
+    assert np.array_equal(scales, want_scales, equal_nan=True)
+    assert not codes[0].any() and not codes[1, 128:].any() and not scales[0].any()
+    fine = np.repeat(np.isfinite(scales), 128, 1)
+    assert np.array_equal(codes[fine], want[fine])
+    assert not codes[:, cols:].any()
+
+
+def test_norm_of_tiny_and_huge_values(lib):
+    """Blocks whose scale or its inverse leaves fp32's normal numbers: exact codes."""
+    y = np.random.default_rng(6).standard_normal((6, 256)).astype(np.float32)
+    y *= np.float32([1e-44, 1e-40, 1e-37, 1e-18, 1e18, 8e37])[:, None]
+    _check_norm(lib, 6, 256, s.F32, "", d={"y": y.astype(np.float64)})
+
+
+# ---- weights ----
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("transposed", [0, 1])
+@pytest.mark.parametrize("n,k,gap,shift", [(1, 1, 0, 0), (1, 200, 3, 1), (200, 1, 0, 0), (128, 128, 0, 0), (127, 129, 0, 0), (130, 257, 1, 1), (256, 384, 8, 0), (515, 70, 0, 3),
+                                           (64, 1000, 0, 0), (1000, 640, 2, 2)])
+def test_quantize_weights(lib, dtype, transposed, n, k, gap, shift):
+    r = np.random.default_rng(n + k)
+    w = _seen(r.standard_normal((n, k)) * np.exp(r.standard_normal((n, 1))), dtype).astype(np.float32)
+    if n > 129:
+        w[128:] = 0  # a block of zeros
+    _check_weights(lib, w, dtype, transposed, gap, shift)
+
+
+def _check_weights(lib, w, dtype, transposed, gap=0, shift=0):
+    n, k = w.shape
+    lies = w if transposed else np.ascontiguousarray(w.T)
+    ld = lies.shape[1] + gap
+    m = Rows(lies.shape, dtype, ld, shift, lies, hole=np.nan)
+    codes, scales = Bytes((n, q.padded(k))), Bytes((q.padded(n) // 128, q.padded(k) // 128), np.float32)
+    _call(lib, "seera_hip_quantize_weights_f8", (m.ptr, codes.ptr, scales.ptr, n, k, ld, transposed, dtype))
+    want, want_scales = q.quantize_weights(w)
+    assert np.array_equal(scales.values(), want_scales, equal_nan=True)
+    fine = np.repeat(np.repeat(np.isfinite(want_scales), 128, 1), 128, 0)[:n]
+    assert np.array_equal(codes.values()[fine], want[fine])
+
+
+@pytest.mark.parametrize("transposed", [0, 1])
+def test_quantize_values_out_of_the_ordinary(lib, transposed):
+    w = np.random.default_rng(7).standard_normal((260, 400)).astype(np.float32)
+    w[:128, :128] *= np.float32(1e-43)
+    w[:128, 128:256] *= np.float32(5e37)
+    w[130, 5], w[259, 399] = np.nan, -np.inf
+    _check_weights(lib, w, s.F32, transposed)
+
+
+# ---- products ----
+
+
+def _operands(m, n, k, seed, bias):
+    r = np.random.default_rng(seed)
+    a = (r.standard_normal((m, k)) * np.exp(r.standard_normal((m, 1)))).astype(np.float32)
+    w = r.standard_normal((n, k)).astype(np.float32)
+    w *= np.repeat(np.exp(r.standard_normal(n // 128 + 1)), 128)[:n, None].astype(np.float32)  # blocks differ
+    return (*q.quantize_rows(a), *q.quantize_weights(w)), r.standard_normal(n).astype(np.float32) if bias else None
+
+
+def _matmul(lib, ops, n, k, bias, dtype, gap=0, shift=0, stream=None):
+    m = ops[0].shape[0]
+    dev = [Bytes(x.shape, x.dtype, x) for x in ops]
+    b = Bytes(bias.shape, np.float32, bias) if bias is not None else None
+    c = Rows((m, n), dtype, n + gap, shift)
+    _call(lib, "seera_hip_matmul_f8", (*[x.ptr for x in dev], b.ptr if b else None, c.ptr, m, n, k, n + gap, dtype), stream)
+    return c.values()
+
+
+def _check_matmul(lib, m, n, k, dtype=s.F32, bias=False, seed=1, **kw):
+    ops, b = _operands(m, n, k, seed, bias)
+    got = _matmul(lib, ops, n, k, b, dtype, **kw)
+    want, bound = q.matmul(*ops, b, fp32=dtype == s.F32)
+    _close(got, want, bound, dtype, "C")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 1000, 129), (2, 16, 128), (15, 17, 127), (16, 128, 256), (17, 129, 640), (33, 130, 1000), (64, 64, 384), (65, 200, 2049),
+                                   (100, 301, 128), (128, 256, 512), (129, 257, 300), (200, 515, 1100), (300, 96, 4096)])
+def test_matmul_sizes(lib, dtype, m, n, k):
+    _check_matmul(lib, m, n, k, dtype, bias=(m + n) % 2 == 0, seed=k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(512, 1024, 256), (1000, 2000, 640), (2050, 1300, 1152), (4096, 512, 128), (256, 4096, 1500), (700, 5001, 257)])
+def test_matmul_many_tiles(lib, dtype, m, n, k):
+    _check_matmul(lib, m, n, k, dtype, bias=n % 2 == 1, seed=m)
+
+
+@pytest.mark.parametrize("m", [1, 3, 40, 300, 1100])
+@pytest.mark.parametrize("gap,shift", [(0, 1), (1, 0), (3, 2), (64, 4)])
+def test_matmul_layouts(lib, stream, m, gap, shift):
+    for dtype in DTYPES:
+        _check_matmul(lib, m, 260, 300, dtype, bias=True, gap=gap, shift=shift, stream=stream)
+
+
+@pytest.mark.parametrize("m", [1, 2, 8, 16, 17, 32, 48, 64, 96, 128, 192, 256, 384, 768])
+def test_matmul_rows_do_not_depend_on_the_batch_but_for_rounding(lib, m):
+    """Every number of rows, with a K of many blocks."""
+    _check_matmul(lib, m, 384, 3001, s.BF16, seed=m)
+
+
+@pytest.mark.parametrize("m", [1, 20, 700])
+def test_matmul_without_k(lib, m):
+    """K == 0: the bias, or zeros."""
+    for bias in (np.arange(9, dtype=np.float32), None):
+        b = Bytes((9,), np.float32, bias) if bias is not None else None
+        c = Rows((m, 9), s.F32)
+        capi.call("seera_hip_matmul_f8", None, None, None, None, b.ptr if b else None, c.ptr, m, 9, 0, 9, s.F32)
+        assert np.array_equal(c.values(), np.tile(bias if bias is not None else np.zeros(9), (m, 1)))
+
+
+@pytest.mark.parametrize("m", [1, 30, 600])
+def test_matmul_nan_stays_in_its_row_or_columns(lib, m):
+    """A scale of NaN of A makes its row NaN, one of W its 128 columns; an fp16 result
+    beyond its range is infinite."""
+    ops, _ = _operands(m, 300, 400, 9, False)
+    a, sa, w, sw = (x.copy() for x in ops)
+    sa[m // 2, 1] = np.nan
+    got = _matmul(lib, (a, sa, w, sw), 300, 400, None, s.F32)
+    assert np.isnan(got[m // 2]).all() and np.isfinite(np.delete(got, m // 2, 0)).all()
+    sw[1, 2] = np.nan
+    got = np.delete(_matmul(lib, (a, sa, w, sw), 300, 400, None, s.F32), m // 2, 0)
+    assert np.isnan(got[:, 128:256]).all() and np.isfinite(got[:, :128]).all() and np.isfinite(got[:, 256:]).all()
+    big = np.full_like(ops[1], 1e6)
+    want, bound = q.matmul(ops[0], big, ops[2], ops[3], fp32=False)
+    got = _matmul(lib, (ops[0], big, ops[2], ops[3]), 300, 400, None, s.F16)
+    sure = np.abs(want) - bound > 65520
+    assert sure.any() and np.array_equal(got[sure], np.copysign(np.inf, want[sure]))
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 200, 700), (64, 512, 1024), (512, 512, 512), (1024, 700, 384)])
+def test_matmul_of_whole_numbers_is_exact(lib, m, n, k):
+    """Small whole numbers with scales of powers of two: every sum is a whole number
+    below 2^24, so that no rounding happens and a term in a wrong place shows."""
+    r = np.random.default_rng(m)
+    kp = q.padded(k)
+    a, w = np.zeros((m, kp)), np.zeros((n, kp))
+    a[:, :k], w[:, :k] = r.integers(-8, 9, (m, k)), r.integers(-8, 9, (n, k))
+    sa, sw = 2.0 ** r.integers(0, 3, (m, kp // 128)), 2.0 ** r.integers(0, 3, (q.padded(n) // 128, kp // 128))
+    ops = (q.encode(a), sa.astype(np.float32), q.encode(w), sw.astype(np.float32))
+    want, _ = q.matmul(*ops)
+    assert np.abs(want).max() < 2**24
+    assert np.array_equal(_matmul(lib, ops, n, k, None, s.F32), want)
+
+
+def test_matmul_rows_beyond_32_bits(lib):
+    """A result whose rows lie so far apart that places in it pass 2^32 bytes."""
+    m, n, k, ld = 40, 20, 128, 60_000_000
+    ops, _ = _operands(m, n, k, 11, False)
+    dev = [Bytes(x.shape, x.dtype, x) for x in ops]
+    c = DeviceBuffer(((m - 1) * ld + n) * 2)
+    capi.call("seera_hip_matmul_f8", *[x.ptr for x in dev], None, c.ptr, m, n, k, ld, s.BF16)
+    want, bound = q.matmul(*ops, fp32=False)
+    for i in (0, 17, 39):
+        row = np.empty(n, np.uint16)
+        capi.check(lib.seera_hip_memcpy_d2h(row.ctypes.data, c.ptr + i * ld * 2, row.nbytes))
+        _close(s.load(row, s.BF16), want[i], bound[i], s.BF16, "C")
+    c.close()
+    capi.check(lib.seera_hip_empty_cache())
+
+
+# ---- sampling ----
+
+
+def _sample(lib, l, u, dtype, gap=0, shift=0, logp=True, stream=None, **params):
+    rows, vocab = l.shape
+    z = Rows((rows, vocab), dtype, vocab + gap, shift, l, hole=np.nan)
+    kinds = {"temperature": np.float32, "top_k": np.int32, "top_p": np.float32, "min_p": np.float32}
+    dev = {k: Bytes((rows,), t, np.broadcast_to(np.asarray(params[k], t), (rows,))) if k in params else None for k, t in kinds.items()}
+    un, tokens, lp = Bytes((rows,), np.float32, u), Bytes((rows,), np.int32), Bytes((rows,), np.float32)
+    _call(lib, "seera_hip_sample", (z.ptr, un.ptr, *[dev[k].ptr if dev[k] else None for k in kinds], tokens.ptr, lp.ptr if logp else None, rows, vocab, vocab + gap, dtype), stream)
+    return tokens.values(), lp.values() if logp else None
+
+
+def _check_sample(lib, l, u, dtype, **kw):
+    """Tokens are equal: the weights of both sides are the same whole numbers but for a
+    last place of the exponential, so that only a u within 2^-30 of a border could fall on
+    its other side (a seed that has one is not used). logp is one rounding to fp32, of a
+    value that is right to about 2^-36 and of weights that are right to 2^-40 of the largest."""
+    params = {k: np.broadcast_to(np.asarray(kw[k]), (len(l),)) for k in ("temperature", "top_k", "top_p", "min_p") if k in kw}
+    tokens, logp = _sample(lib, l, u, dtype, **kw)
+    for i, row in enumerate(_seen(l, dtype)):
+        one = {k: (float if k != "top_k" else int)(np.float32(v[i]) if k != "top_k" else v[i]) for k, v in params.items()}
+        token, lp, near = q.sample_row(row, float(np.float32(u[i])), **one)
+        assert tokens[i] == token, (i, tokens[i], token, near, one)
+        if logp is not None:
+            assert logp[i] == lp if not np.isfinite(lp) else abs(logp[i] - lp) <= 2 * s.U * abs(lp) + 2.0**-36, (i, logp[i], lp)
+
+
+def _logits(rows, vocab, seed, scale=2.5):
+    r = np.random.default_rng(seed)
+    l = r.standard_normal((rows, vocab)) * scale
+    l += np.where(r.random((rows, vocab)) < 10 / vocab, 6, 0)
+    return l, r.random(rows, np.float32)
+
+
+CUTS = [{}, {"temperature": 0.7}, {"top_k": 5}, {"top_p": 0.9}, {"min_p": 0.05}, {"top_k": 40, "top_p": 0.8, "temperature": 1.3}, {"top_k": 300, "top_p": 0.95, "min_p": 0.02}]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cuts", range(len(CUTS)))
+def test_sample_cuts(lib, dtype, cuts):
+    for vocab in (50, 1000, 5003):
+        l, u = _logits(12, vocab, cuts + vocab)
+        _check_sample(lib, l, u, dtype, **CUTS[cuts])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1, 2, 3, 7, 8, 9, 63, 64, 65, 255, 257, 511, 512, 513, 2047, 4097, 8191, 8193, 16385, 32768, 65537, 131072])
+def test_sample_sizes(lib, dtype, vocab):
+    l, u = _logits(3, vocab, vocab)
+    _check_sample(lib, l, u, dtype)
+    _check_sample(lib, l, u, dtype, top_k=max(1, vocab // 3), top_p=0.97, temperature=[0.8, 1.5, 3.0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gap,shift", [(0, 1), (1, 0), (3, 2), (64, 4)])
+def test_sample_layouts(lib, dtype, gap, shift, stream):
+    l, u = _logits(7, 1999, gap)
+    _check_sample(lib, l, u, dtype, gap=gap, shift=shift, top_k=100, top_p=0.9, stream=stream)
+    _check_sample(lib, l, u, dtype, gap=gap, shift=shift, logp=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("values", [1, 2, 5])
+def test_sample_ties(lib, dtype, values):
+    """Few different values: every cut falls among equals, and they are kept by index."""
+    r = np.random.default_rng(values)
+    l = r.integers(0, values, (24, 3000)).astype(np.float64) * 0.5 - 1.0
+    u = r.random(24, np.float32)
+    u[:4] = [0.0, 0.99999994, 0.5, 1e-30]
+    _check_sample(lib, l, u, dtype, top_k=r.integers(1, 3001, 24))
+    _check_sample(lib, l, u, dtype, top_p=r.random(24))
+    _check_sample(lib, l, u, dtype, top_k=r.integers(1, 3001, 24), top_p=r.random(24), temperature=0.3)
+    _check_sample(lib, l, u, dtype, min_p=r.random(24))
+
+
+@pytest.mark.parametrize("vocab", [10, 700, 9000])
+def test_sample_border_values_of_the_parameters(lib, vocab):
+    l, u = _logits(16, vocab, 3)
+    inf, nan = np.inf, np.nan
+    _check_sample(lib, l, u, s.F32, temperature=[0, -1, nan, 1e-30, 1e-44, inf, 100, 1e-3, 0.5, 1, 1, 2, 2, 1e30, 1e-5, 0.01])
+    _check_sample(lib, l, u, s.F32, top_k=[0, -5, 1, 2, vocab - 1, vocab, vocab + 1, 2**31 - 1, 3, -2**31, 5, 6, 7, 8, 9, 10])
+    _check_sample(lib, l, u, s.F32, top_p=[0, -1, 1, 2, nan, 1e-40, 0.99999994, 0.5, 0.1, 0.01, 0.9, 1e-7, inf, -inf, 0.3, 0.7])
+    _check_sample(lib, l, u, s.F32, min_p=[0, -1, 1, 2, nan, 1e-40, 0.99999994, 0.5, 0.1, 0.01, 0.9, 1e-7, inf, -inf, 0.3, 0.7])
+    _check_sample(lib, l, [0, 1, 2, -1, nan, inf, -inf, 0.99999994, 1e-45, 0.5, 0.25, 0.75, 0.1, 0.9, 0.999, 0.001], s.F32, top_k=50)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [9, 600, 5000])
+def test_sample_masks(lib, dtype, vocab):
+    """Rows where little or nothing may be drawn, and logits that are not finite."""
+    l, u = _logits(14, vocab, 4)
+    inf, nan = np.inf, np.nan
+    l[0] = -inf
+    l[1] = nan
+    l[2], l[2, vocab // 2] = -inf, -3.0
+    l[3, ::2], l[4, 1::2] = -inf, nan
+    l[5, [2, vocab - 1]] = inf
+    l[6], l[6, vocab - 1] = -inf, inf
+    l[7], l[7, 3] = nan, -inf
+    l[8] = np.finfo(np.float32).min if dtype != s.F16 else -65504.0
+    l[9], l[9, 4] = l[8], 0.0
+    l[10] = -l[8]
+    l[11], l[11, 5] = inf, nan
+    l[12, ::3] = l[8, 0]
+    l[13, :] = 0.0
+    l[13, ::2] = -0.0
+    for kw in ({}, {"top_k": 3}, {"top_p": 0.6}, {"min_p": 0.3}, {"top_k": 4, "top_p": 0.5, "temperature": 0.9}, {"temperature": 0.0}, {"temperature": inf},
+               {"top_k": vocab // 2 + 1, "temperature": inf}):
+        _check_sample(lib, l, u, dtype, **kw)
+
+
+def test_sample_without_a_vocabulary(lib):
+    tokens, u = Bytes((3,), np.int32), Bytes((3,), np.float32, np.zeros(3))
+    capi.call("seera_hip_sample", None, u.ptr, None, None, None, None, tokens.ptr, None, 3, 0, 0, 0)
+    assert np.all(tokens.values() == -1)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 33, 300])
+def test_sample_rows(lib, rows):
+    l, u = _logits(rows, 3000, rows)
+    r = np.random.default_rng(rows)
+    _check_sample(lib, l, u, s.BF16, temperature=np.where(r.random(rows) < 0.2, 0, 1.1), top_k=r.integers(0, 200, rows), top_p=0.5 + 0.6 * r.random(rows), min_p=0.1 * r.random(rows))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 262144), (2, 1000003), (1, 1 << 22)])
+def test_sample_long_rows(lib, rows, vocab):
+    l, u = _logits(rows, vocab, 8)
+    _check_sample(lib, l, u, s.F16, top_p=0.9)
+    _check_sample(lib, l, u, s.F32, top_k=vocab // 2, temperature=2.0)
+    _check_sample(lib, l, u, s.F32)
+
+
+def test_sample_of_nearly_equal_logits(lib):
+    """One bin of distances holds every token, and their values differ in the last places."""
+    r = np.random.default_rng(5)
+    l = 1.0 + r.integers(0, 4000, (8, 20000)) * 2.0**-23
+    u = r.random(8, np.float32)
+    _check_sample(lib, l, u, s.F32, top_k=[1, 2, 100, 4999, 10000, 19998, 19999, 7])
+    _check_sample(lib, l, u, s.F32, top_p=[0.001, 0.1, 0.5, 0.9, 0.99, 0.9999, 0.3, 0.7])
+    _check_sample(lib, l, u, s.F32, top_k=15000, top_p=0.5, temperature=1e-4)
+
+
+def test_sample_draws_the_distribution(lib):
+    """A grid of u over one row: each token as often as its share, but for the grid's ends."""
+    n, vocab = 4000, 300
+    l = np.tile(_logits(1, vocab, 6)[0], (n, 1))
+    tokens, logp = _sample(lib, l, (np.arange(n) + 0.5) / n, s.F32, top_k=60, top_p=0.9, temperature=0.8)
+    share = np.bincount(tokens, minlength=vocab) / n
+    seen = np.flatnonzero(share)
+    assert len(seen) <= 60 and np.all(np.diff(tokens) >= 0)
+    p = np.array([np.exp(logp[tokens == t][0].astype(np.float64)) for t in seen])
+    assert np.all(np.abs(share[seen] - p) <= 1.01 / n)
+
+
+# ---- a decoding step of all of them ----
+
+
+class Step:
+    """[y, r] -> norm in 8 bits -> product with quantised weights -> token, as a model's last layer has them."""
+
+    def __init__(self, rows, width, vocab, seed=1):
+        r = np.random.default_rng(seed)
+        self.rows, self.width, self.vocab = rows, width, vocab
+        kp = q.padded(width)
+        self.w = Bytes((width, vocab), np.float32, r.standard_normal((width, vocab)) / np.sqrt(width) * 3)
+        self.codes, self.scales = Bytes((vocab, kp)), Bytes((q.padded(vocab) // 128, kp // 128), np.float32)
+        self.y, self.r = Bytes((rows, width), np.uint16), Bytes((rows, width), np.uint16)
+        self.w2 = Bytes((width,), np.float32, 1 + 0.1 * r.standard_normal(width))
+        self.n, self.ns = Bytes((rows, kp)), Bytes((rows, kp // 128), np.float32)
+        self.logits, self.u = Bytes((rows, vocab), np.uint16), Bytes((rows,), np.float32)
+        self.k, self.p = Bytes((rows,), np.int32, np.full(rows, 50)), Bytes((rows,), np.float32, np.full(rows, 0.9))
+        self.tokens, self.logp = Bytes((rows,), np.int32), Bytes((rows,), np.float32)
+
+    def inputs(self, seed):
+        r = np.random.default_rng(seed)
+        for b, v in ((self.y, s.store(r.standard_normal((self.rows, self.width)), s.BF16)), (self.r, s.store(2 * r.standard_normal((self.rows, self.width)), s.BF16)),
+                     (self.u, r.random(self.rows, np.float32))):
+            capi.check(capi.load().seera_hip_memcpy_h2d(b.ptr, v.ctypes.data, v.nbytes))
+
+    def queue(self, stream, quantize=True):
+        rows, width, vocab = self.rows, self.width, self.vocab
+        if quantize:
+            capi.call("seera_hip_quantize_weights_f8_async", self.w.ptr, self.codes.ptr, self.scales.ptr, vocab, width, vocab, 0, s.F32, stream)
+        capi.call("seera_hip_block_norm_fwd_f8_async", self.y.ptr, None, self.r.ptr, None, None, self.w2.ptr, self.r.ptr, self.n.ptr, self.ns.ptr, rows, width, width, width,
+                  1e-6, 0, s.BF16, stream)
+        capi.call("seera_hip_matmul_f8_async", self.n.ptr, self.ns.ptr, self.codes.ptr, self.scales.ptr, None, self.logits.ptr, rows, vocab, width, vocab, s.BF16, stream)
+        capi.call("seera_hip_sample_async", self.logits.ptr, self.u.ptr, None, self.k.ptr, self.p.ptr, None, self.tokens.ptr, self.logp.ptr, rows, vocab, vocab, s.BF16, stream)
+
+    def results(self):
+        return [b.values() for b in (self.r, self.n, self.ns, self.logits, self.tokens, self.logp)]
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(1, 96, 500), (5, 300, 1999), (40, 512, 3001), (300, 640, 1000)])
+def test_step(lib, stream, rows, width, vocab):
+    """Each operator's output against the oracle's on the input that it had."""
+    step = Step(rows, width, vocab)
+    step.inputs(3)
+    y, r = (s.load(b.values(), s.BF16) for b in (step.y, step.r))
+    step.queue(stream)
+    capi.check(lib.seera_hip_stream_synchronize(stream))
+    kept, n, ns, logits, tokens, logp = step.results()
+    kept = s.load(kept, s.BF16)
+    assert np.array_equal(kept, _seen(y + r, s.BF16))
+    q.check_codes(n, ns, *q.norm_values(kept, step.w2.values().astype(np.float64), 1e-6))
+    want, bound = q.matmul(n, ns, *q.quantize_weights(np.ascontiguousarray(step.w.values().T)), fp32=False)
+    l = s.load(logits, s.BF16)
+    _close(l, want, bound, s.BF16, "logits")
+    u = step.u.values()
+    assert [q.sample_row(l[i], float(u[i]), top_k=50, top_p=float(np.float32(0.9)))[0] for i in range(rows)] == tokens.tolist()
+
+
+@pytest.mark.parametrize("rows", [1, 70, 300])
+def test_step_in_a_graph(lib, stream, rows):
+    """Replays with new inputs between eager work of other sizes: the eager results' bits."""
+    step, other = Step(rows, 300, 1999), Step(11, 700, 900)
+    want = []
+    for seed in range(4):
+        step.inputs(seed)
+        step.queue(stream)
+        capi.check(lib.seera_hip_stream_synchronize(stream))
+        want.append(step.results())
+    capi.check(lib.seera_hip_graph_capture_begin(stream))
+    graph = ctypes.c_void_p()
+    try:
+        step.queue(stream, quantize=False)
+    finally:
+        status = lib.seera_hip_graph_capture_end(stream, ctypes.byref(graph))
+    capi.check(status)
+    try:
+        for seed in (2, 0, 3, 1):
+            step.inputs(seed)
+            capi.check(lib.seera_hip_graph_launch(graph.value, stream))
+            capi.check(lib.seera_hip_stream_synchronize(stream))
+            assert all(np.array_equal(a, b) for a, b in zip(step.results(), want[seed]))
+            other.inputs(seed)
+            other.queue(None)
+            capi.check(lib.seera_hip_synchronize())
+    finally:
+        capi.check(lib.seera_hip_graph_destroy(graph))
+
+
+def test_two_streams(lib):
+    """The same calls on two streams at once: each stream's results are its own."""
+    streams = []
+    for _ in range(2):
+        st = ctypes.c_void_p()
+        capi.check(lib.seera_hip_stream_create(ctypes.byref(st)))
+        streams.append(st.value)
+    steps = [Step(64, 512, 5000, seed) for seed in (1, 2)]
+    try:
+        want = []
+        for i, step in enumerate(steps):
+            step.inputs(i)
+            step.queue(streams[i])
+            capi.check(lib.seera_hip_stream_synchronize(streams[i]))
+            want.append(step.results())
+        for _ in range(5):
+            for i, step in enumerate(steps):
+                step.inputs(i)
+            for i, step in enumerate(steps):
+                step.queue(streams[i])
+            for st in streams:
+                capi.check(lib.seera_hip_stream_synchronize(st))
+            for i, step in enumerate(steps):
+                assert all(np.array_equal(a, b) for a, b in zip(step.results(), want[i]))
+    finally:
+        for st in streams:
+            lib.seera_hip_stream_destroy(st)
