@@ -149,9 +149,207 @@ int launch_split(const MatmulF8& g, hipStream_t st) {
     return SEERA_OK;
 }
 
+// ---- tiles through LDS ----
+
+// 4 bytes per lane as dma16 moves 16.
+__device__ __forceinline__ void dma4(dma_rsrc_t r, void* lds, uint32_t voff, uint32_t soff) {
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(at), "v"(voff), "s"(r), "s"(soff)
+                 : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+// A tile of R rows of 128 codes in LDS, its 16-byte pieces moved within a row so that
+// the eight rows that eight lanes read at a time lie in eight places. SPREAD: those
+// rows are four of one group of SPREAD rows and four of the next (W), else
+// consecutive (A).
+template <int R, int SPREAD>
+struct CodeTile {
+    static __device__ __forceinline__ int turn(int row) { return SPREAD ? (row & 3) | (row / (SPREAD ? SPREAD : 1) & 1) << 2 : row & 7; }
+    // Where a lane's two pieces of a row lie; a multiple of 16 rows further (4 rows inside a
+    // group of W) they lie as many rows of 128 bytes further.
+    static __device__ __forceinline__ int place(int row, int g) { return row * 128 + ((g ^ turn(row)) << 4); }
+    static __device__ __forceinline__ intx8 read(const uint8_t* tile, int place) {
+        const intx4 lo = *(const intx4*)(tile + place), hi = *(const intx4*)(tile + (place ^ 64));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+// A tile of BM x BN by WM x WN waves; two stages of LDS, one slice of 128 along K each,
+// filled by DMA. In a wave, W's fragments of a slice stay in registers and A's
+// pass by: NT products of one, while the sums of the products before it are scaled and
+// added. Row r of the j-th 16 of W is column 4 NT (r / 4) + 4 j + r % 4 of the
+// wave's, so that a lane holds 4 NT values next to each other of a row of C.
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, int tiles_m, int tiles_n) {
+    constexpr int THREADS = 64 * WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
+    constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, STAGE = A_BYTES + W_BYTES + WM * WN * 256;
+    constexpr int A_LOADS = BM * 8 / THREADS, W_LOADS = BN * 8 / THREADS;
+    static_assert(BM * 8 % THREADS == 0 && BN * 8 % THREADS == 0 && BM / 64 < WM * WN && BN % 128 == 0 && 128 % (16 * NT) == 0 && MT >= 2, "shapes of a tile");
+    typedef CodeTile<BM, 0> TA;
+    typedef CodeTile<BN, 4 * NT> TW;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the blocks of one XCD walk groups of 4 tile rows column by column
+    const int id = xcd_order(blockIdx.x, tiles_m * tiles_n);
+    const int group = id / (4 * tiles_n), in_group = id - group * 4 * tiles_n, rows = min(tiles_m - group * 4, 4);
+    const int m0 = (group * 4 + in_group % rows) * BM, n0 = in_group / rows * BN;
+    const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    const uint32_t kp = (uint32_t)g.blocks * kF8Block;
+
+    // rows past the end repeat the last one: their results are not stored
+    uint32_t ao[A_LOADS], wo[W_LOADS];
+#pragma unroll
+    for (int p = 0; p < A_LOADS; ++p) {
+        const int i = p * THREADS + tid, row = i >> 3;
+        ao[p] = (uint32_t)min(row, g.m - 1 - m0) * kp + (((i & 7) ^ TA::turn(row)) << 4);
+    }
+#pragma unroll
+    for (int p = 0; p < W_LOADS; ++p) {
+        const int i = p * THREADS + tid, row = i >> 3;
+        wo[p] = (uint32_t)min(row, g.n - 1 - n0) * kp + (((i & 7) ^ TW::turn(row)) << 4);
+    }
+    // the scales of A's rows by the first BM / 64 waves, W's by the next (the others get zeros)
+    const bool a_scales = wave < BM / 64;
+    const uint32_t so = (a_scales ? (uint32_t)min(tid, g.m - 1 - m0) : (uint32_t)min(lane, (g.n - 1) / kF8Block - n0 / kF8Block)) * (uint32_t)g.blocks * 4u;
+    const uint8_t *pa = g.a + (int64_t)m0 * kp, *pw = g.w + (int64_t)n0 * kp;
+    const float* ps = a_scales ? g.a_scales + (int64_t)m0 * g.blocks : g.w_scales + (int64_t)(n0 / kF8Block) * g.blocks;
+    constexpr int LOADS = A_LOADS + W_LOADS + 1;
+    // Load l of a slice, `bytes` of memory being there (0: none, for zeros). No branch: the
+    // loop below stays one block of code, or its sums are moved to its end.
+    auto load = [&](int l, uint8_t* stage, uint32_t bytes) {
+        uint8_t* to = stage + wave * 1024;
+        if (l < A_LOADS) {
+            dma16(make_dma_rsrc(pa, bytes), (half_t*)(to + l * THREADS * 16), ao[l < A_LOADS ? l : 0], 0u);
+        } else if (l < A_LOADS + W_LOADS) {
+            const int p = l < A_LOADS || l >= A_LOADS + W_LOADS ? 0 : l - A_LOADS;
+            dma16(make_dma_rsrc(pw, bytes), (half_t*)(to + A_BYTES + p * THREADS * 16), wo[p], 0u);
+        } else {
+            dma4(make_dma_rsrc(ps, wave <= BM / 64 ? bytes : 0u), stage + A_BYTES + W_BYTES + wave * 256, so, 0u);
+            pa += 128, pw += 128, ps += 1;
+        }
+    };
+
+    floatx4 acc[MT][NT], sums[2][NT];
+    Codes<T> w[NT], a[2];
+    float scale[MT], last = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        sums[1][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int r = lane & 15, gk = lane >> 4;
+    const int a_place = TA::place(wm + r, gk), w_place = TW::place(wn + 4 * NT * (r >> 2) + (r & 3), gk);
+    auto read_a = [&](const uint8_t* stage, int i) { a[i & 1] = Codes<T>(TA::read(stage + i * 2048, a_place)); };
+    auto read_w = [&](const uint8_t* stage) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) w[j] = Codes<T>(TW::read(stage + A_BYTES + j * 512, w_place));
+    };
+    auto read_scales = [&](const uint8_t* stage) {
+        const float* s = (const float*)(stage + A_BYTES + W_BYTES);
+        const float sw = s[BM + wn / kF8Block];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) scale[i] = s[wm + 16 * i + r] * sw;
+    };
+    auto add = [&](int i, int j, float by) {  // the sums of step i
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sums[i & 1][j][e], by, acc[i][j][e]);
+    };
+
+    const int slices = g.blocks;
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) load(l, smem, kMaxTileSpanBytes);
+    wait_vm<0>();
+    lds_barrier();
+    read_w(smem);
+    read_a(smem, 0);
+    read_scales(smem);
+    for (int s = 0; s < slices; ++s) {
+        const uint8_t* now = smem + (s & 1) * STAGE;
+        uint8_t* next = smem + ((s + 1) & 1) * STAGE;
+        const uint32_t bytes = s + 1 < slices ? (uint32_t)kMaxTileSpanBytes : 0u;
+#pragma unroll
+        for (int i = 0; i < MT - 1; ++i) {
+            read_a(now, i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                sums[i & 1][j] = products(w[j], a[i & 1]);
+                if (i == 0) add(MT - 1, j, last);
+                else add(i - 1, j, scale[i ? i - 1 : 0]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int l = i * LOADS / (MT - 1); l < (i + 1) * LOADS / (MT - 1); ++l) load(l, next, bytes);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        wait_vm<0>();
+        lds_barrier();
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            sums[(MT - 1) & 1][j] = products(w[j], a[(MT - 1) & 1]);
+            add(MT - 2, j, scale[MT - 2]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        last = scale[MT - 1];
+        // (after the last slice, of a stage that nothing uses)
+        read_w(next);
+        read_a(next, 0);
+        read_scales(next);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) add(MT - 1, j, last);
+
+    const int n = n0 + wn + 4 * NT * gk;
+    float bias[4 * NT];
+#pragma unroll
+    for (int e = 0; e < 4 * NT; ++e) bias[e] = g.bias && n + e < g.n ? g.bias[n + e] : 0.f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int m = m0 + wm + 16 * i + r;
+        if (m >= g.m) continue;
+        T* c = (T*)g.c + (int64_t)m * g.ldc + n;
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int q = 0; q < 4 * NT / N; ++q) {
+            Pack<T, N> v;
+#pragma unroll
+            for (int e = 0; e < N; ++e) v.v[e] = from_f32<T>(acc[i][(q * N + e) / 4][e % 4] + bias[q * N + e]);
+            if (n + (q + 1) * N <= g.n) {
+                __builtin_memcpy(c + q * N, &v, 16);  // at any alignment of T, as one access
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (n + q * N + e < g.n) c[q * N + e] = v.v[e];
+            }
+        }
+    }
+}
+
+template <class T, int BM, int BN, int WM, int WN>
+int launch_tiles(const MatmulF8& g, hipStream_t st) {
+    constexpr int lds = 2 * ((BM + BN) * 128 + WM * WN * 256);
+    auto kern = matmul_f8_tiles<T, BM, BN, WM, WN>;
+    if (lds > 65536)
+        SEERA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
+    hipLaunchKernelGGL(kern, dim3((uint32_t)(tiles_m * tiles_n)), dim3(64 * WM * WN), lds, st, g, tiles_m, tiles_n);
+    SEERA_HIP_TRY(hipGetLastError());
+    return SEERA_OK;
+}
+
 template <class T>
 int launch_t(const MatmulF8& g, hipStream_t st) {
     if (g.m <= 16) return launch_split<T, 1, 1, 8>(g, st);
+    if (g.m >= 512 && g.blocks) {
+        if constexpr (sizeof(T) == 4) return launch_tiles<T, 128, 128, 2, 2>(g, st);
+        else return launch_tiles<T, 256, 256, 2, 4>(g, st);
+    }
     return launch_split<T, 4, 2, 4>(g, st);
 }
 
