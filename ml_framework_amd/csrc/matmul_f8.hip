@@ -166,12 +166,11 @@ __device__ __forceinline__ void dma4(dma_rsrc_t r, void* lds, uint32_t voff, uin
 // A tile of R rows of 128 codes in LDS, its 16-byte pieces moved within a row so that
 // the eight rows that eight lanes read at a time lie in eight places. SPREAD: those
 // rows are four of one group of SPREAD rows and four of the next (W), else
-// consecutive (A).
-template <int R, int SPREAD>
+// consecutive.
+template <int SPREAD>
 struct CodeTile {
     static __device__ __forceinline__ int turn(int row) { return SPREAD ? (row & 3) | (row / (SPREAD ? SPREAD : 1) & 1) << 2 : row & 7; }
-    // Where a lane's two pieces of a row lie; a multiple of 16 rows further (4 rows inside a
-    // group of W) they lie as many rows of 128 bytes further.
+    // Where a lane's two pieces of a row lie; rows that have the same turn lie a multiple of 128 further.
     static __device__ __forceinline__ int place(int row, int g) { return row * 128 + ((g ^ turn(row)) << 4); }
     static __device__ __forceinline__ intx8 read(const uint8_t* tile, int place) {
         const intx4 lo = *(const intx4*)(tile + place), hi = *(const intx4*)(tile + (place ^ 64));
@@ -182,16 +181,17 @@ struct CodeTile {
 // A tile of BM x BN by WM x WN waves; two stages of LDS, one slice of 128 along K each,
 // filled by DMA. In a wave, W's fragments of a slice stay in registers and A's
 // pass by: NT products of one, while the sums of the products before it are scaled and
-// added. Row r of the j-th 16 of W is column 4 NT (r / 4) + 4 j + r % 4 of the
-// wave's, so that a lane holds 4 NT values next to each other of a row of C.
+// added. With 16-bit results W's rows are permuted so that a lane holds 8 values next to
+// each other of a row of C: 16 bytes, and four lanes 64, as with fp32 without it.
 template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, int tiles_m, int tiles_n) {
     constexpr int THREADS = 64 * WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
     constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, STAGE = A_BYTES + W_BYTES + WM * WN * 256;
     constexpr int A_LOADS = BM * 8 / THREADS, W_LOADS = BN * 8 / THREADS;
-    static_assert(BM * 8 % THREADS == 0 && BN * 8 % THREADS == 0 && BM / 64 < WM * WN && BN % 128 == 0 && 128 % (16 * NT) == 0 && MT >= 2, "shapes of a tile");
-    typedef CodeTile<BM, 0> TA;
-    typedef CodeTile<BN, 4 * NT> TW;
+    static_assert(BM * 8 % THREADS == 0 && BN * 8 % THREADS == 0 && BM / 64 < WM * WN && BN % 128 == 0 && 128 % (16 * NT) == 0 && NT % 2 == 0 && MT >= 2, "shapes of a tile");
+    constexpr int N = 16 / sizeof(T), JJ = N / 4;  // values, and products' rows of 4, in 16 bytes
+    typedef CodeTile<0> TA;
+    typedef CodeTile<JJ == 1 ? 0 : N> TW;
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the blocks of one XCD walk groups of 4 tile rows column by column
@@ -244,11 +244,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, i
         sums[1][j] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
     const int r = lane & 15, gk = lane >> 4;
-    const int a_place = TA::place(wm + r, gk), w_place = TW::place(wn + 4 * NT * (r >> 2) + (r & 3), gk);
+    const int a_place = TA::place(wm + r, gk), w_place = TW::place(wn + N * (r >> 2) + (r & 3), gk);
     auto read_a = [&](const uint8_t* stage, int i) { a[i & 1] = Codes<T>(TA::read(stage + i * 2048, a_place)); };
     auto read_w = [&](const uint8_t* stage) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j] = Codes<T>(TW::read(stage + A_BYTES + j * 512, w_place));
+        for (int j = 0; j < NT; ++j) w[j] = Codes<T>(TW::read(stage + A_BYTES + (16 * JJ * (j / JJ) + 4 * (j % JJ)) * 128, w_place));
     };
     auto read_scales = [&](const uint8_t* stage) {
         const float* s = (const float*)(stage + A_BYTES + W_BYTES);
@@ -305,27 +305,37 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, i
 #pragma unroll
     for (int j = 0; j < NT; ++j) add(MT - 1, j, last);
 
-    const int n = n0 + wn + 4 * NT * gk;
-    float bias[4 * NT];
+    typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));  // at any alignment of T
+    const bool whole = m0 + BM <= g.m && n0 + BN <= g.n;
 #pragma unroll
-    for (int e = 0; e < 4 * NT; ++e) bias[e] = g.bias && n + e < g.n ? g.bias[n + e] : 0.f;
+    for (int q = 0; q < NT / JJ; ++q) {
+        const int n = n0 + wn + 16 * JJ * q + N * gk;
+        float bias[N];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int m = m0 + wm + 16 * i + r;
-        if (m >= g.m) continue;
-        T* c = (T*)g.c + (int64_t)m * g.ldc + n;
-        constexpr int N = 16 / sizeof(T);
-#pragma unroll
-        for (int q = 0; q < 4 * NT / N; ++q) {
-            Pack<T, N> v;
-#pragma unroll
-            for (int e = 0; e < N; ++e) v.v[e] = from_f32<T>(acc[i][(q * N + e) / 4][e % 4] + bias[q * N + e]);
-            if (n + (q + 1) * N <= g.n) {
-                __builtin_memcpy(c + q * N, &v, 16);  // at any alignment of T, as one access
+        for (int e = 0; e < N; ++e) bias[e] = 0.f;
+        if (g.bias) {
+            if (whole) {
+                __builtin_memcpy(bias, g.bias + n, sizeof(bias));
             } else {
 #pragma unroll
+                for (int e = 0; e < N; ++e) bias[e] = g.bias[min(n + e, g.n - 1)];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int m = m0 + wm + 16 * i + r;
+            T* c = (T*)g.c + (int64_t)m * g.ldc + n;
+            Pack<T, N> v;
+#pragma unroll
+            for (int e = 0; e < N; ++e) v.v[e] = from_f32<T>(acc[i][q * JJ + e / 4][e % 4] + bias[e]);
+            if (whole || (m < g.m && n + N <= g.n)) {
+                Bits bits;
+                __builtin_memcpy(&bits, &v, 16);
+                __builtin_nontemporal_store(bits, (Bits*)c);
+            } else if (m < g.m) {
+#pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (n + q * N + e < g.n) c[q * N + e] = v.v[e];
+                    if (n + e < g.n) c[e] = v.v[e];
             }
         }
     }
