@@ -213,9 +213,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, i
         const int i = p * THREADS + tid, row = i >> 3;
         wo[p] = (uint32_t)min(row, g.n - 1 - n0) * kp + (((i & 7) ^ TW::turn(row)) << 4);
     }
-    // the scales of A's rows by the first BM / 64 waves, W's by the next (the others get zeros)
+    // the scales of A's rows by the first BM / 64 waves, so that a lane finds its MT ones next
+    // to each other; W's by the next (the others get zeros)
     const bool a_scales = wave < BM / 64;
-    const uint32_t so = (a_scales ? (uint32_t)min(tid, g.m - 1 - m0) : (uint32_t)min(lane, (g.n - 1) / kF8Block - n0 / kF8Block)) * (uint32_t)g.blocks * 4u;
+    const int scale_row = tid / (16 * MT) * (16 * MT) + tid % MT * 16 + tid % (16 * MT) / MT;
+    const uint32_t so = (a_scales ? (uint32_t)min(scale_row, g.m - 1 - m0) : (uint32_t)min(lane, (g.n - 1) / kF8Block - n0 / kF8Block)) * (uint32_t)g.blocks * 4u;
     const uint8_t *pa = g.a + (int64_t)m0 * kp, *pw = g.w + (int64_t)n0 * kp;
     const float* ps = a_scales ? g.a_scales + (int64_t)m0 * g.blocks : g.w_scales + (int64_t)(n0 / kF8Block) * g.blocks;
     constexpr int LOADS = A_LOADS + W_LOADS + 1;
@@ -234,76 +236,86 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, i
         }
     };
 
-    floatx4 acc[MT][NT], sums[2][NT];
-    Codes<T> w[NT], a[2];
-    float scale[MT], last = 0.f;
+    // A slice's products in order: A's fragments one after another, each by all of W's; the last
+    // TAIL of A's by one of W's after another, so that W's registers become free one by one.
+    // Before these, every wave has read all of the slice: its stage is filled anew, with the
+    // slice after the next, while the fragments of the next are read.
+    constexpr int TAIL = 3, HEAD = (MT - TAIL) * NT, ALL = MT * NT, RING = 4, AS = TAIL + 1;
+    static_assert(MT > TAIL && MT % AS == 0 && HEAD >= RING && TAIL * NT >= LOADS && RING <= 2 * TAIL, "room for the steps' work");
+    auto row_of = [](int t) { return t < HEAD ? t / NT : MT - TAIL + (t - HEAD) % TAIL; };
+    auto col_of = [](int t) { return t < HEAD ? t % NT : (t - HEAD) / TAIL; };
+    floatx4 acc[MT][NT], sums[RING];
+    Codes<T> w[NT], a[AS];
+    float scale[MT], before[TAIL];  // of this slice; of the last rows in the one before
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-        sums[1][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
+#pragma unroll
+    for (int i = 0; i < RING; ++i) sums[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < TAIL; ++i) before[i] = 0.f;
     const int r = lane & 15, gk = lane >> 4;
     const int a_place = TA::place(wm + r, gk), w_place = TW::place(wn + N * (r >> 2) + (r & 3), gk);
-    auto read_a = [&](const uint8_t* stage, int i) { a[i & 1] = Codes<T>(TA::read(stage + i * 2048, a_place)); };
-    auto read_w = [&](const uint8_t* stage) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) w[j] = Codes<T>(TW::read(stage + A_BYTES + (16 * JJ * (j / JJ) + 4 * (j % JJ)) * 128, w_place));
-    };
+    auto read_a = [&](const uint8_t* stage, int i) { a[i % AS] = Codes<T>(TA::read(stage + i * 2048, a_place)); };
+    auto read_w = [&](const uint8_t* stage, int j) { w[j] = Codes<T>(TW::read(stage + A_BYTES + (16 * JJ * (j / JJ) + 4 * (j % JJ)) * 128, w_place)); };
     auto read_scales = [&](const uint8_t* stage) {
         const float* s = (const float*)(stage + A_BYTES + W_BYTES);
+        __builtin_memcpy(scale, __builtin_assume_aligned(s + wm + r * MT, MT % 4 == 0 ? 16 : 8), sizeof(scale));
         const float sw = s[BM + wn / kF8Block];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) scale[i] = s[wm + 16 * i + r] * sw;
+        for (int i = 0; i < MT; ++i) scale[i] *= sw;
     };
-    auto add = [&](int i, int j, float by) {  // the sums of step i
+    auto add = [&](int t, float by) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sums[i & 1][j][e], by, acc[i][j][e]);
+        for (int e = 0; e < 4; ++e) acc[row_of(t)][col_of(t)][e] = fmaf(sums[t % RING][e], by, acc[row_of(t)][col_of(t)][e]);
     };
 
     const int slices = g.blocks;
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) load(l, smem, kMaxTileSpanBytes);
-    wait_vm<0>();
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) load(l, smem + STAGE, slices > 1 ? kMaxTileSpanBytes : 0u);
+    wait_vm<LOADS>();
     lds_barrier();
-    read_w(smem);
-    read_a(smem, 0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) read_w(smem, j);
     read_scales(smem);
+    read_a(smem, 0), read_a(smem, 1), read_a(smem, 2);
     for (int s = 0; s < slices; ++s) {
-        const uint8_t* now = smem + (s & 1) * STAGE;
-        uint8_t* next = smem + ((s + 1) & 1) * STAGE;
-        const uint32_t bytes = s + 1 < slices ? (uint32_t)kMaxTileSpanBytes : 0u;
+        uint8_t* now = smem + (s & 1) * STAGE;
+        const uint8_t* next = smem + ((s + 1) & 1) * STAGE;
+        const uint32_t bytes = s + 2 < slices ? (uint32_t)kMaxTileSpanBytes : 0u;
 #pragma unroll
-        for (int i = 0; i < MT - 1; ++i) {
-            read_a(now, i + 1);
+        for (int t = 0; t < ALL; ++t) {
+            if (t == HEAD) {
+                wait_vm<0>();
+                lds_barrier();
+            }
+            if (t < RING) add(ALL - RING + t, before[row_of(ALL - RING + t) - (MT - TAIL)]);
+            else add(t - RING, scale[row_of(t - RING)]);
             __builtin_amdgcn_sched_barrier(0);
+            sums[t % RING] = products(w[col_of(t)], a[row_of(t) % AS]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (t < HEAD) {
+                if (t % NT == 0) read_a(now, t / NT + TAIL);
+            } else {
+                const int u = t - HEAD;
+                // (after the last slice, of a stage that nothing uses)
+                if (u == 0) read_a(next, 0);
+                if (u % TAIL == TAIL - 1) read_w(next, u / TAIL);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                sums[i & 1][j] = products(w[j], a[i & 1]);
-                if (i == 0) add(MT - 1, j, last);
-                else add(i - 1, j, scale[i ? i - 1 : 0]);
+                for (int l = u * LOADS / (TAIL * NT); l < (u + 1) * LOADS / (TAIL * NT); ++l) load(l, now, bytes);
             }
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int l = i * LOADS / (MT - 1); l < (i + 1) * LOADS / (MT - 1); ++l) load(l, next, bytes);
-            __builtin_amdgcn_sched_barrier(0);
         }
-        wait_vm<0>();
-        lds_barrier();
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            sums[(MT - 1) & 1][j] = products(w[j], a[(MT - 1) & 1]);
-            add(MT - 2, j, scale[MT - 2]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        last = scale[MT - 1];
-        // (after the last slice, of a stage that nothing uses)
-        read_w(next);
-        read_a(next, 0);
+        for (int i = 0; i < TAIL; ++i) before[i] = scale[MT - TAIL + i];
+        read_a(next, 1), read_a(next, 2);
         read_scales(next);
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) add(MT - 1, j, last);
+    for (int t = ALL - RING; t < ALL; ++t) add(t, before[row_of(t) - (MT - TAIL)]);
 
     typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));  // at any alignment of T
     const bool whole = m0 + BM <= g.m && n0 + BN <= g.n;
