@@ -184,7 +184,7 @@ struct CodeTile {
 // added. With 16-bit results W's rows are permuted so that a lane holds 8 values next to
 // each other of a row of C: 16 bytes, and four lanes 64, as with fp32 without it.
 template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, int tiles_m, int tiles_n) {
     constexpr int THREADS = 64 * WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
     constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, STAGE = A_BYTES + W_BYTES + WM * WN * 256;
     constexpr int A_LOADS = BM * 8 / THREADS, W_LOADS = BN * 8 / THREADS;
@@ -194,45 +194,69 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, i
     typedef CodeTile<JJ == 1 ? 0 : N> TW;
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // the blocks of one XCD walk groups of 4 tile rows column by column
-    const int id = xcd_order(blockIdx.x, tiles_m * tiles_n);
-    const int group = id / (4 * tiles_n), in_group = id - group * 4 * tiles_n, rows = min(tiles_m - group * 4, 4);
-    const int m0 = (group * 4 + in_group % rows) * BM, n0 = in_group / rows * BN;
     const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
     const uint32_t kp = (uint32_t)g.blocks * kF8Block;
+    const int total = tiles_m * tiles_n, slices = max(g.blocks, 3);  // (of zeros where there are fewer: loads are two slices ahead)
 
-    // rows past the end repeat the last one: their results are not stored
+    // Tile v of this launch's order: the blocks of one XCD walk groups of 4 tile rows column by column.
+    struct Tile {
+        int m0, n0, live;
+    };
+    auto tile_of = [&](int v) {
+        const int id = xcd_order(min(v, total - 1), total), group = id / (4 * tiles_n), in_group = id - group * 4 * tiles_n, rows = min(tiles_m - group * 4, 4);
+        return Tile{(group * 4 + in_group % rows) * BM, in_group / rows * BN, v < total};
+    };
+    // The stream of slices to load: those of a tile, then the next tile's, so that memory is not
+    // waited for between tiles. Rows past the matrix lie outside of the bytes that a load may
+    // reach, and are zeros. The scales of A's rows are loaded by the first BM / 64 waves, so that a lane
+    // finds its MT ones next to each other, W's by the next wave (the others get zeros).
+    const bool a_scales = wave < BM / 64;
+    const int scale_row = a_scales ? tid / (16 * MT) * (16 * MT) + tid % MT * 16 + tid % (16 * MT) / MT : lane;
+    const uint32_t so = (uint32_t)scale_row * (uint32_t)g.blocks * 4u;
     uint32_t ao[A_LOADS], wo[W_LOADS];
 #pragma unroll
-    for (int p = 0; p < A_LOADS; ++p) {
-        const int i = p * THREADS + tid, row = i >> 3;
-        ao[p] = (uint32_t)min(row, g.m - 1 - m0) * kp + (((i & 7) ^ TA::turn(row)) << 4);
-    }
+    for (int p = 0; p < A_LOADS; ++p) ao[p] = (uint32_t)((p * THREADS + tid) >> 3) * kp + (((tid & 7) ^ TA::turn((p * THREADS + tid) >> 3)) << 4);
 #pragma unroll
-    for (int p = 0; p < W_LOADS; ++p) {
-        const int i = p * THREADS + tid, row = i >> 3;
-        wo[p] = (uint32_t)min(row, g.n - 1 - n0) * kp + (((i & 7) ^ TW::turn(row)) << 4);
-    }
-    // the scales of A's rows by the first BM / 64 waves, so that a lane finds its MT ones next
-    // to each other; W's by the next (the others get zeros)
-    const bool a_scales = wave < BM / 64;
-    const int scale_row = tid / (16 * MT) * (16 * MT) + tid % MT * 16 + tid % (16 * MT) / MT;
-    const uint32_t so = (a_scales ? (uint32_t)min(scale_row, g.m - 1 - m0) : (uint32_t)min(lane, (g.n - 1) / kF8Block - n0 / kF8Block)) * (uint32_t)g.blocks * 4u;
-    const uint8_t *pa = g.a + (int64_t)m0 * kp, *pw = g.w + (int64_t)n0 * kp;
-    const float* ps = a_scales ? g.a_scales + (int64_t)m0 * g.blocks : g.w_scales + (int64_t)(n0 / kF8Block) * g.blocks;
+    for (int p = 0; p < W_LOADS; ++p) wo[p] = (uint32_t)((p * THREADS + tid) >> 3) * kp + (((tid & 7) ^ TW::turn((p * THREADS + tid) >> 3)) << 4);
+    struct Stream {
+        const uint8_t *a, *w;
+        const float* scales;
+        uint32_t a_bytes, w_bytes, scale_bytes;
+    };
+    auto stream_of = [&](const Tile& t) {
+        Stream s;
+        s.a = g.a + (int64_t)t.m0 * kp, s.w = g.w + (int64_t)t.n0 * kp;
+        s.scales = a_scales ? g.a_scales + (int64_t)t.m0 * g.blocks : g.w_scales + (int64_t)(t.n0 / kF8Block) * g.blocks;
+        const uint32_t rows_a = min(g.m - t.m0, BM), rows_w = min(g.n - t.n0, BN);
+        s.a_bytes = t.live ? rows_a * kp : 0u, s.w_bytes = t.live ? rows_w * kp : 0u;
+        s.scale_bytes = t.live && wave <= BM / 64 ? (a_scales ? rows_a : (rows_w + kF8Block - 1) / kF8Block) * (uint32_t)g.blocks * 4u : 0u;
+        return s;
+    };
     constexpr int LOADS = A_LOADS + W_LOADS + 1;
-    // Load l of a slice, `bytes` of memory being there (0: none, for zeros). No branch: the
-    // loop below stays one block of code, or its sums are moved to its end.
-    auto load = [&](int l, uint8_t* stage, uint32_t bytes) {
+    int v = blockIdx.x, at = 0;  // the tile that is computed; the slice that is loaded next
+    Tile tile = tile_of(v);
+    Stream from = stream_of(tile), then = stream_of(tile_of(v + gridDim.x));
+    // Load l of a slice; after the last one the stream is a slice further. No branch: the loop
+    // below stays one block of code, or its sums are moved to its end.
+    auto load = [&](int l, uint8_t* stage) {
         uint8_t* to = stage + wave * 1024;
         if (l < A_LOADS) {
-            dma16(make_dma_rsrc(pa, bytes), (half_t*)(to + l * THREADS * 16), ao[l < A_LOADS ? l : 0], 0u);
+            dma16(make_dma_rsrc(from.a, from.a_bytes), (half_t*)(to + l * THREADS * 16), ao[l < A_LOADS ? l : 0], 0u);
         } else if (l < A_LOADS + W_LOADS) {
             const int p = l < A_LOADS || l >= A_LOADS + W_LOADS ? 0 : l - A_LOADS;
-            dma16(make_dma_rsrc(pw, bytes), (half_t*)(to + A_BYTES + p * THREADS * 16), wo[p], 0u);
+            dma16(make_dma_rsrc(from.w, from.w_bytes), (half_t*)(to + A_BYTES + p * THREADS * 16), wo[p], 0u);
         } else {
-            dma4(make_dma_rsrc(ps, wave <= BM / 64 ? bytes : 0u), stage + A_BYTES + W_BYTES + wave * 256, so, 0u);
-            pa += 128, pw += 128, ps += 1;
+            dma4(make_dma_rsrc(from.scales, from.scale_bytes), stage + A_BYTES + W_BYTES + wave * 256, so, 0u);
+            // a slice further; the bytes in reach stay: a row past the last begins behind them
+            const bool end = ++at == slices;
+            at = end ? 0 : at;
+            const bool zeros = !end && at >= g.blocks;
+            from.a = end ? then.a : from.a + 128;
+            from.w = end ? then.w : from.w + 128;
+            from.scales = end ? then.scales : from.scales + 1;
+            from.a_bytes = end ? then.a_bytes : zeros ? 0u : from.a_bytes;
+            from.w_bytes = end ? then.w_bytes : zeros ? 0u : from.w_bytes;
+            from.scale_bytes = end ? then.scale_bytes : zeros ? 0u : from.scale_bytes;
         }
     };
 
@@ -246,7 +270,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, i
     auto col_of = [](int t) { return t < HEAD ? t % NT : (t - HEAD) / TAIL; };
     floatx4 acc[MT][NT], sums[RING];
     Codes<T> w[NT], a[AS];
-    float scale[MT], before[TAIL];  // of this slice; of the last rows in the one before
+    float scale[MT], w_scale, before[TAIL];  // of this slice; of the last rows in the one before
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -259,98 +283,109 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void matmul_f8_tiles(MatmulF8 g, i
     const int a_place = TA::place(wm + r, gk), w_place = TW::place(wn + N * (r >> 2) + (r & 3), gk);
     auto read_a = [&](const uint8_t* stage, int i) { a[i % AS] = Codes<T>(TA::read(stage + i * 2048, a_place)); };
     auto read_w = [&](const uint8_t* stage, int j) { w[j] = Codes<T>(TW::read(stage + A_BYTES + (16 * JJ * (j / JJ) + 4 * (j % JJ)) * 128, w_place)); };
+    // (a row's two scales are multiplied when its first sums are added: nothing waits for them here)
     auto read_scales = [&](const uint8_t* stage) {
         const float* s = (const float*)(stage + A_BYTES + W_BYTES);
         __builtin_memcpy(scale, __builtin_assume_aligned(s + wm + r * MT, MT % 4 == 0 ? 16 : 8), sizeof(scale));
-        const float sw = s[BM + wn / kF8Block];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) scale[i] *= sw;
+        w_scale = s[BM + wn / kF8Block];
     };
     auto add = [&](int t, float by) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[row_of(t)][col_of(t)][e] = fmaf(sums[t % RING][e], by, acc[row_of(t)][col_of(t)][e]);
     };
 
-    const int slices = g.blocks;
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) load(l, smem, kMaxTileSpanBytes);
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l) load(l, smem + STAGE, slices > 1 ? kMaxTileSpanBytes : 0u);
+        for (int l = 0; l < LOADS; ++l) load(l, smem + k * STAGE);
     wait_vm<LOADS>();
     lds_barrier();
+    read_a(smem, 0);
 #pragma unroll
     for (int j = 0; j < NT; ++j) read_w(smem, j);
-    read_scales(smem);
-    read_a(smem, 0), read_a(smem, 1), read_a(smem, 2);
-    for (int s = 0; s < slices; ++s) {
-        uint8_t* now = smem + (s & 1) * STAGE;
-        const uint8_t* next = smem + ((s + 1) & 1) * STAGE;
-        const uint32_t bytes = s + 2 < slices ? (uint32_t)kMaxTileSpanBytes : 0u;
+    int stage = 0;
+    for (; v < total; v += gridDim.x) {
+        for (int s = 0; s < slices; ++s) {
+            uint8_t* now = smem + stage * STAGE;
+            stage ^= 1;
+            const uint8_t* next = smem + stage * STAGE;
 #pragma unroll
-        for (int t = 0; t < ALL; ++t) {
-            if (t == HEAD) {
-                wait_vm<0>();
-                lds_barrier();
-            }
-            if (t < RING) add(ALL - RING + t, before[row_of(ALL - RING + t) - (MT - TAIL)]);
-            else add(t - RING, scale[row_of(t - RING)]);
-            __builtin_amdgcn_sched_barrier(0);
-            sums[t % RING] = products(w[col_of(t)], a[row_of(t) % AS]);
-            __builtin_amdgcn_sched_barrier(0);
-            if (t < HEAD) {
-                if (t % NT == 0) read_a(now, t / NT + TAIL);
-            } else {
-                const int u = t - HEAD;
-                // (after the last slice, of a stage that nothing uses)
-                if (u == 0) read_a(next, 0);
-                if (u % TAIL == TAIL - 1) read_w(next, u / TAIL);
+            for (int t = 0; t < ALL; ++t) {
+                if (t == HEAD) {
+                    wait_vm<0>();
+                    lds_barrier();
+                }
+                if (t >= RING && t - RING < HEAD && (t - RING) % NT == 0) scale[(t - RING) / NT] *= w_scale;
+                if (t >= RING && t - RING >= HEAD && t - RING < HEAD + TAIL) scale[row_of(t - RING)] *= w_scale;
+                if (t < RING) add(ALL - RING + t, before[row_of(ALL - RING + t) - (MT - TAIL)]);
+                else add(t - RING, scale[row_of(t - RING)]);
+                __builtin_amdgcn_sched_barrier(0);
+                sums[t % RING] = products(w[col_of(t)], a[row_of(t) % AS]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (t < HEAD) {
+                    if (t == 0) read_a(now, 1), read_scales(now);
+                    if (t == 1) read_a(now, 2);
+                    if (t > 1 && t % NT == NT / 2) read_a(now, t / NT + TAIL);
+                } else {
+                    const int u = t - HEAD;
+                    // (after the last slice of the last tile, of a stage of zeros)
+                    if (u == 0) read_a(next, 0);
+                    if (u % TAIL == TAIL - 1) read_w(next, u / TAIL);
 #pragma unroll
-                for (int l = u * LOADS / (TAIL * NT); l < (u + 1) * LOADS / (TAIL * NT); ++l) load(l, now, bytes);
+                    for (int l = u * LOADS / (TAIL * NT); l < (u + 1) * LOADS / (TAIL * NT); ++l) load(l, now);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < TAIL; ++i) before[i] = scale[MT - TAIL + i];
         }
 #pragma unroll
-        for (int i = 0; i < TAIL; ++i) before[i] = scale[MT - TAIL + i];
-        read_a(next, 1), read_a(next, 2);
-        read_scales(next);
+        for (int t = ALL - RING; t < ALL; ++t) add(t, before[row_of(t) - (MT - TAIL)]);
+        typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));  // at any alignment of T
+        const bool whole = tile.m0 + BM <= g.m && tile.n0 + BN <= g.n;
+#pragma unroll
+        for (int q = 0; q < NT / JJ; ++q) {
+            const int n = tile.n0 + wn + 16 * JJ * q + N * gk;
+            float bias[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) bias[e] = 0.f;
+            if (g.bias) {
+                if (whole) {
+                    __builtin_memcpy(bias, g.bias + n, sizeof(bias));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) bias[e] = g.bias[min(n + e, g.n - 1)];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int m = tile.m0 + wm + 16 * i + r;
+                T* c = (T*)g.c + (int64_t)m * g.ldc + n;
+                Pack<T, N> v;
+#pragma unroll
+                for (int e = 0; e < N; ++e) v.v[e] = from_f32<T>(acc[i][q * JJ + e / 4][e % 4] + bias[e]);
+                if (whole || (m < g.m && n + N <= g.n)) {
+                    Bits bits;
+                    __builtin_memcpy(&bits, &v, 16);
+                    __builtin_nontemporal_store(bits, (Bits*)c);
+                } else if (m < g.m) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e)
+                        if (n + e < g.n) c[e] = v.v[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RING; ++i) sums[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        // the stream is in the next tile
+        tile = tile_of(v + gridDim.x);
+        then = stream_of(tile_of(v + 2 * gridDim.x));
     }
-#pragma unroll
-    for (int t = ALL - RING; t < ALL; ++t) add(t, before[row_of(t) - (MT - TAIL)]);
-
-    typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));  // at any alignment of T
-    const bool whole = m0 + BM <= g.m && n0 + BN <= g.n;
-#pragma unroll
-    for (int q = 0; q < NT / JJ; ++q) {
-        const int n = n0 + wn + 16 * JJ * q + N * gk;
-        float bias[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) bias[e] = 0.f;
-        if (g.bias) {
-            if (whole) {
-                __builtin_memcpy(bias, g.bias + n, sizeof(bias));
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) bias[e] = g.bias[min(n + e, g.n - 1)];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int m = m0 + wm + 16 * i + r;
-            T* c = (T*)g.c + (int64_t)m * g.ldc + n;
-            Pack<T, N> v;
-#pragma unroll
-            for (int e = 0; e < N; ++e) v.v[e] = from_f32<T>(acc[i][q * JJ + e / 4][e % 4] + bias[e]);
-            if (whole || (m < g.m && n + N <= g.n)) {
-                Bits bits;
-                __builtin_memcpy(&bits, &v, 16);
-                __builtin_nontemporal_store(bits, (Bits*)c);
-            } else if (m < g.m) {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (n + e < g.n) c[e] = v.v[e];
-            }
-        }
-    }
+    wait_vm<0>();  // (zeros on their way to LDS that another block may have next)
 }
 
 template <class T, int BM, int BN, int WM, int WN>
@@ -360,7 +395,8 @@ int launch_tiles(const MatmulF8& g, hipStream_t st) {
     if (lds > 65536)
         SEERA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
-    hipLaunchKernelGGL(kern, dim3((uint32_t)(tiles_m * tiles_n)), dim3(64 * WM * WN), lds, st, g, tiles_m, tiles_n);
+    // as many blocks as run at once: eight waves a compute unit
+    hipLaunchKernelGGL(kern, dim3((uint32_t)std::min(tiles_m * tiles_n, device_cus() * 8 / (WM * WN))), dim3(64 * WM * WN), lds, st, g, tiles_m, tiles_n);
     SEERA_HIP_TRY(hipGetLastError());
     return SEERA_OK;
 }
