@@ -58,8 +58,9 @@ __device__ __forceinline__ floatx4 products(const Codes16& w, const Codes16& a) 
     for (int i = 0; i < 4; ++i) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], a.v[i], p, 0, 0, 0);
     return p;
 }
-__device__ __forceinline__ intx8 fragment(const uint8_t* row, int lane) {
-    const intx4 lo = *(const intx4*)(row + 16 * (lane >> 4)), hi = *(const intx4*)(row + 64 + 16 * (lane >> 4));
+// Two pieces of 16 codes, 64 apart.
+__device__ __forceinline__ intx8 fragment(const uint8_t* at) {
+    const intx4 lo = *(const intx4*)at, hi = *(const intx4*)(at + 64);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -80,71 +81,45 @@ __device__ __forceinline__ void store4(const MatmulF8& g, int m, int n, floatx4 
     for (int i = 0; n + i < g.n; ++i) c[i] = from_f32<T>(v[i] + (g.bias ? g.bias[n + i] : 0.f));
 }
 
-// A tile of 16 MT x 16 NT, with the blocks along K dealt to the waves of a workgroup
-// and their sums joined in the waves' order. Operands go from memory to registers.
-template <class T, int MT, int NT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void matmul_f8_split(MatmulF8 g) {
-    __shared__ floatx4 sums[WAVES][MT * NT][64];
+// ---- few rows: operands from memory to registers ----
+
+// A tile of 16 x 16, with the blocks along K dealt to eight waves, whose sums are joined
+// in the waves' order. All of a wave's loads for K up to 4096 are in flight at once: 1 x 4096 x
+// 4096 in 4.4 us, of which an empty launch is 3.3 (loads a ring of registers ahead: 4.6; 16 waves: 4.7).
+constexpr int kSplitWaves = 8;
+template <class T>
+__global__ __launch_bounds__(64 * kSplitWaves) void matmul_f8_split(MatmulF8 g) {
+    __shared__ floatx4 sums[kSplitWaves][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tiles_n = (g.n + 16 * NT - 1) / (16 * NT);
-    const int n0 = (int)(blockIdx.x % tiles_n) * 16 * NT, m0 = (int)(blockIdx.x / tiles_n) * 16 * MT;
+    const int tiles_n = (g.n + 15) / 16;
+    const int n0 = (int)(blockIdx.x % tiles_n) * 16, m0 = (int)(blockIdx.x / tiles_n) * 16;
     const int64_t kp = (int64_t)g.blocks * kF8Block;
-    const uint8_t* a[MT];
-    const uint8_t* w[NT];
-    const float* sa[MT];
     // rows past the end repeat the last one: their results are not stored
+    const int64_t row = min(m0 + (lane & 15), g.m - 1);
+    const uint8_t* a = g.a + row * kp + 16 * (lane >> 4);
+    const uint8_t* w = g.w + min(n0 + (lane & 15), g.n - 1) * kp + 16 * (lane >> 4);
+    const float *sa = g.a_scales + row * g.blocks, *sw = g.w_scales + (int64_t)(n0 / kF8Block) * g.blocks;
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int b = wave; b < g.blocks; b += kSplitWaves) {
+        const Codes<T> cw(fragment(w + (int64_t)b * kF8Block)), ca(fragment(a + (int64_t)b * kF8Block));
+        const float s = sa[b] * sw[b];
+        const floatx4 p = products(cw, ca);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t m = min(m0 + 16 * i + (lane & 15), g.m - 1);
-        a[i] = g.a + m * kp;
-        sa[i] = g.a_scales + m * g.blocks;
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(p[e], s, acc[e]);
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) w[j] = g.w + min(n0 + 16 * j + (lane & 15), g.n - 1) * kp;
-    const float* sw = g.w_scales + (int64_t)(n0 / kF8Block) * g.blocks;
-    floatx4 acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    for (int b = wave; b < g.blocks; b += WAVES) {
-        Codes<T> fa[MT], fw[NT];
-        float s[MT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) fw[j] = Codes<T>(fragment(w[j] + (int64_t)b * kF8Block, lane));
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            fa[i] = Codes<T>(fragment(a[i] + (int64_t)b * kF8Block, lane));
-            s[i] = sa[i][b] * sw[b];
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const floatx4 p = products(fw[j], fa[i]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], s[i], acc[i][j][e]);
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
+    sums[wave][lane] = acc;
     __syncthreads();
-    for (int t = wave; t < MT * NT; t += WAVES) {
-        floatx4 v = sums[0][t][lane];
+    if (wave) return;
 #pragma unroll
-        for (int k = 1; k < WAVES; ++k) v += sums[k][t][lane];
-        const int m = m0 + 16 * (t / NT) + (lane & 15), n = n0 + 16 * (t % NT) + 4 * (lane >> 4);
-        if (m < g.m) store4<T>(g, m, n, v);
-    }
+    for (int k = 1; k < kSplitWaves; ++k) acc += sums[k][lane];
+    if (m0 + (lane & 15) < g.m) store4<T>(g, m0 + (lane & 15), n0 + 4 * (lane >> 4), acc);
 }
 
-template <class T, int MT, int NT, int WAVES>
+template <class T>
 int launch_split(const MatmulF8& g, hipStream_t st) {
-    const int64_t tiles = (int64_t)((g.n + 16 * NT - 1) / (16 * NT)) * ((g.m + 16 * MT - 1) / (16 * MT));
-    if (tiles * 64 * WAVES >= kMaxThreads) return fail(SEERA_ERR_INVALID_ARGUMENT, "matmul_f8: the product is too large");
-    hipLaunchKernelGGL((matmul_f8_split<T, MT, NT, WAVES>), dim3((uint32_t)tiles), dim3(64 * WAVES), 0, st, g);
+    const int64_t tiles = (int64_t)((g.n + 15) / 16) * ((g.m + 15) / 16);
+    if (tiles * 64 * kSplitWaves >= kMaxThreads) return fail(SEERA_ERR_INVALID_ARGUMENT, "matmul_f8: the product is too large");
+    hipLaunchKernelGGL((matmul_f8_split<T>), dim3((uint32_t)tiles), dim3(64 * kSplitWaves), 0, st, g);
     SEERA_HIP_TRY(hipGetLastError());
     return SEERA_OK;
 }
@@ -178,12 +153,140 @@ struct CodeTile {
     }
 };
 
-// A tile of BM x BN by WM x WN waves; two stages of LDS, one slice of 128 along K each,
+// Where a workgroup's rows begin and how many bytes of memory a load may reach from there:
+// rows past the matrix lie behind them, and are zeros.
+struct Panel {
+    const uint8_t* rows;
+    const float* scales;
+    uint32_t bytes, scale_bytes;
+    __device__ __forceinline__ Panel(const uint8_t* codes, const float* s, int first, int last, int most, int first_scale, int scales_there, int blocks)
+        : rows(codes + (int64_t)first * blocks * kF8Block),
+          scales(s + (int64_t)first_scale * blocks),
+          bytes((uint32_t)min(last - first, most) * (uint32_t)blocks * kF8Block),
+          scale_bytes((uint32_t)scales_there * (uint32_t)blocks * 4u) {}
+};
+
+// Small tiles of BM x BN by four waves for products that larger ones would give too few
+// workgroups: what bounds them is how much is on its way from memory, so LDS holds
+// STAGES stages of two slices each, all but one of them in flight, and a barrier every two slices
+// is all that the waves wait for. BM / 16 or four waves along m, the others along n.
+template <class T, int BM, int BN, int STAGES>
+__global__ __launch_bounds__(256, 1) void matmul_f8_stream(MatmulF8 g, int tiles_m, int tiles) {
+    constexpr int WM = BM >= 64 ? 4 : BM / 16, WN = 4 / WM, MT = BM / WM / 16, NT = BN / WN / 16, KS = 2;
+    constexpr int PIECES = (BM + BN) * 8, LOADS_K = (PIECES + 255) / 256, ROWS = BM + BN;
+    constexpr int SLICE = LOADS_K * 4096 + 2048, STAGE = KS * SLICE, LOADS = KS * (LOADS_K + 2);
+    static_assert(BM <= 128 && BN <= 128 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && MT && NT && (STAGES - 2) * LOADS < 64, "shapes of a tile");
+    typedef CodeTile<0> Tile;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = xcd_order(blockIdx.x, tiles), m0 = id % tiles_m * BM, n0 = id / tiles_m * BN;
+    const uint32_t kp = (uint32_t)g.blocks * kF8Block;
+    const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    const Panel pa(g.a, g.a_scales, m0, g.m, BM, m0, min(g.m - m0, BM), g.blocks);
+    const Panel pw(g.w, g.w_scales, n0, g.n, BN, n0 / kF8Block, 1, g.blocks);
+    // a piece of 16 bytes each: rows of A, then of W; whole waves have one of the two
+    uint32_t at[LOADS_K];
+#pragma unroll
+    for (int p = 0; p < LOADS_K; ++p) {
+        const int row = (p * 256 + tid) >> 3, r = row < BM ? row : row - BM;
+        at[p] = row < ROWS ? (uint32_t)r * kp + (((tid & 7) ^ Tile::turn(row)) << 4) : kBufOOB;
+    }
+    const uint32_t so = (uint32_t)min(tid, BM - 1) * (uint32_t)g.blocks * 4u;
+    auto load = [&](int b, uint8_t* to) {
+        const bool there = b < g.blocks;
+        const int64_t off = (int64_t)b * kF8Block;
+#pragma unroll
+        for (int p = 0; p < LOADS_K; ++p) {
+            const bool of_a = (p * 256 + wave * 64) / 8 < BM;
+            dma16(make_dma_rsrc((of_a ? pa.rows : pw.rows) + off, !there ? 0u : of_a ? pa.bytes : pw.bytes), (half_t*)(to + p * 4096 + wave * 1024), at[p], 0u);
+        }
+        dma4(make_dma_rsrc(pa.scales + b, there ? pa.scale_bytes : 0u), to + LOADS_K * 4096 + wave * 256, so, 0u);
+        dma4(make_dma_rsrc(pw.scales + b, there ? 4u : 0u), to + LOADS_K * 4096 + 1024 + wave * 256, 0u, 0u);
+    };
+    floatx4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const int r = lane & 15, gk = lane >> 4;
+    const int a_place = Tile::place(wm + r, gk), w_place = Tile::place(BM + wn + r, gk);
+
+    const int rounds = (g.blocks + KS - 1) / KS;
+#pragma unroll
+    for (int k = 0; k < (STAGES - 1) * KS; ++k) load(k, smem + k * SLICE);
+    int stage = 0;
+    for (int it = 0; it < rounds; ++it) {
+        // this stage has landed, and every wave has read all of the one before, which is filled anew
+        wait_vm<(STAGES - 2) * LOADS>();
+        lds_barrier();
+        const uint8_t* now = smem + stage * STAGE;
+        uint8_t* before = smem + (stage == 0 ? STAGES - 1 : stage - 1) * STAGE;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) load((it + STAGES - 1) * KS + k, before + k * SLICE);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        intx8 a[KS][MT], w[KS][NT];
+        float s[KS][MT];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const uint8_t* slice = now + k * SLICE;
+            const float* scales = (const float*)(slice + LOADS_K * 4096);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) w[k][j] = Tile::read(slice + j * 2048, w_place);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) a[k][i] = Tile::read(slice + i * 2048, a_place);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) s[k][i] = scales[wm + 16 * i + r];
+            const float sw = scales[256 + wave * 64];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) s[k][i] *= sw;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            Codes<T> cw[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) cw[j] = Codes<T>(w[k][j]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const Codes<T> ca(a[k][i]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const floatx4 p = products(cw[j], ca);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], s[k][i], acc[i][j][e]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int m = m0 + wm + 16 * i + r, n = n0 + wn + 16 * j + 4 * gk;
+            if (m < g.m) store4<T>(g, m, n, acc[i][j]);
+        }
+    wait_vm<0>();  // (zeros on their way to LDS that another block may have next)
+}
+
+template <class T, int BM, int BN, int STAGES>
+int launch_stream(const MatmulF8& g, hipStream_t st) {
+    constexpr int lds = STAGES * 2 * (((BM + BN) * 8 + 255) / 256 * 4096 + 2048);
+    static_assert(lds <= 160 * 1024, "LDS of a compute unit");
+    const int64_t tiles_m = (g.m + BM - 1) / BM, tiles = tiles_m * ((g.n + BN - 1) / BN);
+    if (tiles * 256 >= kMaxThreads) return fail(SEERA_ERR_INVALID_ARGUMENT, "matmul_f8: the product is too large");
+    auto kern = matmul_f8_stream<T, BM, BN, STAGES>;
+    if (lds > 65536)
+        SEERA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL(kern, dim3((uint32_t)tiles), dim3(256), lds, st, g, (int)tiles_m, (int)tiles);
+    SEERA_HIP_TRY(hipGetLastError());
+    return SEERA_OK;
+}
+
+// A tile of BM x BN by WM x WN waves; STAGES stages of LDS, one slice of 128 along K each,
 // filled by DMA. In a wave, W's fragments of a slice stay in registers and A's
 // pass by: NT products of one, while the sums of the products before it are scaled and
 // added. With 16-bit results W's rows are permuted so that a lane holds 8 values next to
 // each other of a row of C: 16 bytes, and four lanes 64, as with fp32 without it.
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, int tiles_m, int tiles_n) {
     constexpr int THREADS = 64 * WM * WN, MT = BM / WM / 16, NT = BN / WN / 16;
     constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, STAGE = A_BYTES + W_BYTES + WM * WN * 256;
@@ -196,7 +299,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
     const uint32_t kp = (uint32_t)g.blocks * kF8Block;
-    const int total = tiles_m * tiles_n, slices = max(g.blocks, 3);  // (of zeros where there are fewer: loads are two slices ahead)
+    const int total = tiles_m * tiles_n, slices = max(g.blocks, STAGES + 1);  // (of zeros where there are fewer: loads are STAGES slices ahead)
 
     // Tile v of this launch's order: the blocks of one XCD walk groups of 4 tile rows column by column.
     struct Tile {
@@ -295,10 +398,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
     };
 
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < STAGES; ++k)
 #pragma unroll
         for (int l = 0; l < LOADS; ++l) load(l, smem + k * STAGE);
-    wait_vm<LOADS>();
+    wait_vm<(STAGES - 1) * LOADS>();
     lds_barrier();
     read_a(smem, 0);
 #pragma unroll
@@ -307,12 +410,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
     for (; v < total; v += gridDim.x) {
         for (int s = 0; s < slices; ++s) {
             uint8_t* now = smem + stage * STAGE;
-            stage ^= 1;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
             const uint8_t* next = smem + stage * STAGE;
 #pragma unroll
             for (int t = 0; t < ALL; ++t) {
                 if (t == HEAD) {
-                    wait_vm<0>();
+                    wait_vm<(STAGES - 2) * LOADS>();
                     lds_barrier();
                 }
                 if (t >= RING && t - RING < HEAD && (t - RING) % NT == 0) scale[(t - RING) / NT] *= w_scale;
@@ -388,27 +491,73 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
     wait_vm<0>();  // (zeros on their way to LDS that another block may have next)
 }
 
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, int BM, int BN, int WM, int WN, int STAGES>
 int launch_tiles(const MatmulF8& g, hipStream_t st) {
-    constexpr int lds = 2 * ((BM + BN) * 128 + WM * WN * 256);
-    auto kern = matmul_f8_tiles<T, BM, BN, WM, WN>;
+    constexpr int lds = STAGES * ((BM + BN) * 128 + WM * WN * 256);
+    static_assert(lds <= 160 * 1024, "LDS of a compute unit");
+    const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
+    if ((int64_t)tiles_m * tiles_n >= 1 << 30) return fail(SEERA_ERR_INVALID_ARGUMENT, "matmul_f8: the product is too large");
+    auto kern = matmul_f8_tiles<T, BM, BN, WM, WN, STAGES>;
     if (lds > 65536)
         SEERA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    const int tiles_m = (g.m + BM - 1) / BM, tiles_n = (g.n + BN - 1) / BN;
-    // as many blocks as run at once: eight waves a compute unit
-    hipLaunchKernelGGL(kern, dim3((uint32_t)std::min(tiles_m * tiles_n, device_cus() * 8 / (WM * WN))), dim3(64 * WM * WN), lds, st, g, tiles_m, tiles_n);
+    // as many blocks as run at once
+    hipLaunchKernelGGL(kern, dim3((uint32_t)std::min(tiles_m * tiles_n, device_cus())), dim3(64 * WM * WN), lds, st, g, tiles_m, tiles_n);
     SEERA_HIP_TRY(hipGetLastError());
     return SEERA_OK;
 }
 
+// The ways to compute a product: tiles of rows x cols, `at_once` workgroups a compute unit. A
+// launch takes `start` us (3.3 of them an empty one) and, for each slice of 128 along K, `few` where most
+// compute units have nothing to do, `full` where each has its workgroup, `pair` where each has two. Fitted
+// to times of 16 to 8192 rows with every way at K = 1024, 4096 and 16384 (bf16; fp32 below).
+enum Way { kSplit, kStream16x64, kStream32x32, kStream32x64, kStream64x64, kTiles128, kTiles128x256, kTiles256, kWays };
+struct Cost {
+    int rows, cols, at_once;
+    double start, few, full, pair;
+};
+constexpr Cost kCosts16[kWays] = {{16, 16, 1, 1.9, 0, 0, 0}, {16, 64, 1, 3.0, .20, .23, 0}, {32, 32, 1, 3.4, .18, .19, 0}, {32, 64, 1, 3.2, .22, .23, 0},
+                                  {64, 64, 2, 3.2, .38, .39, .49}, {128, 128, 1, 4.6, .49, .66, 0}, {128, 256, 1, 6.0, .68, .96, 0}, {256, 256, 1, 9.0, 1.15, 1.63, 0}};
+// (fp32 results: twice the matrix instructions' time, which binds the larger tiles)
+constexpr Cost kCosts32[kWays] = {{16, 16, 1, 1.9, 0, 0, 0}, {16, 64, 1, 3.2, .27, .28, 0}, {32, 32, 1, 3.6, .26, .26, 0}, {32, 64, 1, 3.4, .34, .34, 0},
+                                  {64, 64, 2, 3.4, .46, .48, .76}, {128, 128, 1, 4.6, 1.40, 1.45, 0}, {128, 256, 1, 6.0, 1.65, 1.95, 0}, {256, 256, 0, 0, 0, 0, 0}};
+
+double time_of(const Cost& c, int64_t m, int64_t n, int64_t slices, int64_t cus) {
+    const int64_t tiles = ((m + c.rows - 1) / c.rows) * ((n + c.cols - 1) / c.cols);
+    // the way from registers reads a row of A and of W for each of its 16 (where there are as many)
+    const double full = c.rows == 16 && c.cols == 16 ? .10 + .003 * std::min<int64_t>(m, 16) : c.full, few = c.few > 0 ? c.few : full;
+    const int64_t round = cus * c.at_once, rounds = tiles / round, rest = tiles % round;
+    double slice = rounds * (c.at_once == 2 ? c.pair : full);
+    if (rest) slice += c.at_once == 2 && rest > cus ? c.pair : few + (full - few) * std::min<int64_t>(rest, cus) / cus;
+    return c.start + slices * slice;
+}
+
 template <class T>
 int launch_t(const MatmulF8& g, hipStream_t st) {
-    if (g.m <= 16) return launch_split<T, 1, 1, 8>(g, st);
-    if (g.m >= 512 && g.blocks) {
-        if constexpr (sizeof(T) == 4) return launch_tiles<T, 128, 128, 2, 2>(g, st);
-        else return launch_tiles<T, 256, 256, 2, 4>(g, st);
+    constexpr bool F32 = sizeof(T) == 4;
+    const Cost* costs = F32 ? kCosts32 : kCosts16;
+    // offsets inside a tile are 31 bits
+    const bool short_rows = (int64_t)256 * g.blocks * kF8Block < kMaxTileSpanBytes;
+    int best = kSplit;
+    if (g.blocks && short_rows) {
+        const int64_t cus = device_cus();
+        double least = g.m <= 16 ? time_of(costs[kSplit], g.m, g.n, g.blocks, cus) : 1e300;
+        for (int way = kSplit + 1; way < kWays; ++way) {
+            if (!costs[way].at_once) continue;
+            const double t = time_of(costs[way], g.m, g.n, g.blocks, cus);
+            if (t < least) least = t, best = way;
+        }
     }
-    return launch_split<T, 4, 2, 4>(g, st);
+    switch (best) {
+        case kStream16x64: return launch_stream<T, 16, 64, 5>(g, st);
+        case kStream32x32: return launch_stream<T, 32, 32, 8>(g, st);
+        case kStream32x64: return launch_stream<T, 32, 64, 5>(g, st);
+        case kStream64x64: return launch_stream<T, 64, 64, 2>(g, st);
+        case kTiles128: return launch_tiles<T, 128, 128, 2, 2, 3>(g, st);
+        case kTiles128x256: return launch_tiles<T, 128, 256, 2, 4, 3>(g, st);
+        case kTiles256:
+            if constexpr (!F32) return launch_tiles<T, 256, 256, 2, 4, 2>(g, st);
+    }
+    return launch_split<T>(g, st);
 }
 
 }  // namespace
