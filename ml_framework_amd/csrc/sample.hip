@@ -8,9 +8,12 @@
 // that top-k kept, min-p those of at least min_p of the first one's weight. The token
 // drawn is the first, by index, where the sum of kept weights passes u of their total.
 //
-// No order is made. A cut is found as (value, how many of the tokens that have it):
-// a histogram over distances from the largest (monotone in l, so a bin is a stretch
-// of the order), then the bin that holds the cut by the digits of its tokens' values.
+// No order is made. A cut is found as (value, how many of the tokens that have it): a
+// histogram over distances from the largest (monotone in l, so a bin is a stretch of the
+// order), then the bin that holds the cut, whose tokens are listed and compared with each
+// other (or, if they are many, told apart digit by digit of their values). The histogram first covers
+// weights down to 2^-16, the rest only being summed up, and all of them where the cut lies lower.
+// One workgroup has a row, which it reads four or five times, mostly from the caches.
 #include <algorithm>
 
 #include "inference.h"
@@ -22,9 +25,12 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
-constexpr float kBinsPerBit = 48.f;  // 42.67 bits in all: weights behind them are 0
+// the bins' distance in bits of weight, first and where the cut lies lower: in all 16 bits, or
+// 42.67, behind which weights are 0
+constexpr float kBinsPerBit[2] = {128.f, 48.f};
 constexpr int kBits = 40;
 constexpr int kSegments = 1024;
+constexpr int kListed = 512;
 
 // The order of values as unsigned numbers (-0 counts as 0).
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -32,50 +38,96 @@ __device__ __forceinline__ uint32_t key_of(float l) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// 2^(i / 64), times 2^40.
+constexpr int kPowers = 64;
+
 struct Row {
     float largest;
     float bins;     // bins for each unit of distance
-    double scale;   // log2(e) / T
-    // The token's weight. -infinity and NaN have none; of infinities each has 1.
-    __device__ uint64_t weight(float l) const {
-        if (l == largest) return 1ull << kBits;
-        const double z = ((double)l - (double)largest) * scale;
-        return z > -42.0 ? (uint64_t)rint(exp2(z) * (double)(1ull << kBits)) : 0ull;
+    double scale;   // 64 log2(e) / T
+    const double* powers;
+    // The token's weight. -infinity has none; of infinities each has 1. 2^(z / 64) with z = 64 a + i + f is
+    // 2^a, a value of the table and four terms of 2^(f / 64)'s series: within 2^-46 of itself.
+    __device__ __forceinline__ uint64_t weight(float l) const {
+        double z = ((double)l - (double)largest) * scale;
+        z = l == largest ? 0.0 : z;
+        if (!(z > -42.0 * kPowers)) return 0;
+        const double n = rint(z), f = z - n;
+        const int whole = (int)n;
+        constexpr double c1 = 0.6931471805599453 / kPowers, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
+        const double series = fma(f, fma(f, fma(f, fma(f, c4, c3), c2), c1), 1.0);
+        const double w = ldexp(powers[whole & (kPowers - 1)] * series, whole >> 6);
+        // rounded to a whole number by the addition of 2^52
+        return (uint64_t)(__double_as_longlong(w + 0x1p52) - __double_as_longlong(0x1p52));
     }
-    __device__ int bin(float l) const {
-        if (l == largest) return 0;
-        return (int)fminf((largest - l) * bins, (float)(kBins - 1));
+    // the bin, kBins or more where it lies behind them
+    __device__ __forceinline__ int bin(float l) const { return l == largest ? 0 : (int)fminf((largest - l) * bins, 1e6f); }
+};
+
+// A row of logits as a thread sees it: tiles of 64 N tokens for each wave in turn, a tile's
+// lane having N next to each other. -infinity past the end and in place of NaN.
+template <class T>
+struct Logits {
+    static constexpr int N = 16 / sizeof(T);
+    struct alignas(16) Values {
+        T v[N];
+    };
+    const T* row;
+    int vocab, tiles, lane, wave;
+
+    __device__ __forceinline__ Values load(int tile) const {
+        const int at = (tile * 64 + lane) * N;
+        Values x;
+        const bool whole = at + N <= vocab;
+        if (whole) __builtin_memcpy(&x, row + at, 16);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) x.v[i] = at + i < vocab ? row[at + i] : from_f32<T>(-__builtin_huge_valf());
+        return x;
+    }
+    __device__ __forceinline__ Logits(const T* logits, int n) : row(logits), vocab(n), tiles((n + 64 * N - 1) / (64 * N)) {
+        lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    }
+    static __device__ __forceinline__ float value(T v) {
+        const float l = to_f32(v);
+        return l == l ? l : -__builtin_huge_valf();
+    }
+    // f(values, tile) for each of the wave's tiles, the next one being loaded meanwhile
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        if (wave >= tiles) return;
+        Values now = load(wave);
+        for (int t = wave; t < tiles; t += kWaves) {
+            const Values next = load(min(t + kWaves, tiles - 1));
+            f(now, t);
+            now = next;
+        }
+    }
+    // f(l) for each token
+    template <class F>
+    __device__ __forceinline__ void tokens(F f) const {
+        each([&](const Values& x, int) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f(value(x.v[i]));
+        });
     }
 };
 
-// The part of a row of logits that a step walks: `f(l, index)` for N values of each
-// lane at a time, in tiles of 64 N from `begin` on; -infinity past the end and in
-// place of NaN.
-template <class T, class F>
-__device__ __forceinline__ void tile_values(const T* row, int vocab, int tile, int lane, F f) {
-    constexpr int N = 16 / sizeof(T);
-    const int at = (tile * 64 + lane) * N;
-    T v[N];
-    const bool whole = at + N <= vocab;
-    if (whole) __builtin_memcpy(v, row + at, 16);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        float l = whole ? to_f32(v[i]) : at + i < vocab ? to_f32(row[at + i]) : -__builtin_huge_valf();
-        if (l != l) l = -__builtin_huge_valf();
-        f(i, l, at + i);
-    }
-}
-
 struct Shared {
-    uint32_t counts[kBins];
+    double powers[kPowers];
     uint64_t masses[kBins];
+    uint64_t listed_weights[kListed];
     uint64_t wave_mass[kWaves];
+    uint64_t above_mass, found_mass;
+    uint32_t counts[kBins];
+    float listed[kListed];
     uint32_t wave_count[kWaves];
     float best[kWaves];
     int best_at[kWaves];
-    uint64_t above_mass, found_mass;
-    uint32_t above_count, found_count;
+    uint32_t above_count, found_count, listed_count;
     int found;
+    uint32_t cut_key, cut_ties;
+    uint64_t cut_mass;
 };
 
 // Inclusive sums over the block's threads of (count, mass).
@@ -138,26 +190,73 @@ __device__ __forceinline__ void find(int n, uint32_t count, uint64_t mass, Share
     __syncthreads();
 }
 
-// The cut inside bin `bin`, above which lie `above_count` and `above_mass`.
-template <bool BY_COUNT, class T>
-__device__ Cut cut_in_bin(const T* row, int vocab, int tiles, const Row& r, int bin, uint32_t count, uint64_t mass, uint32_t above_count,
-                          uint64_t above_mass, Shared& sh) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t prefix = 0;
-    uint32_t in = 0;
+// The sum over the block's threads, in all of them.
+__device__ __forceinline__ uint64_t block_total(uint64_t mass, Shared& sh) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) mass += __shfl_xor((unsigned long long)mass, m);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave_mass[threadIdx.x >> 6] = mass;
+    __syncthreads();
+    mass = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mass += sh.wave_mass[w];
+    return mass;
+}
+
+// The cut inside bin `bin`, above which lie `above_count` and `above_mass`: where the count
+// reaches `count` (BY_COUNT), or the mass `mass`.
+template <bool BY_COUNT, class L>
+__device__ __forceinline__ Cut cut_in_bin(const L& logits, const Row& r, int bin, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass, Shared& sh) {
+    const float lowest = -__builtin_huge_valf();
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed_count = 0;
+    __syncthreads();
+    logits.tokens([&](float l) {
+        if (l == lowest || r.bin(l) != bin) return;
+        const uint32_t at = atomicAdd(&sh.listed_count, 1u);
+        if (at >= kListed) return;
+        sh.listed[at] = l;
+        sh.listed_weights[at] = r.weight(l);
+    });
+    __syncthreads();
+    const uint32_t n = sh.listed_count;
+    if (n <= kListed) {
+        // each token against all others: one of those that have the cut's value writes it down
+        if (threadIdx.x < n) {
+            const float l = sh.listed[threadIdx.x];
+            const uint64_t w = sh.listed_weights[threadIdx.x];
+            uint32_t c = above_count, same = 0;
+            uint64_t m = above_mass;
+            for (uint32_t k = 0; k < n; ++k) {
+                const float other = sh.listed[k];
+                const uint64_t ow = sh.listed_weights[k];
+                c += other > l;
+                m += other > l ? ow : 0;
+                same += other == l;
+            }
+            if (BY_COUNT ? c < count && c + same >= count : m < mass && m + same * w >= mass) {
+                const uint32_t ties = BY_COUNT ? count - c : (uint32_t)((mass - m + w - 1) / w);
+                sh.cut_key = key_of(l), sh.cut_ties = ties, sh.cut_mass = m + ties * w;  // the same from each of them
+            }
+        }
+        __syncthreads();
+        const Cut cut = {sh.cut_key, sh.cut_ties, sh.cut_mass};
+        __syncthreads();
+        return cut;
+    }
+    uint32_t prefix = 0, in = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
         if (threadIdx.x < 256) sh.counts[threadIdx.x] = 0, sh.masses[threadIdx.x] = 0;
         __syncthreads();
-        for (int t = wave; t < tiles; t += kWaves)
-            tile_values(row, vocab, t, lane, [&](int, float l, int) {
-                if (l == -__builtin_huge_valf() || r.bin(l) != bin) return;
-                const uint32_t key = key_of(l);
-                if (shift < 24 && key >> (shift + 8) != prefix) return;
-                const uint32_t digit = 255 - (key >> shift & 255);  // larger values first
-                atomicAdd(&sh.counts[digit], 1u);
-                atomicAdd((unsigned long long*)&sh.masses[digit], (unsigned long long)r.weight(l));
-            });
+        logits.tokens([&](float l) {
+            if (l == lowest || r.bin(l) != bin) return;
+            const uint32_t key = key_of(l);
+            if (shift < 24 && key >> (shift + 8) != prefix) return;
+            const uint32_t digit = 255 - (key >> shift & 255);  // larger values first
+            atomicAdd(&sh.counts[digit], 1u);
+            atomicAdd((unsigned long long*)&sh.masses[digit], (unsigned long long)r.weight(l));
+        });
         __syncthreads();
         find<BY_COUNT>(256, count - above_count, mass - above_mass, sh);
         prefix = prefix << 8 | (uint32_t)(255 - sh.found);
@@ -172,36 +271,111 @@ __device__ Cut cut_in_bin(const T* row, int vocab, int tiles, const Row& r, int 
     return Cut{prefix, ties, above_mass + ties * each};
 }
 
+// The histogram of the row's tokens; the weights of those behind the bins are returned.
+template <class L>
+__device__ __forceinline__ uint64_t histogram(const L& logits, const Row& r, bool counts, bool masses, Shared& sh) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
+    __syncthreads();
+    uint64_t behind = 0;
+    logits.tokens([&](float l) {
+        if (l == -__builtin_huge_valf()) return;
+        const int b = r.bin(l);
+        const uint64_t w = masses ? r.weight(l) : 0;
+        if (b >= kBins) {
+            behind += w;
+            return;
+        }
+        if (counts) atomicAdd(&sh.counts[b], 1u);
+        if (masses) atomicAdd((unsigned long long*)&sh.masses[b], (unsigned long long)w);
+    });
+    __syncthreads();
+    return behind;
+}
+
+// What top-k and top-p keep.
+template <class L>
+__device__ __forceinline__ Cut find_cut(const L& logits, Row& r, uint32_t k, float p, Shared& sh) {
+    Cut cut = {0, 0, 0};  // all values are above
+    bool by_count = k > 0;
+    const bool by_mass = p < 1.f;
+    for (int wide = 0; wide < 2 && (by_count || by_mass); ++wide) {
+        r.bins = (float)min(r.scale / kPowers * (double)kBinsPerBit[wide], 3e38);
+        const uint64_t behind = histogram(logits, r, by_count, by_mass, sh);
+        uint64_t all = 0;
+        if (by_mass) {
+            uint64_t own = behind;
+            for (int i = threadIdx.x; i < kBins; i += kThreads) own += sh.masses[i];
+            all = block_total(own, sh);
+        }
+        // the bins that the cuts are found in are looked up before the first cut uses their memory
+        int bin_k = -1;
+        uint32_t count_k = 0;
+        uint64_t mass_k = 0;
+        if (by_count) {
+            __syncthreads();
+            find<true>(kBins, k, 0, sh);
+            bin_k = sh.found, count_k = sh.above_count, mass_k = sh.above_mass;
+            if (bin_k < 0 && !wide) continue;  // it lies behind them, or there are not so many
+            if (bin_k < 0) by_count = false;
+        }
+        if (bin_k >= 0) {
+            cut = cut_in_bin<true>(logits, r, bin_k, k, 0, count_k, mass_k, sh);
+            all = cut.mass;
+        }
+        if (!by_mass) break;
+        const uint64_t target = max((uint64_t)1, (uint64_t)ceil(p > 0.f ? (double)p * (double)all : 0.0));
+        if (bin_k >= 0 && sh.listed_count > kListed) histogram(logits, r, false, true, sh);  // its memory was used
+        __syncthreads();
+        find<false>(kBins, 0, target, sh);
+        const int bin_p = sh.found;
+        const uint64_t mass_p = sh.above_mass;
+        if (bin_p < 0 && !wide) continue;
+        if (bin_p >= 0) {
+            const Cut c = cut_in_bin<false>(logits, r, bin_p, 0, target, 0, mass_p, sh);
+            if (bin_k < 0 || c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
+        }
+        break;
+    }
+    return cut;
+}
+
 template <class T>
 __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     constexpr int N = 16 / sizeof(T);
     __shared__ Shared sh;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t at = blockIdx.x;
-    const T* row = (const T*)a.logits + at * a.ld;
-    const int tiles = (a.vocab + 64 * N - 1) / (64 * N);
+    const Logits<T> logits((const T*)a.logits + at * a.ld, a.vocab);
+    const int lane = logits.lane, wave = logits.wave, tiles = logits.tiles;
     const float lowest = -__builtin_huge_valf();
+    if (threadIdx.x < kPowers) sh.powers[threadIdx.x] = exp2((double)threadIdx.x / kPowers) * (double)(1ull << kBits);
 
     // the largest, and where it is first
     float best = lowest;
-    int best_at = 0x7fffffff;
-    for (int t = wave; t < tiles; t += kWaves)
-        tile_values(row, a.vocab, t, lane, [&](int, float l, int i) {
-            if (l > best) best = l, best_at = i;
-        });
-    auto join = [&](float l, int i) {
-        if (l > best || (l == best && i < best_at)) best = l, best_at = i;
-    };
+    logits.tokens([&](float l) { best = fmaxf(best, l); });
 #pragma unroll
-    for (int m = 32; m; m >>= 1) join(__shfl_xor(best, m), __shfl_xor(best_at, m));
-    if (lane == 0) sh.best[wave] = best, sh.best_at[wave] = best_at;
+    for (int m = 32; m; m >>= 1) best = fmaxf(best, __shfl_xor(best, m));
+    if (lane == 0) sh.best[wave] = best;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) join(sh.best[w], sh.best_at[w]);
+    for (int w = 0; w < kWaves; ++w) best = fmaxf(best, sh.best[w]);
     const float temperature = a.temperature ? a.temperature[at] : 1.f;
     if (best == lowest || !(temperature > 0.f)) {
+        int first = 0x7fffffff;
+        if (best != lowest) {
+            logits.each([&](const typename Logits<T>::Values& x, int tile) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (logits.value(x.v[i]) == best) first = min(first, (tile * 64 + lane) * N + i);
+            });
+        }
+#pragma unroll
+        for (int m = 32; m; m >>= 1) first = min(first, __shfl_xor(first, m));
+        if (lane == 0) sh.best_at[wave] = first;
+        __syncthreads();
         if (threadIdx.x == 0) {
-            a.tokens[at] = best == lowest ? -1 : best_at;
+            for (int w = 0; w < kWaves; ++w) first = min(first, sh.best_at[w]);
+            a.tokens[at] = best == lowest ? -1 : first;
             if (a.logp) a.logp[at] = best == lowest ? lowest : 0.f;
         }
         return;
@@ -209,102 +383,60 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 
     Row r;
     r.largest = best;
-    r.scale = 1.4426950408889634 / (double)temperature;
-    r.bins = (float)min(r.scale * (double)kBinsPerBit, 3e38);
+    r.powers = sh.powers;
+    r.scale = kPowers * 1.4426950408889634 / (double)temperature;
     const int k = a.top_k ? a.top_k[at] : 0;
     const float p = a.top_p ? a.top_p[at] : 1.f;
-    const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.f;
-    Cut cut = {0, 0, 0};  // all values are above
-    if (by_count || by_mass) {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
-        __syncthreads();
-        for (int t = wave; t < tiles; t += kWaves)
-            tile_values(row, a.vocab, t, lane, [&](int, float l, int) {
-                if (l == lowest) return;
-                const int b = r.bin(l);
-                atomicAdd(&sh.counts[b], 1u);
-                atomicAdd((unsigned long long*)&sh.masses[b], (unsigned long long)r.weight(l));
-            });
-        __syncthreads();
-        uint64_t all = 0;
-        if (by_mass) {
-            // the cut by mass needs what top-k keeps
-            uint64_t own = 0;
-            for (int i = threadIdx.x; i < kBins; i += kThreads) own += sh.masses[i];
-            const Sums s = block_scan(Sums{0, own}, sh);
-            __syncthreads();
-            if (threadIdx.x == kThreads - 1) sh.above_mass = s.mass;
-            __syncthreads();
-            all = sh.above_mass;
-            __syncthreads();
-        }
-        int bin_k = -1, bin_p = -1;
-        uint32_t count_k = 0, count_p = 0;
-        uint64_t mass_k = 0, mass_p = 0;
-        if (by_count) {
-            find<true>(kBins, (uint32_t)k, 0, sh);
-            bin_k = sh.found, count_k = sh.above_count, mass_k = sh.above_mass;
-            __syncthreads();
-        }
-        const bool within = bin_k >= 0;
-        // (the histogram is made anew by the cut inside a bin, and once more for the other)
-        if (within) {
-            cut = cut_in_bin<true>(row, a.vocab, tiles, r, bin_k, (uint32_t)k, 0, count_k, mass_k, sh);
-            all = cut.mass;
-        }
-        if (by_mass) {
-            const double share = p > 0.f ? (double)p * (double)all : 0.0;
-            const uint64_t target = max((uint64_t)1, (uint64_t)ceil(share));
-            if (within) {
-                for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
-                __syncthreads();
-                for (int t = wave; t < tiles; t += kWaves)
-                    tile_values(row, a.vocab, t, lane, [&](int, float l, int) {
-                        if (l == lowest) return;
-                        const int b = r.bin(l);
-                        atomicAdd(&sh.counts[b], 1u);
-                        atomicAdd((unsigned long long*)&sh.masses[b], (unsigned long long)r.weight(l));
-                    });
-                __syncthreads();
-            }
-            find<false>(kBins, 0, target, sh);
-            bin_p = sh.found, count_p = sh.above_count, mass_p = sh.above_mass;
-            __syncthreads();
-            if (bin_p >= 0) {
-                const Cut c = cut_in_bin<false>(row, a.vocab, tiles, r, bin_p, 0, target, count_p, mass_p, sh);
-                if (!within || c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
-            }
-        }
-    }
+    const Cut cut = find_cut(logits, r, k > 0 && k < a.vocab ? (uint32_t)k : 0u, p, sh);
     const float min_p = a.min_p ? a.min_p[at] : 0.f;
-    const double z_least = min_p > 0.f ? log2((double)fminf(min_p, 1.f)) : -1e300;
+    const double z_least = min_p > 0.f ? kPowers * log2((double)fminf(min_p, 1.f)) : -1e300;
 
     // What each segment of the row keeps: the mass above the cut's value, and how many have it.
     // 0: not kept, 1: kept, 2: kept if among the first ties
+    const float cut_value = cut.key ? __uint_as_float(cut.key & 0x80000000u ? cut.key & 0x7fffffffu : ~cut.key) : lowest;
+    const bool by_weight = min_p > 0.f;
     auto kept = [&](float l) {
-        if (l == lowest) return 0;
-        const uint32_t key = key_of(l);
-        if (key < cut.key) return 0;
-        if (l != r.largest && ((double)l - (double)r.largest) * r.scale < z_least) return 0;
-        return key > cut.key ? 1 : 2;
+        if (!(l >= cut_value) || l == lowest) return 0;
+        if (by_weight && l != r.largest && ((double)l - (double)r.largest) * r.scale < z_least) return 0;
+        return l > cut_value ? 1 : 2;
     };
     const int per = (tiles + kSegments - 1) / kSegments, segments = (tiles + per - 1) / per;
     __syncthreads();
-    for (int s = wave; s < segments; s += kWaves) {
-        uint64_t mass = 0;
-        uint32_t ties = 0;
-        for (int t = s * per; t < min((s + 1) * per, tiles); ++t)
-            tile_values(row, a.vocab, t, lane, [&](int, float l, int) {
-                const int how = kept(l);
-                if (how == 1) mass += r.weight(l);
-                ties += how == 2;
-            });
-        const Sums all = wave_scan(Sums{ties, mass});
+    auto sum_tile = [&](const typename Logits<T>::Values& x, uint64_t& mass, uint32_t& ties) {
+        float top = lowest;
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = fmaxf(top, logits.value(x.v[i]));
+        if (!__any(top >= cut_value && top > lowest)) return;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int how = kept(logits.value(x.v[i]));
+            if (how == 1) mass += r.weight(logits.value(x.v[i]));
+            ties += how == 2;
+        }
+    };
+    auto segment_done = [&](int s, uint64_t mass, uint32_t ties) {
+        const bool some = __any(ties != 0 || mass != 0);
+        Sums all = {0, 0};
+        if (some) all = wave_scan(Sums{ties, mass});
         if (lane == 63) sh.counts[s] = all.count, sh.masses[s] = all.mass;
+    };
+    if (per == 1) {
+        logits.each([&](const typename Logits<T>::Values& x, int tile) {
+            uint64_t mass = 0;
+            uint32_t ties = 0;
+            sum_tile(x, mass, ties);
+            segment_done(tile, mass, ties);
+        });
+    } else {
+        for (int s = wave; s < segments; s += kWaves) {
+            uint64_t mass = 0;
+            uint32_t ties = 0;
+            for (int t = s * per; t < min((s + 1) * per, tiles); ++t) sum_tile(logits.load(t), mass, ties);
+            segment_done(s, mass, ties);
+        }
     }
     __syncthreads();
     // the weight of the cut's own value (its ties all have it)
-    float cut_value = __uint_as_float(cut.key & 0x80000000u ? cut.key & 0x7fffffffu : ~cut.key);
     const uint64_t each = cut.ties ? r.weight(cut_value) : 0;
     Sums own = {0, 0};
     if ((int)threadIdx.x < segments) own = Sums{sh.counts[threadIdx.x], sh.masses[threadIdx.x]};
@@ -329,17 +461,17 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     uint64_t before = sh.found_mass;
     uint32_t ties = sh.found_count;
     for (int t = sh.found * per; t < min((sh.found + 1) * per, tiles); ++t) {
+        const auto x = logits.load(t);
         uint64_t w[N];
         uint32_t tie[N];
-        int index = 0;
         Sums mine = {0, 0};
-        tile_values(row, a.vocab, t, lane, [&](int i, float l, int where) {
-            const int how = kept(l);
-            w[i] = how == 1 ? r.weight(l) : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int how = kept(logits.value(x.v[i]));
+            w[i] = how == 1 ? r.weight(logits.value(x.v[i])) : 0;
             tie[i] = how == 2;
             mine.count += tie[i];
-            if (i == 0) index = where;
-        });
+        }
         const Sums upto_ties = wave_scan(Sums{mine.count, 0});
         uint32_t rank = ties + upto_ties.count - mine.count;
 #pragma unroll
@@ -353,9 +485,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (m <= target && m + w[i] > target) {
-                    a.tokens[at] = index + i;
+                    a.tokens[at] = (t * 64 + lane) * N + i;
                     if (a.logp) {
-                        const float l = to_f32(row[index + i]);
+                        const float l = logits.value(x.v[i]);
                         const double d = l == r.largest ? 0.0 : ((double)l - (double)r.largest) / (double)temperature;
                         a.logp[at] = (float)(d - log((double)total * 0x1p-40));
                     }
