@@ -10,10 +10,13 @@
 //
 // No order is made. A cut is found as (value, how many of the tokens that have it): a
 // histogram over distances from the largest (monotone in l, so a bin is a stretch of the
-// order), then the bin that holds the cut, whose tokens are listed and compared with each
-// other (or, if they are many, told apart digit by digit of their values). The histogram first covers
-// weights down to 2^-16, the rest only being summed up, and all of them where the cut lies lower.
-// One workgroup has a row, which it reads four or five times, mostly from the caches.
+// order); then the bin that holds the cut, whose tokens are listed and compared with each
+// other, after a histogram of that bin alone if they are too many for it, or told apart digit by digit of
+// their values if that is not enough. Bins of 16-bit logits are 32 values each, so that the second histogram
+// has a bin for each value and ends the search.
+//
+// One workgroup has a row and reads it two to six times, mostly from the caches. Instructions bind it: about
+// 40 for a weight, of which 13 are on 64 bits, 64 tokens' a cycle on a compute unit.
 #include <algorithm>
 
 #include "inference.h"
@@ -25,9 +28,12 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
-// the bins' distance in bits of weight, first and where the cut lies lower: in all 16 bits, or
-// 42.67, behind which weights are 0
-constexpr float kBinsPerBit[2] = {128.f, 48.f};
+// Of fp32 logits the bins cover 42.67 bits of weight, behind which weights are 0; of 16-bit ones
+// all values, 32 in each.
+constexpr float kBinsPerBit = 48.f;
+constexpr int kShift = 5;
+// weights of 16-bit values that are tabled: those from the largest down
+constexpr int kTabled = 2048;
 constexpr int kBits = 40;
 constexpr int kSegments = 1024;
 constexpr int kListed = 512;
@@ -38,36 +44,59 @@ __device__ __forceinline__ uint32_t key_of(float l) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// 2^(i / 64), times 2^40.
-constexpr int kPowers = 64;
+// 2^(i / 256), times 2^40.
+constexpr int kPowers = 256;
 
 struct Row {
     float largest;
-    float bins;     // bins for each unit of distance
-    double scale;   // 64 log2(e) / T
+    float bins;  // for each unit of distance (fp32)
+    int top;     // the largest's place among the type's values (16 bits)
+    double scale;   // 256 log2(e) / T
     const double* powers;
-    // The token's weight. -infinity has none; of infinities each has 1. 2^(z / 64) with z = 64 a + i + f is
-    // 2^a, a value of the table and four terms of 2^(f / 64)'s series: within 2^-46 of itself.
+    // The token's weight. -infinity has none; of infinities each has 1. 2^(z / 256) with z = 256 a + i + f is
+    // 2^a, a value of the table and three terms of 2^(f / 256)'s series: within 2^-42 of itself.
+    // (No branch: the table's values of several tokens are asked for at once.)
     __device__ __forceinline__ uint64_t weight(float l) const {
-        double z = ((double)l - (double)largest) * scale;
-        z = l == largest ? 0.0 : z;
-        if (!(z > -42.0 * kPowers)) return 0;
-        const double n = rint(z), f = z - n;
+        // (from 2^-42 on a weight is none)
+        const double z = fmax(((double)l - (double)largest) * scale, -42.0 * kPowers), n = rint(z), f = z - n;
         const int whole = (int)n;
-        constexpr double c1 = 0.6931471805599453 / kPowers, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4;
-        const double series = fma(f, fma(f, fma(f, fma(f, c4, c3), c2), c1), 1.0);
-        const double w = ldexp(powers[whole & (kPowers - 1)] * series, whole >> 6);
+        constexpr double c1 = 0.6931471805599453 / kPowers, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3;
+        const double w = powers[whole & (kPowers - 1)] * fma(f, fma(f, fma(f, c3, c2), c1), 1.0);
+        const double power = __hiloint2double(((whole >> 8) + 1023) << 20, 0);
         // rounded to a whole number by the addition of 2^52
-        return (uint64_t)(__double_as_longlong(w + 0x1p52) - __double_as_longlong(0x1p52));
+        const uint64_t all = (uint64_t)(__double_as_longlong(fma(w, power, 0x1p52)) - __double_as_longlong(0x1p52));
+        return l == largest ? 1ull << kBits : l > -__builtin_huge_valf() && largest < __builtin_huge_valf() ? all : 0ull;
     }
-    // the bin, kBins or more where it lies behind them
-    __device__ __forceinline__ int bin(float l) const { return l == largest ? 0 : (int)fminf((largest - l) * bins, 1e6f); }
+    // The bin of a token, and its place in the finer bins that `outer` is divided into.
+    __device__ __forceinline__ int bin(float, float l) const { return l == largest ? 0 : (int)fminf((largest - l) * bins, kBins - 1.f); }
+    __device__ __forceinline__ int inner(float, float l, int outer) const {
+        return l == largest ? 0 : (int)fminf(fmaxf(((largest - l) * bins - outer) * kBins, 0.f), kBins - 1.f);
+    }
+    template <class T>
+    __device__ __forceinline__ int bin(T v, float) const {
+        return (top - place(v)) >> kShift;
+    }
+    template <class T>
+    __device__ __forceinline__ int inner(T v, float, int) const {
+        return (top - place(v)) & ((1 << kShift) - 1);
+    }
+    // the order of 16-bit values as whole numbers (-0 counts as 0), and the value at a place
+    template <class T>
+    static __device__ __forceinline__ int place(T v) {
+        const int b = __builtin_bit_cast(uint16_t, v);
+        return b & 0x8000 ? 0x8000 - (b & 0x7fff) : b | 0x8000;
+    }
+    template <class T>
+    static __device__ __forceinline__ T value_at(int place) {
+        return __builtin_bit_cast(T, (uint16_t)(place & 0x8000 ? place & 0x7fff : 0x8000 | (0x8000 - place)));
+    }
 };
 
 // A row of logits as a thread sees it: tiles of 64 N tokens for each wave in turn, a tile's
 // lane having N next to each other. -infinity past the end and in place of NaN.
 template <class T>
 struct Logits {
+    typedef T Type;
     static constexpr int N = 16 / sizeof(T);
     struct alignas(16) Values {
         T v[N];
@@ -103,12 +132,12 @@ struct Logits {
             now = next;
         }
     }
-    // f(l) for each token
+    // f(v, l) for each token: as it is stored, and its value
     template <class F>
     __device__ __forceinline__ void tokens(F f) const {
         each([&](const Values& x, int) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) f(value(x.v[i]));
+            for (int i = 0; i < N; ++i) f(x.v[i], value(x.v[i]));
         });
     }
 };
@@ -117,17 +146,17 @@ struct Shared {
     double powers[kPowers];
     uint64_t masses[kBins];
     uint64_t listed_weights[kListed];
+    uint64_t table[kTabled];
     uint64_t wave_mass[kWaves];
-    uint64_t above_mass, found_mass;
+    uint64_t above_mass, found_mass, cut_mass;
     uint32_t counts[kBins];
     float listed[kListed];
     uint32_t wave_count[kWaves];
     float best[kWaves];
     int best_at[kWaves];
     uint32_t above_count, found_count, listed_count;
-    int found;
     uint32_t cut_key, cut_ties;
-    uint64_t cut_mass;
+    int found;
 };
 
 // Inclusive sums over the block's threads of (count, mass).
@@ -135,17 +164,24 @@ struct Sums {
     uint32_t count;
     uint64_t mass;
 };
-__device__ __forceinline__ uint64_t up64(uint64_t v, int by) {
-    return (uint64_t)(uint32_t)__shfl_up((int)(uint32_t)(v >> 32), by) << 32 | (uint32_t)__shfl_up((int)(uint32_t)v, by);
+// Lanes are added in rows of 16, then over the four rows; a lane that nothing comes to adds 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ void scan_step(Sums& s) {
+    const uint32_t lo = moved<CTRL, ROWS>((uint32_t)s.mass), hi = moved<CTRL, ROWS>((uint32_t)(s.mass >> 32));
+    s.count += moved<CTRL, ROWS>(s.count);
+    s.mass += (uint64_t)hi << 32 | lo;
 }
 __device__ __forceinline__ Sums wave_scan(Sums s) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int by = 1; by < 64; by <<= 1) {
-        const uint32_t c = (uint32_t)__shfl_up((int)s.count, by);
-        const uint64_t m = up64(s.mass, by);
-        if (lane >= by) s.count += c, s.mass += m;
-    }
+    scan_step<0x111, 0xf>(s);  // row_shr:1
+    scan_step<0x112, 0xf>(s);
+    scan_step<0x114, 0xf>(s);
+    scan_step<0x118, 0xf>(s);
+    scan_step<0x142, 0xa>(s);  // row_bcast:15
+    scan_step<0x143, 0xc>(s);  // row_bcast:31
     return s;
 }
 __device__ __forceinline__ Sums block_scan(Sums s, Shared& sh) {
@@ -154,7 +190,11 @@ __device__ __forceinline__ Sums block_scan(Sums s, Shared& sh) {
     __syncthreads();
     if (lane == 63) sh.wave_count[wave] = s.count, sh.wave_mass[wave] = s.mass;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) s.count += sh.wave_count[w], s.mass += sh.wave_mass[w];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        s.count += w < wave ? sh.wave_count[w] : 0;
+        s.mass += w < wave ? sh.wave_mass[w] : 0;
+    }
     return s;
 }
 
@@ -203,16 +243,17 @@ __device__ __forceinline__ uint64_t block_total(uint64_t mass, Shared& sh) {
     return mass;
 }
 
-// The cut inside bin `bin`, above which lie `above_count` and `above_mass`: where the count
-// reaches `count` (BY_COUNT), or the mass `mass`.
-template <bool BY_COUNT, class L>
-__device__ __forceinline__ Cut cut_in_bin(const L& logits, const Row& r, int bin, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass, Shared& sh) {
-    const float lowest = -__builtin_huge_valf();
+// The cut among the tokens that `in(v, l)` says are there, above which lie `above_count` and
+// `above_mass`, if they are not too many to be listed: where the count reaches `count` (BY_COUNT), or the
+// mass `mass`.
+template <bool BY_COUNT, class L, class In>
+__device__ __forceinline__ bool cut_in_list(const L& logits, const Row& r, In in, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass,
+                                            Shared& sh, Cut& cut) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed_count = 0;
     __syncthreads();
-    logits.tokens([&](float l) {
-        if (l == lowest || r.bin(l) != bin) return;
+    logits.tokens([&](auto v, float l) {
+        if (!in(v, l)) return;
         const uint32_t at = atomicAdd(&sh.listed_count, 1u);
         if (at >= kListed) return;
         sh.listed[at] = l;
@@ -220,122 +261,161 @@ __device__ __forceinline__ Cut cut_in_bin(const L& logits, const Row& r, int bin
     });
     __syncthreads();
     const uint32_t n = sh.listed_count;
-    if (n <= kListed) {
-        // each token against all others: one of those that have the cut's value writes it down
-        if (threadIdx.x < n) {
-            const float l = sh.listed[threadIdx.x];
-            const uint64_t w = sh.listed_weights[threadIdx.x];
-            uint32_t c = above_count, same = 0;
-            uint64_t m = above_mass;
-            for (uint32_t k = 0; k < n; ++k) {
-                const float other = sh.listed[k];
-                const uint64_t ow = sh.listed_weights[k];
-                c += other > l;
-                m += other > l ? ow : 0;
-                same += other == l;
-            }
-            if (BY_COUNT ? c < count && c + same >= count : m < mass && m + same * w >= mass) {
-                const uint32_t ties = BY_COUNT ? count - c : (uint32_t)((mass - m + w - 1) / w);
-                sh.cut_key = key_of(l), sh.cut_ties = ties, sh.cut_mass = m + ties * w;  // the same from each of them
-            }
+    if (n > kListed) return false;
+    // each token against all others: one of those that have the cut's value writes it down
+    if (threadIdx.x < n) {
+        const float l = sh.listed[threadIdx.x];
+        const uint64_t w = sh.listed_weights[threadIdx.x];
+        uint32_t c = above_count, same = 0;
+        uint64_t m = above_mass;
+        for (uint32_t k = 0; k < n; ++k) {
+            const float other = sh.listed[k];
+            const uint64_t ow = sh.listed_weights[k];
+            c += other > l;
+            m += other > l ? ow : 0;
+            same += other == l;
         }
-        __syncthreads();
-        const Cut cut = {sh.cut_key, sh.cut_ties, sh.cut_mass};
-        __syncthreads();
-        return cut;
+        if (BY_COUNT ? c < count && c + same >= count : m < mass && m + same * w >= mass) {
+            const uint32_t ties = BY_COUNT ? count - c : (uint32_t)((mass - m + w - 1) / w);
+            sh.cut_key = key_of(l), sh.cut_ties = ties, sh.cut_mass = m + ties * w;  // the same from each of them
+        }
     }
-    uint32_t prefix = 0, in = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (threadIdx.x < 256) sh.counts[threadIdx.x] = 0, sh.masses[threadIdx.x] = 0;
-        __syncthreads();
-        logits.tokens([&](float l) {
-            if (l == lowest || r.bin(l) != bin) return;
-            const uint32_t key = key_of(l);
-            if (shift < 24 && key >> (shift + 8) != prefix) return;
-            const uint32_t digit = 255 - (key >> shift & 255);  // larger values first
-            atomicAdd(&sh.counts[digit], 1u);
-            atomicAdd((unsigned long long*)&sh.masses[digit], (unsigned long long)r.weight(l));
-        });
-        __syncthreads();
-        find<BY_COUNT>(256, count - above_count, mass - above_mass, sh);
-        prefix = prefix << 8 | (uint32_t)(255 - sh.found);
-        above_count += sh.above_count;
-        above_mass += sh.above_mass;
-        in = sh.found_count;
-    }
-    const uint64_t each = sh.found_mass / in;  // tokens of one value have one weight
     __syncthreads();
-    uint32_t ties = count - above_count;
-    if (!BY_COUNT) ties = (uint32_t)min((uint64_t)in, (mass - above_mass + each - 1) / each);
-    return Cut{prefix, ties, above_mass + ties * each};
+    cut = Cut{sh.cut_key, sh.cut_ties, sh.cut_mass};
+    __syncthreads();
+    return true;
 }
 
-// The histogram of the row's tokens; the weights of those behind the bins are returned.
+// The cut inside bin `bin`, above which lie `above_count` and `above_mass`. The histogram's memory is used.
+template <bool BY_COUNT, class L>
+__device__ __forceinline__ Cut cut_in_bin(const L& logits, const Row& r, int bin, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass,
+                                          Shared& sh) {
+    const float lowest = -__builtin_huge_valf();
+    Cut cut;
+    auto in_bin = [&](auto v, float l) { return l > lowest && r.bin(v, l) == bin; };
+    constexpr bool SHORT = L::N == 8;
+    if (!SHORT && cut_in_list<BY_COUNT>(logits, r, in_bin, count, mass, above_count, above_mass, sh, cut)) return cut;
+    // the bin's own histogram
+    constexpr int FINE = SHORT ? 1 << kShift : kBins;
+    __syncthreads();
+    for (int i = threadIdx.x; i < FINE; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
+    __syncthreads();
+    logits.tokens([&](auto v, float l) {
+        if (!in_bin(v, l)) return;
+        const int at = r.inner(v, l, bin);
+        if (SHORT || BY_COUNT) atomicAdd(&sh.counts[at], 1u);
+        if (!SHORT) atomicAdd((unsigned long long*)&sh.masses[at], (unsigned long long)r.weight(l));
+    });
+    __syncthreads();
+    if constexpr (SHORT) {  // a bin is a value
+        auto value = [&](int at) { return to_f32(Row::value_at<typename L::Type>(r.top - (bin << kShift) - at)); };
+        if (threadIdx.x < FINE) sh.masses[threadIdx.x] = sh.counts[threadIdx.x] * r.weight(value(threadIdx.x));
+        __syncthreads();
+        find<BY_COUNT>(FINE, count - above_count, mass - above_mass, sh);
+        above_count += sh.above_count, above_mass += sh.above_mass;
+        const float l = value(sh.found);
+        const uint64_t w = r.weight(l);
+        const uint32_t ties = BY_COUNT ? count - above_count : (uint32_t)min((uint64_t)sh.found_count, (mass - above_mass + w - 1) / w);
+        __syncthreads();
+        return Cut{key_of(l), ties, above_mass + ties * w};
+    } else {
+        find<BY_COUNT>(FINE, count - above_count, mass - above_mass, sh);
+        const int fine = sh.found;
+        above_count += sh.above_count, above_mass += sh.above_mass;
+        auto in_fine = [&](auto v, float l) { return in_bin(v, l) && r.inner(v, l, bin) == fine; };
+        if (cut_in_list<BY_COUNT>(logits, r, in_fine, count, mass, above_count, above_mass, sh, cut)) return cut;
+        uint32_t prefix = 0, in = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
+            if (threadIdx.x < 256) sh.counts[threadIdx.x] = 0, sh.masses[threadIdx.x] = 0;
+            __syncthreads();
+            logits.tokens([&](auto v, float l) {
+                if (!in_fine(v, l)) return;
+                const uint32_t key = key_of(l);
+                if (shift < 24 && key >> (shift + 8) != prefix) return;
+                const uint32_t digit = 255 - (key >> shift & 255);  // larger values first
+                atomicAdd(&sh.counts[digit], 1u);
+                atomicAdd((unsigned long long*)&sh.masses[digit], (unsigned long long)r.weight(l));
+            });
+            __syncthreads();
+            find<BY_COUNT>(256, count - above_count, mass - above_mass, sh);
+            prefix = prefix << 8 | (uint32_t)(255 - sh.found);
+            above_count += sh.above_count;
+            above_mass += sh.above_mass;
+            in = sh.found_count;
+        }
+        const uint64_t each = sh.found_mass / in;  // tokens of one value have one weight
+        __syncthreads();
+        uint32_t ties = count - above_count;
+        if (!BY_COUNT) ties = (uint32_t)min((uint64_t)in, (mass - above_mass + each - 1) / each);
+        return Cut{prefix, ties, above_mass + ties * each};
+    }
+}
+
+// The histogram of the row's tokens.
 template <class L>
-__device__ __forceinline__ uint64_t histogram(const L& logits, const Row& r, bool counts, bool masses, Shared& sh) {
+__device__ __forceinline__ void histogram(const L& logits, const Row& r, bool counts, bool masses, Shared& sh) {
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
     __syncthreads();
-    uint64_t behind = 0;
-    logits.tokens([&](float l) {
-        if (l == -__builtin_huge_valf()) return;
-        const int b = r.bin(l);
-        const uint64_t w = masses ? r.weight(l) : 0;
-        if (b >= kBins) {
-            behind += w;
-            return;
+    logits.each([&](const typename L::Values& x, int) {
+#pragma unroll
+        for (int from = 0; from < L::N; from += 4) {  // four at a time: registers
+            int bin[4];
+            uint64_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const auto v = x.v[from + i];
+                const float l = L::value(v);
+                bin[i] = l == -__builtin_huge_valf() ? -1 : r.bin(v, l);
+                w[i] = masses ? r.weight(l) : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (bin[i] < 0) continue;
+                if (counts) atomicAdd(&sh.counts[bin[i]], 1u);
+                if (masses) atomicAdd((unsigned long long*)&sh.masses[bin[i]], (unsigned long long)w[i]);
+            }
         }
-        if (counts) atomicAdd(&sh.counts[b], 1u);
-        if (masses) atomicAdd((unsigned long long*)&sh.masses[b], (unsigned long long)w);
     });
     __syncthreads();
-    return behind;
 }
 
 // What top-k and top-p keep.
 template <class L>
-__device__ __forceinline__ Cut find_cut(const L& logits, Row& r, uint32_t k, float p, Shared& sh) {
+__device__ __forceinline__ Cut find_cut(const L& logits, const Row& r, uint32_t k, float p, Shared& sh) {
     Cut cut = {0, 0, 0};  // all values are above
-    bool by_count = k > 0;
     const bool by_mass = p < 1.f;
-    for (int wide = 0; wide < 2 && (by_count || by_mass); ++wide) {
-        r.bins = (float)min(r.scale / kPowers * (double)kBinsPerBit[wide], 3e38);
-        const uint64_t behind = histogram(logits, r, by_count, by_mass, sh);
-        uint64_t all = 0;
+    if (!k && !by_mass) return cut;
+    histogram(logits, r, k != 0, by_mass, sh);
+    // the bins of the masses stay where they are wanted after the first cut has used their memory
+    uint64_t kept[kBins / kThreads], all = 0;
+    if (by_mass) {
+#pragma unroll
+        for (int i = 0; i < kBins / kThreads; ++i) all += kept[i] = sh.masses[threadIdx.x + i * kThreads];
+        all = block_total(all, sh);
+    }
+    bool by_count = k != 0;
+    if (by_count) {
+        find<true>(kBins, k, 0, sh);
+        by_count = sh.found >= 0;  // (else there are not so many)
+    }
+    if (by_count) {
+        cut = cut_in_bin<true>(logits, r, sh.found, k, 0, sh.above_count, sh.above_mass, sh);
+        all = cut.mass;
         if (by_mass) {
-            uint64_t own = behind;
-            for (int i = threadIdx.x; i < kBins; i += kThreads) own += sh.masses[i];
-            all = block_total(own, sh);
-        }
-        // the bins that the cuts are found in are looked up before the first cut uses their memory
-        int bin_k = -1;
-        uint32_t count_k = 0;
-        uint64_t mass_k = 0;
-        if (by_count) {
             __syncthreads();
-            find<true>(kBins, k, 0, sh);
-            bin_k = sh.found, count_k = sh.above_count, mass_k = sh.above_mass;
-            if (bin_k < 0 && !wide) continue;  // it lies behind them, or there are not so many
-            if (bin_k < 0) by_count = false;
+#pragma unroll
+            for (int i = 0; i < kBins / kThreads; ++i) sh.masses[threadIdx.x + i * kThreads] = kept[i];
         }
-        if (bin_k >= 0) {
-            cut = cut_in_bin<true>(logits, r, bin_k, k, 0, count_k, mass_k, sh);
-            all = cut.mass;
-        }
-        if (!by_mass) break;
-        const uint64_t target = max((uint64_t)1, (uint64_t)ceil(p > 0.f ? (double)p * (double)all : 0.0));
-        if (bin_k >= 0 && sh.listed_count > kListed) histogram(logits, r, false, true, sh);  // its memory was used
-        __syncthreads();
-        find<false>(kBins, 0, target, sh);
-        const int bin_p = sh.found;
-        const uint64_t mass_p = sh.above_mass;
-        if (bin_p < 0 && !wide) continue;
-        if (bin_p >= 0) {
-            const Cut c = cut_in_bin<false>(logits, r, bin_p, 0, target, 0, mass_p, sh);
-            if (bin_k < 0 || c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
-        }
-        break;
+    }
+    if (!by_mass) return cut;
+    const uint64_t target = max((uint64_t)1, (uint64_t)ceil(p > 0.f ? (double)p * (double)all : 0.0));
+    __syncthreads();
+    find<false>(kBins, 0, target, sh);
+    if (sh.found >= 0) {
+        const Cut c = cut_in_bin<false>(logits, r, sh.found, 0, target, 0, sh.above_mass, sh);
+        if (!by_count || c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
     }
     return cut;
 }
@@ -352,7 +432,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 
     // the largest, and where it is first
     float best = lowest;
-    logits.tokens([&](float l) { best = fmaxf(best, l); });
+    logits.tokens([&](T, float l) { best = fmaxf(best, l); });
 #pragma unroll
     for (int m = 32; m; m >>= 1) best = fmaxf(best, __shfl_xor(best, m));
     if (lane == 0) sh.best[wave] = best;
@@ -384,6 +464,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     Row r;
     r.largest = best;
     r.powers = sh.powers;
+    r.bins = (float)min(1.4426950408889634 / (double)temperature * (double)kBinsPerBit, 3e38);
+    if constexpr (N == 8) r.top = Row::place(from_f32<T>(best));
     r.scale = kPowers * 1.4426950408889634 / (double)temperature;
     const int k = a.top_k ? a.top_k[at] : 0;
     const float p = a.top_p ? a.top_p[at] : 1.f;
@@ -402,15 +484,25 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     };
     const int per = (tiles + kSegments - 1) / kSegments, segments = (tiles + per - 1) / per;
     __syncthreads();
+    // weights of 16-bit values from the largest to the cut's, where the table has room for them: 28 us
+    // instead of 54 for 131072 tokens, of which the nucleus was a third
+    bool tabled = false;
+    if constexpr (N == 8) {
+        tabled = cut.key && r.top - Row::place(from_f32<T>(cut_value)) < kTabled;
+        if (tabled)
+            for (int i = threadIdx.x; i < kTabled; i += kThreads) sh.table[i] = r.top >= i ? r.weight(to_f32(Row::value_at<T>(r.top - i))) : 0;
+        __syncthreads();
+    }
     auto sum_tile = [&](const typename Logits<T>::Values& x, uint64_t& mass, uint32_t& ties) {
-        float top = lowest;
-#pragma unroll
-        for (int i = 0; i < N; ++i) top = fmaxf(top, logits.value(x.v[i]));
-        if (!__any(top >= cut_value && top > lowest)) return;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int how = kept(logits.value(x.v[i]));
-            if (how == 1) mass += r.weight(logits.value(x.v[i]));
+            const float l = logits.value(x.v[i]);
+            if (!__any(l >= cut_value && l > lowest)) continue;  // most tokens of a row are not kept
+            const int how = kept(l);
+            uint64_t w;
+            if constexpr (N == 8) w = tabled ? sh.table[how ? r.top - Row::place(x.v[i]) : 0] : r.weight(l);
+            else w = r.weight(l);
+            mass += how == 1 ? w : 0;
             ties += how == 2;
         }
     };
