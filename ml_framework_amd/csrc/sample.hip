@@ -8,16 +8,24 @@
 // that top-k kept, min-p those of at least min_p of the first one's weight. The token
 // drawn is the first, by index, where the sum of kept weights passes u of their total.
 //
-// No order is made. A cut is found as (value, how many of the tokens that have it): a
-// histogram over distances from the largest (monotone in l, so a bin is a stretch of the
-// order); then the bin that holds the cut, whose tokens are listed and compared with each
-// other, after a histogram of that bin alone if they are too many for it, or told apart digit by digit of
-// their values if that is not enough. Bins of 16-bit logits are 32 values each, so that the second histogram
-// has a bin for each value and ends the search.
+// No order is made. A cut is found as (value, how many of the tokens that have it).
+// 16-bit logits are counted value by value, two counters a word, in 128 KB of shared
+// memory; sums over 128 values next to each other, then the values of the 128 that hold
+// the cut, end the search. Others (and rows where a counter runs over: 65536
+// tokens of one value) have a histogram over distances from the largest (monotone in l, so a
+// bin is a stretch of the order); the tokens of the bin that holds the cut are listed and
+// compared with each other, after a histogram of that bin alone if they are too many for
+// it, or told apart digit by digit of their values if that is not enough. Tokens too
+// far below the largest to have a weight take no part: rows masked by the type's
+// lowest value would meet at one counter.
 //
-// One workgroup has a row and reads it two to six times, mostly from the caches. Instructions bind it: about
-// 40 for a weight, of which 13 are on 64 bits, 64 tokens' a cycle on a compute unit.
+// One workgroup has a row and reads it three to six times, mostly from the caches. 64 x 131072
+// bf16 with top-p 93 us (32 values a histogram bin and every token's weight summed there: 132),
+// 256 x 50001 with top-k and top-p 50 (64), 1 x 32768 fp32 with all cuts 36. Where weights are
+// not those of 16-bit values, instructions bind it: about 40 for a weight, of which 13 are on
+// 64 bits, 64 tokens' a cycle on a compute unit.
 #include <algorithm>
+#include <type_traits>
 
 #include "inference.h"
 #include "io_types.h"
@@ -28,15 +36,17 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
-// Of fp32 logits the bins cover 42.67 bits of weight, behind which weights are 0; of 16-bit ones
-// all values, 32 in each.
+// The bins cover 42.67 bits of weight, behind which weights are 0.
 constexpr float kBinsPerBit = 48.f;
-constexpr int kShift = 5;
-// weights of 16-bit values that are tabled: those from the largest down
-constexpr int kTabled = 2048;
 constexpr int kBits = 40;
+// 2^-42 of the largest's weight and less is no weight
+constexpr double kNone = -42.0;
 constexpr int kSegments = 1024;
 constexpr int kListed = 512;
+// counters of 16-bit values, two a word, and the chunks of them that are summed up. Weights of
+// values take the same memory when the cuts are found.
+constexpr int kValueWords = 32768, kChunk = 128, kChunks = 2 * kValueWords / kChunk;
+constexpr int kTabled = kValueWords / 2;
 
 // The order of values as unsigned numbers (-0 counts as 0).
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -49,16 +59,17 @@ constexpr int kPowers = 256;
 
 struct Row {
     float largest;
-    float bins;  // for each unit of distance (fp32)
-    int top;     // the largest's place among the type's values (16 bits)
+    float least;  // tokens below it have no weight
+    float bins;   // for each unit of distance
+    int top;      // the largest's place among the type's values (16 bits)
+    int reach;    // and how far below it the places go that have weights
     double scale;   // 256 log2(e) / T
     const double* powers;
     // The token's weight. -infinity has none; of infinities each has 1. 2^(z / 256) with z = 256 a + i + f is
     // 2^a, a value of the table and three terms of 2^(f / 256)'s series: within 2^-42 of itself.
     // (No branch: the table's values of several tokens are asked for at once.)
     __device__ __forceinline__ uint64_t weight(float l) const {
-        // (from 2^-42 on a weight is none)
-        const double z = fmax(((double)l - (double)largest) * scale, -42.0 * kPowers), n = rint(z), f = z - n;
+        const double z = fmax(((double)l - (double)largest) * scale, kNone * kPowers), n = rint(z), f = z - n;
         const int whole = (int)n;
         constexpr double c1 = 0.6931471805599453 / kPowers, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3;
         const double w = powers[whole & (kPowers - 1)] * fma(f, fma(f, fma(f, c3, c2), c1), 1.0);
@@ -68,17 +79,9 @@ struct Row {
         return l == largest ? 1ull << kBits : l > -__builtin_huge_valf() && largest < __builtin_huge_valf() ? all : 0ull;
     }
     // The bin of a token, and its place in the finer bins that `outer` is divided into.
-    __device__ __forceinline__ int bin(float, float l) const { return l == largest ? 0 : (int)fminf((largest - l) * bins, kBins - 1.f); }
-    __device__ __forceinline__ int inner(float, float l, int outer) const {
+    __device__ __forceinline__ int bin(float l) const { return l == largest ? 0 : (int)fminf((largest - l) * bins, kBins - 1.f); }
+    __device__ __forceinline__ int inner(float l, int outer) const {
         return l == largest ? 0 : (int)fminf(fmaxf(((largest - l) * bins - outer) * kBins, 0.f), kBins - 1.f);
-    }
-    template <class T>
-    __device__ __forceinline__ int bin(T v, float) const {
-        return (top - place(v)) >> kShift;
-    }
-    template <class T>
-    __device__ __forceinline__ int inner(T v, float, int) const {
-        return (top - place(v)) & ((1 << kShift) - 1);
     }
     // the order of 16-bit values as whole numbers (-0 counts as 0), and the value at a place
     template <class T>
@@ -132,12 +135,12 @@ struct Logits {
             now = next;
         }
     }
-    // f(v, l) for each token: as it is stored, and its value
+    // f(l) for each token
     template <class F>
     __device__ __forceinline__ void tokens(F f) const {
         each([&](const Values& x, int) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) f(x.v[i], value(x.v[i]));
+            for (int i = 0; i < N; ++i) f(value(x.v[i]));
         });
     }
 };
@@ -145,12 +148,9 @@ struct Logits {
 struct Shared {
     double powers[kPowers];
     uint64_t masses[kBins];
-    uint64_t listed_weights[kListed];
-    uint64_t table[kTabled];
     uint64_t wave_mass[kWaves];
     uint64_t above_mass, found_mass, cut_mass;
     uint32_t counts[kBins];
-    float listed[kListed];
     uint32_t wave_count[kWaves];
     float best[kWaves];
     int best_at[kWaves];
@@ -158,6 +158,20 @@ struct Shared {
     uint32_t cut_key, cut_ties;
     int found;
 };
+
+// Shared memory of which a row has one use after the other.
+union Scratch {
+    uint32_t words[kValueWords];  // 16-bit logits only, as `table` is
+    uint64_t table[kTabled];
+    struct {
+        uint64_t weights[kListed];
+        float values[kListed];
+    } list;
+};
+__device__ __forceinline__ Scratch& scratch() {
+    extern __shared__ uint64_t memory[];
+    return *(Scratch*)memory;
+}
 
 // Inclusive sums over the block's threads of (count, mass).
 struct Sums {
@@ -205,25 +219,25 @@ struct Cut {
     uint64_t mass;  // what is kept
 };
 
-// In sh.counts / sh.masses [0, n), in rank's order, the entry that holds the cut:
-// the one where the count reaches `count` (BY_COUNT), or the mass `mass`. Sets
+// In n entries of sh.counts / sh.masses from `base` on, in rank's order, the one that holds
+// the cut: where the count reaches `count` (BY_COUNT), or the mass `mass`. Sets
 // sh.found (-1: none) and what lies above it and in it.
 template <bool BY_COUNT>
-__device__ __forceinline__ void find(int n, uint32_t count, uint64_t mass, Shared& sh) {
+__device__ __forceinline__ void find(int n, uint32_t count, uint64_t mass, Shared& sh, int base = 0) {
     if (threadIdx.x == 0) sh.found = -1;
     const int per = (n + kThreads - 1) / kThreads, first = threadIdx.x * per;
     Sums own = {0, 0};
-    for (int i = first; i < min(first + per, n); ++i) own.count += sh.counts[i], own.mass += sh.masses[i];
+    for (int i = first; i < min(first + per, n); ++i) own.count += sh.counts[base + i], own.mass += sh.masses[base + i];
     const Sums all = block_scan(own, sh);
     uint32_t c = all.count - own.count;
     uint64_t m = all.mass - own.mass;
     for (int i = first; i < min(first + per, n); ++i) {
-        const uint32_t c2 = c + sh.counts[i];
-        const uint64_t m2 = m + sh.masses[i];
+        const uint32_t c2 = c + sh.counts[base + i];
+        const uint64_t m2 = m + sh.masses[base + i];
         if (BY_COUNT ? c < count && c2 >= count : m < mass && m2 >= mass) {
             sh.found = i;
             sh.above_count = c, sh.above_mass = m;
-            sh.found_count = sh.counts[i], sh.found_mass = sh.masses[i];
+            sh.found_count = sh.counts[base + i], sh.found_mass = sh.masses[base + i];
         }
         c = c2, m = m2;
     }
@@ -243,34 +257,35 @@ __device__ __forceinline__ uint64_t block_total(uint64_t mass, Shared& sh) {
     return mass;
 }
 
-// The cut among the tokens that `in(v, l)` says are there, above which lie `above_count` and
+// The cut among the tokens that `in(l)` says are there, above which lie `above_count` and
 // `above_mass`, if they are not too many to be listed: where the count reaches `count` (BY_COUNT), or the
 // mass `mass`.
 template <bool BY_COUNT, class L, class In>
 __device__ __forceinline__ bool cut_in_list(const L& logits, const Row& r, In in, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass,
                                             Shared& sh, Cut& cut) {
+    auto& list = scratch().list;
     __syncthreads();
     if (threadIdx.x == 0) sh.listed_count = 0;
     __syncthreads();
-    logits.tokens([&](auto v, float l) {
-        if (!in(v, l)) return;
+    logits.tokens([&](float l) {
+        if (!in(l)) return;
         const uint32_t at = atomicAdd(&sh.listed_count, 1u);
         if (at >= kListed) return;
-        sh.listed[at] = l;
-        sh.listed_weights[at] = r.weight(l);
+        list.values[at] = l;
+        list.weights[at] = r.weight(l);
     });
     __syncthreads();
     const uint32_t n = sh.listed_count;
     if (n > kListed) return false;
     // each token against all others: one of those that have the cut's value writes it down
     if (threadIdx.x < n) {
-        const float l = sh.listed[threadIdx.x];
-        const uint64_t w = sh.listed_weights[threadIdx.x];
+        const float l = list.values[threadIdx.x];
+        const uint64_t w = list.weights[threadIdx.x];
         uint32_t c = above_count, same = 0;
         uint64_t m = above_mass;
         for (uint32_t k = 0; k < n; ++k) {
-            const float other = sh.listed[k];
-            const uint64_t ow = sh.listed_weights[k];
+            const float other = list.values[k];
+            const uint64_t ow = list.weights[k];
             c += other > l;
             m += other > l ? ow : 0;
             same += other == l;
@@ -290,66 +305,50 @@ __device__ __forceinline__ bool cut_in_list(const L& logits, const Row& r, In in
 template <bool BY_COUNT, class L>
 __device__ __forceinline__ Cut cut_in_bin(const L& logits, const Row& r, int bin, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass,
                                           Shared& sh) {
-    const float lowest = -__builtin_huge_valf();
     Cut cut;
-    auto in_bin = [&](auto v, float l) { return l > lowest && r.bin(v, l) == bin; };
-    constexpr bool SHORT = L::N == 8;
-    if (!SHORT && cut_in_list<BY_COUNT>(logits, r, in_bin, count, mass, above_count, above_mass, sh, cut)) return cut;
+    auto in_bin = [&](float l) { return l >= r.least && r.bin(l) == bin; };
+    if (cut_in_list<BY_COUNT>(logits, r, in_bin, count, mass, above_count, above_mass, sh, cut)) return cut;
     // the bin's own histogram
-    constexpr int FINE = SHORT ? 1 << kShift : kBins;
     __syncthreads();
-    for (int i = threadIdx.x; i < FINE; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
     __syncthreads();
-    logits.tokens([&](auto v, float l) {
-        if (!in_bin(v, l)) return;
-        const int at = r.inner(v, l, bin);
-        if (SHORT || BY_COUNT) atomicAdd(&sh.counts[at], 1u);
-        if (!SHORT) atomicAdd((unsigned long long*)&sh.masses[at], (unsigned long long)r.weight(l));
+    logits.tokens([&](float l) {
+        if (!in_bin(l)) return;
+        const int at = r.inner(l, bin);
+        if (BY_COUNT) atomicAdd(&sh.counts[at], 1u);
+        atomicAdd((unsigned long long*)&sh.masses[at], (unsigned long long)r.weight(l));
     });
     __syncthreads();
-    if constexpr (SHORT) {  // a bin is a value
-        auto value = [&](int at) { return to_f32(Row::value_at<typename L::Type>(r.top - (bin << kShift) - at)); };
-        if (threadIdx.x < FINE) sh.masses[threadIdx.x] = sh.counts[threadIdx.x] * r.weight(value(threadIdx.x));
+    find<BY_COUNT>(kBins, count - above_count, mass - above_mass, sh);
+    const int fine = sh.found;
+    above_count += sh.above_count, above_mass += sh.above_mass;
+    auto in_fine = [&](float l) { return in_bin(l) && r.inner(l, bin) == fine; };
+    if (cut_in_list<BY_COUNT>(logits, r, in_fine, count, mass, above_count, above_mass, sh, cut)) return cut;
+    uint32_t prefix = 0, in = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
-        find<BY_COUNT>(FINE, count - above_count, mass - above_mass, sh);
-        above_count += sh.above_count, above_mass += sh.above_mass;
-        const float l = value(sh.found);
-        const uint64_t w = r.weight(l);
-        const uint32_t ties = BY_COUNT ? count - above_count : (uint32_t)min((uint64_t)sh.found_count, (mass - above_mass + w - 1) / w);
+        if (threadIdx.x < 256) sh.counts[threadIdx.x] = 0, sh.masses[threadIdx.x] = 0;
         __syncthreads();
-        return Cut{key_of(l), ties, above_mass + ties * w};
-    } else {
-        find<BY_COUNT>(FINE, count - above_count, mass - above_mass, sh);
-        const int fine = sh.found;
-        above_count += sh.above_count, above_mass += sh.above_mass;
-        auto in_fine = [&](auto v, float l) { return in_bin(v, l) && r.inner(v, l, bin) == fine; };
-        if (cut_in_list<BY_COUNT>(logits, r, in_fine, count, mass, above_count, above_mass, sh, cut)) return cut;
-        uint32_t prefix = 0, in = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (threadIdx.x < 256) sh.counts[threadIdx.x] = 0, sh.masses[threadIdx.x] = 0;
-            __syncthreads();
-            logits.tokens([&](auto v, float l) {
-                if (!in_fine(v, l)) return;
-                const uint32_t key = key_of(l);
-                if (shift < 24 && key >> (shift + 8) != prefix) return;
-                const uint32_t digit = 255 - (key >> shift & 255);  // larger values first
-                atomicAdd(&sh.counts[digit], 1u);
-                atomicAdd((unsigned long long*)&sh.masses[digit], (unsigned long long)r.weight(l));
-            });
-            __syncthreads();
-            find<BY_COUNT>(256, count - above_count, mass - above_mass, sh);
-            prefix = prefix << 8 | (uint32_t)(255 - sh.found);
-            above_count += sh.above_count;
-            above_mass += sh.above_mass;
-            in = sh.found_count;
-        }
-        const uint64_t each = sh.found_mass / in;  // tokens of one value have one weight
+        logits.tokens([&](float l) {
+            if (!in_fine(l)) return;
+            const uint32_t key = key_of(l);
+            if (shift < 24 && key >> (shift + 8) != prefix) return;
+            const uint32_t digit = 255 - (key >> shift & 255);  // larger values first
+            atomicAdd(&sh.counts[digit], 1u);
+            atomicAdd((unsigned long long*)&sh.masses[digit], (unsigned long long)r.weight(l));
+        });
         __syncthreads();
-        uint32_t ties = count - above_count;
-        if (!BY_COUNT) ties = (uint32_t)min((uint64_t)in, (mass - above_mass + each - 1) / each);
-        return Cut{prefix, ties, above_mass + ties * each};
+        find<BY_COUNT>(256, count - above_count, mass - above_mass, sh);
+        prefix = prefix << 8 | (uint32_t)(255 - sh.found);
+        above_count += sh.above_count;
+        above_mass += sh.above_mass;
+        in = sh.found_count;
     }
+    const uint64_t each = sh.found_mass / in;  // tokens of one value have one weight
+    __syncthreads();
+    uint32_t ties = count - above_count;
+    if (!BY_COUNT) ties = (uint32_t)min((uint64_t)in, (mass - above_mass + each - 1) / each);
+    return Cut{prefix, ties, above_mass + ties * each};
 }
 
 // The histogram of the row's tokens.
@@ -365,9 +364,8 @@ __device__ __forceinline__ void histogram(const L& logits, const Row& r, bool co
             uint64_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const auto v = x.v[from + i];
-                const float l = L::value(v);
-                bin[i] = l == -__builtin_huge_valf() ? -1 : r.bin(v, l);
+                const float l = L::value(x.v[from + i]);
+                bin[i] = l >= r.least ? r.bin(l) : -1;
                 w[i] = masses ? r.weight(l) : 0;
             }
 #pragma unroll
@@ -381,13 +379,84 @@ __device__ __forceinline__ void histogram(const L& logits, const Row& r, bool co
     __syncthreads();
 }
 
+// 16-bit logits: the tokens of each value, of kChunk values their sums. False if a counter
+// ran over, which leaves fewer than there are.
+template <class L>
+__device__ __forceinline__ bool count_values(const L& logits, const Row& r, bool masses, Shared& sh) {
+    typedef typename L::Type T;
+    uint32_t* words = scratch().words;
+    const int chunks = r.reach / kChunk + 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < chunks * (kChunk / 8); i += kThreads) ((uint4*)words)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
+    __syncthreads();
+    uint32_t counted = 0;
+    logits.each([&](const typename L::Values& x, int) {
+#pragma unroll
+        for (int i = 0; i < L::N; ++i) {
+            if (!(L::value(x.v[i]) >= r.least)) continue;
+            const int at = r.top - Row::place(x.v[i]);
+            atomicAdd(&words[at >> 1], at & 1 ? 65536u : 1u);
+            ++counted;
+        }
+    });
+    __syncthreads();
+    for (int c = logits.wave; c < chunks; c += kWaves) {
+        const uint32_t word = words[c * 64 + logits.lane];
+        if (!__any(word != 0)) continue;
+        Sums s = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t n = i ? word >> 16 : word & 0xffffu;
+            s.count += n;
+            if (masses && __any(n != 0)) s.mass += n * r.weight(to_f32(Row::value_at<T>(r.top - (c * kChunk + 2 * logits.lane + i))));
+        }
+        s = wave_scan(s);
+        if (logits.lane == 63) sh.counts[c] = s.count, sh.masses[c] = s.mass;
+    }
+    __syncthreads();
+    if (logits.vocab < 65536) return true;
+    return block_total((uint64_t)counted - (threadIdx.x < kChunks ? sh.counts[threadIdx.x] : 0u), sh) == 0;
+}
+
+// The cut among the values of one chunk.
+template <bool BY_COUNT, class L>
+__device__ __forceinline__ Cut cut_in_chunk(const L&, const Row& r, int chunk, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass,
+                                            Shared& sh) {
+    auto value = [&](int at) { return to_f32(Row::value_at<typename L::Type>(r.top - (chunk * kChunk + at))); };
+    __syncthreads();
+    if (threadIdx.x < kChunk) {
+        const uint32_t n = scratch().words[chunk * (kChunk / 2) + threadIdx.x / 2] >> (threadIdx.x & 1) * 16 & 0xffffu;
+        sh.counts[kChunks + threadIdx.x] = n, sh.masses[kChunks + threadIdx.x] = n * r.weight(value(threadIdx.x));
+    }
+    __syncthreads();
+    find<BY_COUNT>(kChunk, count - above_count, mass - above_mass, sh, kChunks);
+    above_count += sh.above_count, above_mass += sh.above_mass;
+    const float l = value(sh.found);
+    const uint64_t w = r.weight(l);
+    const uint32_t ties = BY_COUNT ? count - above_count : (uint32_t)min((uint64_t)sh.found_count, (mass - above_mass + w - 1) / w);
+    __syncthreads();
+    return Cut{key_of(l), ties, above_mass + ties * w};
+}
+
 // What top-k and top-p keep.
 template <class L>
 __device__ __forceinline__ Cut find_cut(const L& logits, const Row& r, uint32_t k, float p, Shared& sh) {
     Cut cut = {0, 0, 0};  // all values are above
     const bool by_mass = p < 1.f;
     if (!k && !by_mass) return cut;
-    histogram(logits, r, k != 0, by_mass, sh);
+    bool counted = false;
+    if constexpr (L::N == 8) counted = count_values(logits, r, by_mass, sh);
+    if (!counted) histogram(logits, r, k != 0, by_mass, sh);
+    auto cut_in = [&](auto by_count, uint32_t count, uint64_t mass) {
+        constexpr bool BY_COUNT = decltype(by_count)::value;
+        find<BY_COUNT>(counted ? kChunks : kBins, count, mass, sh);
+        const int found = sh.found;
+        if (found < 0) return Cut{0, 0, 0};
+        if constexpr (L::N == 8)
+            if (counted) return cut_in_chunk<BY_COUNT>(logits, r, found, count, mass, sh.above_count, sh.above_mass, sh);
+        return cut_in_bin<BY_COUNT>(logits, r, found, count, mass, BY_COUNT ? sh.above_count : 0, sh.above_mass, sh);
+    };
     // the bins of the masses stay where they are wanted after the first cut has used their memory
     uint64_t kept[kBins / kThreads], all = 0;
     if (by_mass) {
@@ -395,28 +464,16 @@ __device__ __forceinline__ Cut find_cut(const L& logits, const Row& r, uint32_t 
         for (int i = 0; i < kBins / kThreads; ++i) all += kept[i] = sh.masses[threadIdx.x + i * kThreads];
         all = block_total(all, sh);
     }
-    bool by_count = k != 0;
-    if (by_count) {
-        find<true>(kBins, k, 0, sh);
-        by_count = sh.found >= 0;  // (else there are not so many)
-    }
-    if (by_count) {
-        cut = cut_in_bin<true>(logits, r, sh.found, k, 0, sh.above_count, sh.above_mass, sh);
-        all = cut.mass;
-        if (by_mass) {
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kBins / kThreads; ++i) sh.masses[threadIdx.x + i * kThreads] = kept[i];
-        }
-    }
+    if (k) cut = cut_in(std::true_type(), k, 0);  // none if there are not so many
+    if (cut.key) all = cut.mass;
     if (!by_mass) return cut;
     const uint64_t target = max((uint64_t)1, (uint64_t)ceil(p > 0.f ? (double)p * (double)all : 0.0));
     __syncthreads();
-    find<false>(kBins, 0, target, sh);
-    if (sh.found >= 0) {
-        const Cut c = cut_in_bin<false>(logits, r, sh.found, 0, target, 0, sh.above_mass, sh);
-        if (!by_count || c.key > cut.key || (c.key == cut.key && c.ties < cut.ties)) cut = c;
-    }
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) sh.masses[threadIdx.x + i * kThreads] = kept[i];
+    __syncthreads();
+    const Cut c = cut_in(std::false_type(), 0, target);
+    if (c.key && (!cut.key || c.key > cut.key || (c.key == cut.key && c.ties < cut.ties))) cut = c;
     return cut;
 }
 
@@ -432,7 +489,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 
     // the largest, and where it is first
     float best = lowest;
-    logits.tokens([&](T, float l) { best = fmaxf(best, l); });
+    logits.tokens([&](float l) { best = fmaxf(best, l); });
 #pragma unroll
     for (int m = 32; m; m >>= 1) best = fmaxf(best, __shfl_xor(best, m));
     if (lane == 0) sh.best[wave] = best;
@@ -465,8 +522,14 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     r.largest = best;
     r.powers = sh.powers;
     r.bins = (float)min(1.4426950408889634 / (double)temperature * (double)kBinsPerBit, 3e38);
-    if constexpr (N == 8) r.top = Row::place(from_f32<T>(best));
     r.scale = kPowers * 1.4426950408889634 / (double)temperature;
+    // (rounding it does not carry it past a value)
+    r.least = best < __builtin_huge_valf() ? fmaxf((float)((double)best + kNone * kPowers / r.scale), -3.4028235e38f) : best;
+    if constexpr (N == 8) {
+        r.top = Row::place(from_f32<T>(best));
+        // (rounded to 16 bits it may)
+        r.reach = min(r.top - Row::place(from_f32<T>(r.least)) + 1, 2 * kValueWords - 1);
+    }
     const int k = a.top_k ? a.top_k[at] : 0;
     const float p = a.top_p ? a.top_p[at] : 1.f;
     const Cut cut = find_cut(logits, r, k > 0 && k < a.vocab ? (uint32_t)k : 0u, p, sh);
@@ -476,31 +539,33 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     // What each segment of the row keeps: the mass above the cut's value, and how many have it.
     // 0: not kept, 1: kept, 2: kept if among the first ties
     const float cut_value = cut.key ? __uint_as_float(cut.key & 0x80000000u ? cut.key & 0x7fffffffu : ~cut.key) : lowest;
+    const float last = fmaxf(cut_value, r.least);
     const bool by_weight = min_p > 0.f;
     auto kept = [&](float l) {
-        if (!(l >= cut_value) || l == lowest) return 0;
+        if (!(l >= last)) return 0;
         if (by_weight && l != r.largest && ((double)l - (double)r.largest) * r.scale < z_least) return 0;
         return l > cut_value ? 1 : 2;
     };
     const int per = (tiles + kSegments - 1) / kSegments, segments = (tiles + per - 1) / per;
     __syncthreads();
-    // weights of 16-bit values from the largest to the cut's, where the table has room for them: 28 us
-    // instead of 54 for 131072 tokens, of which the nucleus was a third
+    // weights of 16-bit values from the largest to the last that is kept, where the table has room for
+    // them and there are not more of them than tokens
     bool tabled = false;
     if constexpr (N == 8) {
-        tabled = cut.key && r.top - Row::place(from_f32<T>(cut_value)) < kTabled;
+        const int values = (cut.key ? r.top - Row::place(from_f32<T>(cut_value)) : r.reach) + 1;
+        tabled = values <= kTabled && values <= a.vocab;
         if (tabled)
-            for (int i = threadIdx.x; i < kTabled; i += kThreads) sh.table[i] = r.top >= i ? r.weight(to_f32(Row::value_at<T>(r.top - i))) : 0;
+            for (int i = threadIdx.x; i < values; i += kThreads) scratch().table[i] = r.weight(to_f32(Row::value_at<T>(r.top - i)));
         __syncthreads();
     }
     auto sum_tile = [&](const typename Logits<T>::Values& x, uint64_t& mass, uint32_t& ties) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float l = logits.value(x.v[i]);
-            if (!__any(l >= cut_value && l > lowest)) continue;  // most tokens of a row are not kept
+            if (!__any(l >= last)) continue;  // most tokens of a row are not kept
             const int how = kept(l);
             uint64_t w;
-            if constexpr (N == 8) w = tabled ? sh.table[how ? r.top - Row::place(x.v[i]) : 0] : r.weight(l);
+            if constexpr (N == 8) w = tabled ? scratch().table[how ? r.top - Row::place(x.v[i]) : 0] : r.weight(l);
             else w = r.weight(l);
             mass += how == 1 ? w : 0;
             ties += how == 2;
@@ -596,9 +661,11 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 template <class T>
 int launch(Sample a, hipStream_t st) {
     constexpr int kMost = (int)(kMaxThreads / kThreads / 2);
+    constexpr size_t memory = sizeof(T) == 2 ? sizeof(Scratch) : sizeof(Scratch::list);
+    if (memory > 65536) SEERA_HIP_TRY(hipFuncSetAttribute((const void*)sample_rows<T>, hipFuncAttributeMaxDynamicSharedMemorySize, memory));
     for (int left = a.rows; left > 0; left -= kMost) {
         a.rows = std::min(left, kMost);
-        hipLaunchKernelGGL((sample_rows<T>), dim3(a.rows), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((sample_rows<T>), dim3(a.rows), dim3(kThreads), memory, st, a);
         SEERA_HIP_TRY(hipGetLastError());
         auto on = [&](auto& p, int64_t bytes) {
             if (p) p = (std::decay_t<decltype(p)>)((char*)p + a.rows * bytes);
