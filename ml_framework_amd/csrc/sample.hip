@@ -62,7 +62,7 @@ struct Row {
     float least;  // tokens below it have no weight
     float bins;   // for each unit of distance
     int top;      // the largest's place among the type's values (16 bits)
-    int reach;    // and how far below it the places go that have weights
+    int reach;    // and how far below it the last place is that may have a weight
     double scale;   // 256 log2(e) / T
     const double* powers;
     // The token's weight. -infinity has none; of infinities each has 1. 2^(z / 256) with z = 256 a + i + f is
@@ -123,6 +123,14 @@ struct Logits {
     static __device__ __forceinline__ float value(T v) {
         const float l = to_f32(v);
         return l == l ? l : -__builtin_huge_valf();
+    }
+    // How far below the place `top` each of 16-bit values lies (two a register). NaN comes out farther than
+    // the type's lowest value.
+    typedef uint16_t Steps __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ Steps below(const Values& x, int top) {
+        typedef int16_t Signed __attribute__((ext_vector_type(8)));
+        const Signed v = __builtin_bit_cast(Signed, x), sign = v >> 15;
+        return __builtin_bit_cast(Steps, (Signed)((int16_t)(top - 0x8000) - ((v ^ (sign & (int16_t)0x7fff)) - sign)));
     }
     // f(values, tile) for each of the wave's tiles, the next one being loaded meanwhile
     template <class F>
@@ -392,10 +400,11 @@ __device__ __forceinline__ bool count_values(const L& logits, const Row& r, bool
     __syncthreads();
     uint32_t counted = 0;
     logits.each([&](const typename L::Values& x, int) {
+        const typename L::Steps steps = L::below(x, r.top);
 #pragma unroll
         for (int i = 0; i < L::N; ++i) {
-            if (!(L::value(x.v[i]) >= r.least)) continue;
-            const int at = r.top - Row::place(x.v[i]);
+            const uint32_t at = steps[i];
+            if (at > (uint32_t)r.reach) continue;
             atomicAdd(&words[at >> 1], at & 1 ? 65536u : 1u);
             ++counted;
         }
@@ -527,8 +536,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     r.least = best < __builtin_huge_valf() ? fmaxf((float)((double)best + kNone * kPowers / r.scale), -3.4028235e38f) : best;
     if constexpr (N == 8) {
         r.top = Row::place(from_f32<T>(best));
-        // (rounded to 16 bits it may)
-        r.reach = min(r.top - Row::place(from_f32<T>(r.least)) + 1, 2 * kValueWords - 1);
+        const T least = from_f32<T>(r.least);  // may be rounded down past it
+        r.reach = r.top - Row::place(least) - (to_f32(least) < r.least);
     }
     const int k = a.top_k ? a.top_k[at] : 0;
     const float p = a.top_p ? a.top_p[at] : 1.f;
@@ -548,25 +557,41 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     };
     const int per = (tiles + kSegments - 1) / kSegments, segments = (tiles + per - 1) / per;
     __syncthreads();
-    // weights of 16-bit values from the largest to the last that is kept, where the table has room for
-    // them and there are not more of them than tokens
+    // The kept weights of 16-bit values, from the largest's to the last that is kept, if the table has room
+    // for them and there are not more of them than tokens: 12 instructions a token, not 40.
     bool tabled = false;
+    int values = 0, tie_at = -1;
     if constexpr (N == 8) {
-        const int values = (cut.key ? r.top - Row::place(from_f32<T>(cut_value)) : r.reach) + 1;
-        tabled = values <= kTabled && values <= a.vocab;
-        if (tabled)
-            for (int i = threadIdx.x; i < values; i += kThreads) scratch().table[i] = r.weight(to_f32(Row::value_at<T>(r.top - i)));
+        values = (cut.key ? r.top - Row::place(from_f32<T>(cut_value)) : r.reach) + 1;
+        tabled = values < kTabled && values <= a.vocab;
+        if (tabled) {
+            for (int i = threadIdx.x; i <= values; i += kThreads) {
+                const float l = to_f32(Row::value_at<T>(r.top - i));
+                scratch().table[i] = i < values && kept(l) == 1 ? r.weight(l) : 0;
+            }
+            if (cut.key && kept(cut_value) == 2) tie_at = values - 1;
+        }
         __syncthreads();
     }
     auto sum_tile = [&](const typename Logits<T>::Values& x, uint64_t& mass, uint32_t& ties) {
+        if constexpr (N == 8) {
+            if (tabled) {
+                const typename Logits<T>::Steps steps = logits.below(x, r.top);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int at = min((int)steps[i], values);
+                    mass += scratch().table[at];
+                    ties += at == tie_at;
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float l = logits.value(x.v[i]);
             if (!__any(l >= last)) continue;  // most tokens of a row are not kept
             const int how = kept(l);
-            uint64_t w;
-            if constexpr (N == 8) w = tabled ? scratch().table[how ? r.top - Row::place(x.v[i]) : 0] : r.weight(l);
-            else w = r.weight(l);
+            const uint64_t w = r.weight(l);
             mass += how == 1 ? w : 0;
             ties += how == 2;
         }
