@@ -557,31 +557,54 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     };
     const int per = (tiles + kSegments - 1) / kSegments, segments = (tiles + per - 1) / per;
     __syncthreads();
-    // The kept weights of 16-bit values, from the largest's to the last that is kept, if the table has room
-    // for them and there are not more of them than tokens: 12 instructions a token, not 40.
+    // The kept weights of 16-bit values, from the largest's to the last that is kept, are tabled: 15
+    // instructions a token, not 40. Values around zero (below 2^-12 of the farthest, more if the table has no
+    // room) would take most of the table and few tokens have them: they share an entry, and their tokens' weights
+    // are their own.
     bool tabled = false;
-    int values = 0, tie_at = -1;
+    int values = 0, tie_at = -1, gap_at = -1;
+    uint16_t gap_from = 0, gap_less = 0;
     if constexpr (N == 8) {
         values = (cut.key ? r.top - Row::place(from_f32<T>(cut_value)) : r.reach) + 1;
-        tabled = values < kTabled && values <= a.vocab;
+        const int above = r.top - 0x8000;  // the largest's places above zero
+        const float far = fmaxf(fabsf(r.largest), fabsf(to_f32(Row::value_at<T>(r.top - values + 1))));
+        const int half = max(Row::place(from_f32<T>(far * 0x1p-12f)) - 0x8000, (values - kTabled) / 2 + 2);
+        const int from = min(max(above - half, 0), values), to = min(max(above + half + 1, 0), values);
+        if (to > from) gap_at = gap_from = from, gap_less = to - from - 1;
+        const int entries = values - gap_less;
+        tabled = entries < kTabled && entries <= a.vocab;
+        auto value = [&](int i) { return to_f32(Row::value_at<T>(r.top - i)); };
         if (tabled) {
-            for (int i = threadIdx.x; i <= values; i += kThreads) {
-                const float l = to_f32(Row::value_at<T>(r.top - i));
-                scratch().table[i] = i < values && kept(l) == 1 ? r.weight(l) : 0;
+            for (int i = threadIdx.x; i <= entries; i += kThreads) {
+                const float l = value(i > gap_from ? i + gap_less : i);
+                scratch().table[i] = i < entries && i != gap_at && kept(l) == 1 ? r.weight(l) : 0;
             }
-            if (cut.key && kept(cut_value) == 2) tie_at = values - 1;
+            const bool in_gap = to > from && to == values;  // the last value
+            if (cut.key && kept(cut_value) == 2 && !in_gap) tie_at = entries - 1;
         }
         __syncthreads();
     }
     auto sum_tile = [&](const typename Logits<T>::Values& x, uint64_t& mass, uint32_t& ties) {
         if constexpr (N == 8) {
             if (tabled) {
-                const typename Logits<T>::Steps steps = logits.below(x, r.top);
+                typedef typename Logits<T>::Steps Steps;
+                const Steps steps = __builtin_elementwise_min(logits.below(x, r.top), (Steps)(uint16_t)values);
+                const Steps at = steps - __builtin_elementwise_min(__builtin_elementwise_max(steps, (Steps)gap_from) - gap_from, (Steps)gap_less);
+                bool gap = false;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int at = min((int)steps[i], values);
-                    mass += scratch().table[at];
-                    ties += at == tie_at;
+                    mass += scratch().table[at[i]];
+                    ties += at[i] == tie_at;
+                    gap |= at[i] == gap_at;
+                }
+                if (!__any(gap)) return;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (at[i] != gap_at) continue;
+                    const float l = logits.value(x.v[i]);
+                    const int how = kept(l);
+                    mass += how == 1 ? r.weight(l) : 0;
+                    ties += how == 2;
                 }
                 return;
             }
