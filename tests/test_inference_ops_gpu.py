@@ -450,6 +450,47 @@ def test_sample_long_rows(lib, rows, vocab):
     _check_sample(lib, l, u, s.F32)
 
 
+@pytest.mark.parametrize("dtype", [s.F16, s.BF16])
+@pytest.mark.parametrize("vocab", [300, 40000, 70001, 140000])
+def test_sample_of_16_bit_values(lib, dtype, vocab):
+    """Values are counted and tabled one by one: on either side of zero, across it, a few of them and nearly all."""
+    r = np.random.default_rng(vocab)
+    l = np.zeros((12, vocab))
+    tiny = 2.0**-20
+    l[0] = 1.0 + np.abs(r.standard_normal(vocab))
+    l[1] = -1.0 - np.abs(r.standard_normal(vocab))
+    l[2] = r.standard_normal(vocab) * tiny
+    l[3] = np.where(r.random(vocab) < 0.5, r.standard_normal(vocab) * tiny, r.standard_normal(vocab))
+    l[4] = -np.abs(r.standard_normal(vocab)) * 2.0 ** -r.integers(0, 14, vocab)
+    l[5] = np.abs(r.standard_normal(vocab)) * 2.0 ** -r.integers(0, 14, vocab)
+    l[6] = 0.25  # one counter for all, and more than it holds
+    l[7, : vocab // 2], l[7, vocab // 2 :] = 1.0, 1.0 + (2.0**-7 if dtype == s.BF16 else 2.0**-10)  # two in a word
+    l[8], l[8, ::7] = -(2.0**128 - 2.0**120) if dtype == s.BF16 else -65504.0, r.standard_normal(len(l[8, ::7]))
+    l[9] = np.where(r.random(vocab) < 0.9, 0.0, r.standard_normal(vocab))
+    l[10] = r.standard_normal(vocab) * 1000
+    l[11] = r.integers(-40, 2, vocab) * 0.5
+    u = r.random(12, np.float32)
+    for kw in ({}, {"top_p": 0.7}, {"top_k": vocab // 2}, {"top_k": vocab - 1, "top_p": 0.99}, {"top_p": r.random(12), "min_p": 0.2, "temperature": 0.7},
+               {"top_k": r.integers(1, vocab, 12), "temperature": 40.0}, {"min_p": 0.6, "temperature": 1e6}):
+        _check_sample(lib, l, u, dtype, **kw)
+
+
+@pytest.mark.parametrize("dtype", [s.F16, s.BF16])
+@pytest.mark.parametrize("temperature", [1.0, 3e4, 1e30, np.inf])
+def test_sample_of_every_16_bit_value(lib, dtype, temperature):
+    """Each bit pattern once, NaN and the infinities among them, in an order of no meaning."""
+    bits = np.random.default_rng(1).permutation(1 << 16).astype(np.uint16)
+    with np.errstate(invalid="ignore"):
+        l = s.load(bits if dtype == s.BF16 else bits.view(np.float16), dtype).astype(np.float64)
+    l[l == np.inf] = np.nan
+    l = np.tile(l, (4, 1))
+    for limit, row in ((100.0, l[1]), (1.0, l[2]), (-1.0, l[3])):
+        row[~(row <= limit)] = np.nan
+    u = np.array([0.1, 0.5, 0.9, 0.3], np.float32)
+    for kw in ({}, {"top_p": 0.5}, {"top_k": 20000}, {"top_k": 40000, "top_p": 0.9}):
+        _check_sample(lib, l, u, dtype, temperature=temperature, **kw)
+
+
 def test_sample_of_nearly_equal_logits(lib):
     """One bin of distances holds every token, and their values differ in the last places."""
     r = np.random.default_rng(5)
