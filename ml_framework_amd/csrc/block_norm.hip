@@ -1,5 +1,6 @@
 // block_norm.hip -- the norms after and before a block with its gate, residual
-// scale and residual, forward and backward (seera_hip_block_norm_fwd / _bwd).
+// scale and residual, forward and backward (seera_hip_block_norm_fwd / _bwd), and the
+// forward with its output in 8 bits (seera_hip_block_norm_fwd_f8).
 //
 //   z = rms(y) w1, u = z act(g) s, r' = r + u, n = rms(r') w2
 //   dr = dr' + rstd2 (q - r^ mean(q r^)),  q = dn w2, r^ = r' rstd2
@@ -16,14 +17,48 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "norm_rows.h"
+#include "f8.h"
+#include "inference.h"
+#include "io_types.h"
 #include "runtime.h"
 #include "sequence.h"
+#include "sequence_rules.h"
 
 namespace seera {
 namespace {
 
 constexpr int kThreads = 256;
+
+// The sum over a wave's 64 lanes, in every lane. The lanes are added in a fixed
+// order: along rows of 16, then over the four rows.
+__device__ __forceinline__ float wave_sum(float v) {
+    auto add = [&](auto ctrl, auto rows) {
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr:1
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});  // row_shr:2
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});  // row_shr:4
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});  // row_shr:8
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast:15
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast:31
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// The sum over the NT threads of a row, with one barrier: `halves` is the block's
+// own, kept over all of its sums.
+template <int NT>
+__device__ __forceinline__ float row_sum(float v, float* part, Halves& halves) {
+    v = wave_sum(v);
+    if (NT == 64) return v;
+    constexpr int W = NT / 64;
+    float* at = part + halves.next() * W;
+    if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += at[w];
+    return s;
+}
 
 __device__ __forceinline__ float block_sum(float v, float* part) {
     __syncthreads();
@@ -36,6 +71,11 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     return s;
 }
 
+// The activation of a gate.
+__device__ __forceinline__ float act_of(int act, float g) {
+    const float q = __builtin_amdgcn_rcpf(1.f + __expf(-g));
+    return act == SEERA_GATE_ACT_SILU ? g * q : q;
+}
 // The activation and its slope. The sigmoid's slope is the product of its two sides
 // q and e^-g q: 1 - q has no digit left where q is near 1. (Below g = -88 that is
 // infinity times 0, and the side is 1.)
@@ -47,8 +87,90 @@ __device__ __forceinline__ Act act_and_slope(int act, float g) {
     return act == SEERA_GATE_ACT_SILU ? Act{g * q, fmaf(g, d, q)} : Act{q, d};
 }
 
-// A row in the registers of NT threads, K wide packs each; ROWS rows a block.
-template <class T, int K, int NT, int ROWS, bool CUT>
+// 16 bytes of a row, moved as one access at any alignment of T (the hardware
+// takes unaligned addresses) and without a branch, so that nothing waits for a
+// load before its values are used. The pack at column `want` lies at `c`: moved
+// back where it would pass the row's end, so that some of its values belong to
+// the pack before it, or all of them. Values lo <= i < hi are its own: only they
+// enter sums and are stored. With CUT false (cols is a multiple of N) a pack is
+// whole or has no value.
+template <class T>
+struct Wide {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+template <int N, bool CUT>
+struct Place {
+    int c, lo, hi;
+    __device__ Place(int want, int cols) {
+        c = max(min(want, cols - N), 0);
+        lo = CUT ? min(want - c, N) : want < cols ? 0 : N;
+        hi = CUT ? min(N, cols - c) : N;
+    }
+    __device__ bool whole() const { return lo == 0 && (!CUT || hi == N); }
+    __device__ bool own(int i) const { return CUT ? i >= lo && i < hi : lo == 0; }
+    // sum + a b, of value i: not added where it is not the pack's own (a factor of 0 would
+    // make an infinity there a NaN)
+    __device__ float add(int i, float a, float b, float sum) const { return !CUT || own(i) ? fmaf(a, b, sum) : sum; }
+    // a pack's part of a sum
+    __device__ float part(float x) const { return CUT || lo == 0 ? x : 0.f; }
+};
+template <class T, bool CUT>
+__device__ __forceinline__ void load_wide(Wide<T>& to, const T* row, const Place<Wide<T>::N, CUT>& at, int cols) {
+    typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));
+    if (CUT && cols < Wide<T>::N) {
+#pragma unroll
+        for (int i = 0; i < Wide<T>::N; ++i) to.v[i] = i < at.hi ? row[i] : from_f32<T>(0.f);
+        return;
+    }
+    // past the cache where rows share no line of it: forward 16384 x 2048 69 -> 64 us (and 60
+    // with the stores); with cut rows the neighbour's line is lost, 8192 x 1501 30 -> 34
+    const Bits w = CUT ? *(const Bits*)(row + at.c) : __builtin_nontemporal_load((const Bits*)(row + at.c));
+    __builtin_memcpy(&to, &w, 16);
+}
+template <class T, bool CUT>
+__device__ __forceinline__ void store_wide(T* row, const Place<Wide<T>::N, CUT>& at, const Wide<T>& from) {
+    typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));
+    if (at.whole()) {
+        Bits w;
+        __builtin_memcpy(&w, &from, 16);
+        __builtin_nontemporal_store(w, (Bits*)(row + at.c));
+    } else if (CUT) {
+#pragma unroll
+        for (int i = 0; i < Wide<T>::N; ++i)
+            if (at.own(i)) row[at.c + i] = from.v[i];
+    }
+}
+// The N fp32 weights of a pack.
+template <int N, bool CUT>
+__device__ __forceinline__ void load_weights(float (&to)[N], const float* w, const Place<N, CUT>& at, int cols) {
+    if (CUT && cols < N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = i < at.hi ? w[i] : 0.f;
+        return;
+    }
+    __builtin_memcpy(to, w + at.c, sizeof(to));
+}
+
+// The largest of LANES (16 or 32) lanes next to each other, in each of them.
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    auto turn = [&](auto ctrl) { v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true)); };
+    turn(std::integral_constant<int, 0x128>{});  // row_ror:8
+    turn(std::integral_constant<int, 0x124>{});
+    turn(std::integral_constant<int, 0x122>{});
+    turn(std::integral_constant<int, 0x121>{});
+    if constexpr (LANES == 32) v = max(v, (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x401f));  // lane ^ 16
+    return v;
+}
+
+// A row in the registers of NT threads, K wide packs each; ROWS rows a block. With F8 its
+// output is codes, of n as it is before rounding: 128 columns are 16 lanes (32 with
+// fp32) next to each other, so a block's largest value is found within them and nothing
+// more is moved than the inputs, r' and a byte a value. 16384 x 4096 bf16 of all inputs,
+// 0.6 GB, in 115 us (5.3 TB/s, a copy's rate at this size); 16 x 4096 in 5, of which an
+// empty launch is 3.3.
+template <class T, int K, int NT, int ROWS, bool CUT, bool F8>
 __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape s) {
     constexpr int N = Wide<T>::N;
     typedef Place<N, CUT> At;
@@ -57,12 +179,107 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
     const int tid = threadIdx.x % NT;
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT;
     if (ROWS > 1 && row >= s.rows) return;  // whole waves: such rows take no barrier
+    const T* yr = (const T*)p.y + row * p.ldy;
+    const T* gr = (const T*)p.g + row * p.ldg;
+    const T* rr = (const T*)p.r + row * s.cols;
     auto place = [&](int k) { return At((k * NT + tid) * N, s.cols); };
-    Wide<T> y[K];
-    const float sum = residual_row<T, K, NT, CUT>(p, s, tid, row, part, halves, y);
-    if (!p.w2) return;
-    const float rstd2 = rsqrtf(row_sum<NT>(sum, part, halves) / s.cols + p.eps);
+    Wide<T> y[K], g[K], r[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) load_wide(y[k], yr, place(k), s.cols);
+    if (p.g)
+#pragma unroll
+        for (int k = 0; k < K; ++k) load_wide(g[k], gr, place(k), s.cols);
+    if (p.r)
+#pragma unroll
+        for (int k = 0; k < K; ++k) load_wide(r[k], rr, place(k), s.cols);
+    float rstd1 = 1.f;
+    if (p.w1) {
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const At at = place(k);
+            float own = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) own = at.add(i, to_f32(y[k].v[i]), to_f32(y[k].v[i]), own);
+            sum += at.part(own);
+        }
+        rstd1 = rsqrtf(row_sum<NT>(sum, part, halves) / s.cols + p.eps);
+        if (p.rstd1 && tid == 0) p.rstd1[row] = rstd1;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const At at = place(k);
+        float u[N], w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) u[i] = to_f32(y[k].v[i]);
+        if (p.w1) {
+            load_weights(w, p.w1, at, s.cols);
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] = u[i] * rstd1 * w[i];
+        }
+        if (p.g)
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] *= act_of(s.act, to_f32(g[k].v[i]));
+        if (p.s) {
+            load_weights(w, p.s, at, s.cols);
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] *= w[i];
+        }
+        if (p.r)
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] += to_f32(r[k].v[i]);
+        float own = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            y[k].v[i] = from_f32<T>(u[i]);  // as it is kept
+            own = at.add(i, to_f32(y[k].v[i]), to_f32(y[k].v[i]), own);
+        }
+        sum += at.part(own);
+    }
+    // a row's packs may reach into each other: all of it is read before any is written
+    if (CUT && NT > 64 && !p.w1) __syncthreads();
+    if (p.r_out)
+#pragma unroll
+        for (int k = 0; k < K; ++k) store_wide((T*)p.r_out + row * s.cols, place(k), y[k]);
+    if (!F8 && !p.w2) return;
+    const float rstd2 = p.w2 ? rsqrtf(row_sum<NT>(sum, part, halves) / s.cols + p.eps) : 1.f;
     if (p.rstd2 && tid == 0) p.rstd2[row] = rstd2;
+    if constexpr (F8) {
+        const int padded = (int)f8_padded(s.cols);
+        uint8_t* codes = p.codes + row * padded;
+        float* scales = p.scales + row * (padded / kF8Block);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const At at = place(k);
+            const int want = (k * NT + tid) * N;
+            float n[N], w[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) n[i] = to_f32(y[k].v[i]);
+            if (p.w2) {
+                load_weights(w, p.w2, at, s.cols);
+#pragma unroll
+                for (int i = 0; i < N; ++i) n[i] = n[i] * rstd2 * w[i];
+            }
+            uint32_t largest = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                n[i] = at.own(i) ? n[i] : 0.f;
+                largest = max(largest, magnitude(n[i]));
+            }
+            const F8Scale f(lanes_max<kF8Block / N>(largest));
+#pragma unroll
+            for (int i = 0; i < N; ++i) n[i] = f.quotient(n[i]);
+            // the values that are the pack's own come first, the row's padding after them
+            typedef std::conditional_t<N == 8, uint64_t, uint32_t> Bytes;
+            Bytes c = f8_codes(n[0], n[1], n[2], n[3]);
+            if constexpr (N == 8) c |= (uint64_t)f8_codes(n[4], n[5], n[6], n[7]) << 32;
+            if (CUT) c = at.lo < N ? c >> (8 * at.lo) : 0;
+            if (want < padded) *(Bytes*)(codes + want) = c;
+            if (want < padded && want % kF8Block == 0) scales[want / kF8Block] = f.scale;
+        }
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const At at = place(k);
@@ -321,15 +538,15 @@ __global__ __launch_bounds__(kSumCols * kSumRows) void norm_bwd_sums(const float
     out[c] = sum;
 }
 
-template <class T, int K, int NT, int ROWS>
+template <bool F8, class T, int K, int NT, int ROWS>
 int fwd_launch(NormShape s, NormFwd a, hipStream_t st) {
     // as many rows at once as a launch may have threads for
     constexpr int kMost = (int)std::min<int64_t>(kMaxThreads / NT / 2, 1 << 30);
     for (int left = s.rows; left > 0; left -= kMost) {
         s.rows = std::min(left, kMost);
         const dim3 grid((s.rows + ROWS - 1) / ROWS), block(NT * ROWS);
-        if (s.cols % Wide<T>::N) hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, true>), grid, block, 0, st, a, s);
-        else hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, false>), grid, block, 0, st, a, s);
+        if (s.cols % Wide<T>::N) hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, true, F8>), grid, block, 0, st, a, s);
+        else hipLaunchKernelGGL((norm_fwd_rows<T, K, NT, ROWS, false, F8>), grid, block, 0, st, a, s);
         SEERA_HIP_TRY(hipGetLastError());
         auto on = [&](auto& p, int64_t ld) {
             if (p) p = (std::decay_t<decltype(p)>)((char*)p + s.rows * ld);
@@ -337,24 +554,26 @@ int fwd_launch(NormShape s, NormFwd a, hipStream_t st) {
         on(a.y, a.ldy * sizeof(T)), on(a.g, a.ldg * sizeof(T));
         on(a.r, s.cols * sizeof(T)), on(a.r_out, s.cols * sizeof(T)), on(a.n_out, s.cols * sizeof(T));
         on(a.rstd1, sizeof(float)), on(a.rstd2, sizeof(float));
+        on(a.codes, f8_padded(s.cols)), on(a.scales, f8_padded(s.cols) / kF8Block * sizeof(float));
     }
     return SEERA_OK;
 }
 
 // A row in one wave up to 32 (16-bit) or 16 (fp32) values a lane: no barrier, and
 // many rows in flight (16 x 1024 bf16 in 4 us); wider ones in 256 or 1024 threads,
-// two to four packs each: 4096 x 8192 fp16 63 us, 5.4 TB/s.
-template <class T>
+// two to four packs each: 4096 x 8192 fp16 63 us, 5.4 TB/s. (Codes: a row's padding
+// has threads of its own.)
+template <bool F8, class T>
 int fwd_t(const NormShape& s, const NormFwd& a, hipStream_t st) {
     constexpr int N = Wide<T>::N;
-    const int packs = (s.cols + N - 1) / N;
-    if (packs <= 64) return fwd_launch<T, 1, 64, 4>(s, a, st);
-    if (packs <= 128) return fwd_launch<T, 2, 64, 4>(s, a, st);
-    if (packs <= 256) return fwd_launch<T, 4, 64, 4>(s, a, st);
-    if (packs <= 512) return fwd_launch<T, 2, 256, 1>(s, a, st);
-    if (packs <= 1024) return fwd_launch<T, 4, 256, 1>(s, a, st);
-    if (packs <= 2048) return fwd_launch<T, 2, 1024, 1>(s, a, st);
-    if constexpr (N == 4) return fwd_launch<T, 4, 1024, 1>(s, a, st);
+    const int packs = F8 ? (int)f8_padded(s.cols) / N : (s.cols + N - 1) / N;
+    if (packs <= 64) return fwd_launch<F8, T, 1, 64, 4>(s, a, st);
+    if (packs <= 128) return fwd_launch<F8, T, 2, 64, 4>(s, a, st);
+    if (packs <= 256) return fwd_launch<F8, T, 4, 64, 4>(s, a, st);
+    if (packs <= 512) return fwd_launch<F8, T, 2, 256, 1>(s, a, st);
+    if (packs <= 1024) return fwd_launch<F8, T, 4, 256, 1>(s, a, st);
+    if (packs <= 2048) return fwd_launch<F8, T, 2, 1024, 1>(s, a, st);
+    if constexpr (N == 4) return fwd_launch<F8, T, 4, 1024, 1>(s, a, st);
     return SEERA_OK;  // 16384 columns of 16 bits are 2048 packs
 }
 
@@ -406,7 +625,14 @@ int bwd_t(const NormShape& s, const NormBwd& a, hipStream_t st) {
 }  // namespace
 
 int block_norm_fwd(const NormShape& s, const NormFwd& a, hipStream_t st) {
-    return s.dtype == SEERA_DTYPE_F32 ? fwd_t<float>(s, a, st) : s.dtype == SEERA_DTYPE_F16 ? fwd_t<f16_t>(s, a, st) : fwd_t<bf16_t>(s, a, st);
+    return s.dtype == SEERA_DTYPE_F32   ? fwd_t<false, float>(s, a, st)
+           : s.dtype == SEERA_DTYPE_F16 ? fwd_t<false, f16_t>(s, a, st)
+                                        : fwd_t<false, bf16_t>(s, a, st);
+}
+int block_norm_fwd_f8(const NormShape& s, const NormFwd& a, hipStream_t st) {
+    return s.dtype == SEERA_DTYPE_F32   ? fwd_t<true, float>(s, a, st)
+           : s.dtype == SEERA_DTYPE_F16 ? fwd_t<true, f16_t>(s, a, st)
+                                        : fwd_t<true, bf16_t>(s, a, st);
 }
 int block_norm_bwd(const NormShape& s, const NormBwd& a, hipStream_t st) {
     return s.dtype == SEERA_DTYPE_F32 ? bwd_t<float>(s, a, st) : s.dtype == SEERA_DTYPE_F16 ? bwd_t<f16_t>(s, a, st) : bwd_t<bf16_t>(s, a, st);

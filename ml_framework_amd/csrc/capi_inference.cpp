@@ -14,7 +14,7 @@ namespace {
 // The largest matrix of codes: places in it, and its tiles' distances, stay in 63 bits.
 bool too_many(double rows, double row) { return rows * row > 0x1p60; }
 
-int norm_f8(const NormShape& s, const NormFwd& a, uint8_t* codes, float* scales, hipStream_t st) {
+int norm_f8(const NormShape& s, const NormFwd& a, hipStream_t st) {
     const char* op = "block_norm_f8";
     if (s.rows < 0 || s.cols < 0) return bad(op, "dims must be >= 0");
     if (s.cols > kNormMaxCols) return fail(SEERA_ERR_INVALID_ARGUMENT, "%s: cols %d above %d", op, s.cols, kNormMaxCols);
@@ -28,11 +28,11 @@ int norm_f8(const NormShape& s, const NormFwd& a, uint8_t* codes, float* scales,
     if (!(a.eps >= 0.f)) return bad(op, "eps must be >= 0");
     if (s.rows == 0 || s.cols == 0) return SEERA_OK;
     SEERA_TRY(required(op, e, {a.y}));
-    SEERA_TRY(required(op, 4, {scales}));
-    SEERA_TRY(required(op, 16, {codes}));
+    SEERA_TRY(required(op, 4, {a.scales}));
+    SEERA_TRY(required(op, 16, {a.codes}));
     SEERA_TRY(optional(op, e, {a.g, a.r, a.r_out}));
     SEERA_TRY(optional(op, 4, {a.w1, a.s, a.w2}));
-    return block_norm_fwd_f8(s, a, codes, scales, st);
+    return block_norm_fwd_f8(s, a, st);
 }
 
 int quantize(const QuantizeF8& a, hipStream_t st) {
@@ -93,8 +93,8 @@ extern "C" {
         uint8_t *codes, float *scales, int rows, int cols, int64_t ldy, int64_t ldg, float eps, int act, int dtype
 #define NORM_F8_CALL                                                                                                        \
     [&](hipStream_t st) {                                                                                                   \
-        return norm_f8({rows, cols, act, dtype}, {y, g, r, w1, s, w2, r_out, nullptr, nullptr, nullptr, ldy, ldg, eps},     \
-                       codes, scales, st);                                                                                  \
+        return norm_f8({rows, cols, act, dtype}, {y, g, r, w1, s, w2, r_out, nullptr, nullptr, nullptr, ldy, ldg, eps,      \
+                       codes, scales}, st);                                                                                 \
     }
 int seera_hip_block_norm_fwd_f8(NORM_F8_ARGS) { return now(NORM_F8_CALL); }
 int seera_hip_block_norm_fwd_f8_async(NORM_F8_ARGS, void* stream) { return later(stream, NORM_F8_CALL); }

@@ -1,5 +1,5 @@
 // inference.h -- internal entry points of the operators that a model answers with:
-// the block norm with its output in 8 bits (block_norm_f8.hip), weights in 8 bits
+// the block norm with its output in 8 bits (block_norm.hip), weights in 8 bits
 // (quantize_f8.hip), their product (matmul_f8.hip) and sampling (sample.hip).
 // Arguments are checked by capi_inference.cpp; all enqueue on `st` without
 // synchronizing and return a SEERA_* status.
@@ -14,7 +14,7 @@ namespace seera {
 
 // `a` without n_out and statistics; codes [rows][f8_padded(cols)], scales
 // [rows][f8_padded(cols) / 128].
-int block_norm_fwd_f8(const NormShape& s, const NormFwd& a, uint8_t* codes, float* scales, hipStream_t st);
+int block_norm_fwd_f8(const NormShape& s, const NormFwd& a, hipStream_t st);
 
 // w is [k, n], or [n, k] where transposed, rows ldw elements apart.
 struct QuantizeF8 {

@@ -51,6 +51,8 @@ struct NormFwd {
     float *rstd1, *rstd2;
     int64_t ldy, ldg;
     float eps;
+    uint8_t* codes;  // of the output in 8 bits (inference.h), in n_out's place
+    float* scales;
 };
 struct NormBwd {
     const void *y, *g, *r_out;
