@@ -204,6 +204,67 @@ def test_quantize_values_out_of_the_ordinary(lib, transposed):
     _check_weights(lib, w, s.F32, transposed)
 
 
+@pytest.mark.parametrize("dtype", [s.F16, s.BF16])
+@pytest.mark.parametrize("transposed", [0, 1])
+def test_quantize_16_bit_values_out_of_the_ordinary(lib, dtype, transposed):
+    """The largest of a block is positive or negative, in either half of a word, the least there is or none at all."""
+    r = np.random.default_rng(8)
+    w = r.standard_normal((640, 640)).astype(np.float32)
+    least, most = (2.0**-24, 65504.0) if dtype == s.F16 else (2.0**-133, 2.0**128 - 2.0**120)
+    for i, (at, v) in enumerate([((3, 4), 9.0), ((3, 5), -9.0), ((4, 4), -10.0), ((4, 7), 10.0), ((127, 127), -11.0), ((0, 0), most), ((0, 0), -most), ((64, 33), np.inf), ((65, 32), -np.inf),
+                                 ((1, 2), np.nan)]):
+        w[128 * (i // 5) + at[0], 128 * (i % 5) + at[1]] = v
+    w[256:384, :128] = 0.0
+    w[256:384, 128:256] = -0.0
+    w[256:384, 256:384] = 0.0
+    w[300, 300] = -least
+    w[256:384, 384:512] = r.integers(-3, 4, (128, 128)) * least
+    w[256:384, 512:] = r.choice(np.float32([most, -most]), (128, 128))
+    w = _seen(w, dtype).astype(np.float32)
+    _check_weights(lib, w, dtype, transposed)
+    _check_weights(lib, w[:600, :601], dtype, transposed, 1, 1)
+
+
+# ---- rows that lie far apart ----
+
+
+class Far:
+    """Rows of 16-bit values `ld` elements apart, of which only the rows are written and read."""
+
+    def __init__(self, lib, values, ld):
+        self.lib, self.ld, self.n = lib, ld, values.shape[1]
+        self.buf = DeviceBuffer(((len(values) - 1) * ld + self.n) * 2)
+        self.ptr = self.buf.ptr
+        for i, row in enumerate(s.store(values, s.BF16)):
+            capi.check(lib.seera_hip_memcpy_h2d(self.ptr + i * ld * 2, row.ctypes.data, row.nbytes))
+
+    def close(self):
+        self.buf.close()
+        capi.check(self.lib.seera_hip_empty_cache())
+
+
+def test_rows_beyond_32_bits(lib):
+    """Inputs whose rows lie so far apart that places in them pass 2^32 elements."""
+    r = np.random.default_rng(12)
+    ld, rows = 1 << 30, 6
+    x = _seen(r.standard_normal((rows, 300)), s.BF16)
+    far = Far(lib, x, ld)
+    codes, scales = Bytes((rows, 384)), Bytes((rows, 3), np.float32)
+    capi.call("seera_hip_block_norm_fwd_f8", far.ptr, None, None, None, None, None, None, codes.ptr, scales.ptr, rows, 300, ld, ld, 1e-6, 0, s.BF16)
+    want = q.quantize_rows(x.astype(np.float32))
+    assert np.array_equal(codes.values(), want[0]) and np.array_equal(scales.values(), want[1])
+    for transposed in (0, 1):
+        n, k = (rows, 300) if transposed else (300, rows)
+        codes, scales = Bytes((n, q.padded(k))), Bytes((q.padded(n) // 128, q.padded(k) // 128), np.float32)
+        capi.call("seera_hip_quantize_weights_f8", far.ptr, codes.ptr, scales.ptr, n, k, ld, transposed, s.BF16)
+        want = q.quantize_weights((x if transposed else np.ascontiguousarray(x.T)).astype(np.float32))
+        assert np.array_equal(codes.values(), want[0]) and np.array_equal(scales.values(), want[1])
+    u, tokens = Bytes((rows,), np.float32, r.random(rows)), Bytes((rows,), np.int32)
+    capi.call("seera_hip_sample", far.ptr, u.ptr, None, None, None, None, tokens.ptr, None, rows, 300, ld, s.BF16)
+    assert [q.sample_row(row, float(v))[0] for row, v in zip(x, u.values())] == list(tokens.values())
+    far.close()
+
+
 # ---- products ----
 
 
