@@ -20,10 +20,10 @@
 // lowest value would meet at one counter.
 //
 // One workgroup has a row and reads it three to six times, mostly from the caches. 64 x 131072
-// bf16 with top-p 93 us (32 values a histogram bin and every token's weight summed there: 132),
-// 256 x 50001 with top-k and top-p 50 (64), 1 x 32768 fp32 with all cuts 36. Where weights are
-// not those of 16-bit values, instructions bind it: about 40 for a weight, of which 13 are on
-// 64 bits, 64 tokens' a cycle on a compute unit.
+// bf16 with top-p 60 us (32 values a histogram bin and every token's weight summed there: 132),
+// 256 x 50001 fp16 with top-k and top-p 43 (64), 1 x 32768 fp32 with all cuts 36. Instructions
+// bind it, 118 a token of the last (40 of them a weight, of which 13 are on 64 bits), and with
+// 16-bit logits the random accesses to shared memory as well: an atomic and a read a token.
 #include <algorithm>
 #include <type_traits>
 
@@ -557,12 +557,13 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     };
     const int per = (tiles + kSegments - 1) / kSegments, segments = (tiles + per - 1) / per;
     __syncthreads();
-    // The kept weights of 16-bit values, from the largest's to the last that is kept, are tabled: 15
+    // The kept weights of 16-bit values, from the largest's to the last that is kept, are tabled: 12
     // instructions a token, not 40. Values around zero (below 2^-12 of the farthest, more if the table has no
     // room) would take most of the table and few tokens have them: they share an entry, and their tokens' weights
     // are their own.
     bool tabled = false;
-    int values = 0, tie_at = -1, gap_at = -1;
+    int values = 0, gap_at = -1;
+    constexpr int kTies = 48, kGap = 56;  // a tie and a value of the gap are counted in these bits of a weight
     uint16_t gap_from = 0, gap_less = 0;
     if constexpr (N == 8) {
         values = (cut.key ? r.top - Row::place(from_f32<T>(cut_value)) : r.reach) + 1;
@@ -577,10 +578,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
         if (tabled) {
             for (int i = threadIdx.x; i <= entries; i += kThreads) {
                 const float l = value(i > gap_from ? i + gap_less : i);
-                scratch().table[i] = i < entries && i != gap_at && kept(l) == 1 ? r.weight(l) : 0;
+                const int how = i < entries ? kept(l) : 0;
+                scratch().table[i] = i == gap_at ? 1ull << kGap : how == 1 ? r.weight(l) : how == 2 ? 1ull << kTies : 0;
             }
-            const bool in_gap = to > from && to == values;  // the last value
-            if (cut.key && kept(cut_value) == 2 && !in_gap) tie_at = entries - 1;
         }
         __syncthreads();
     }
@@ -590,14 +590,12 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
                 typedef typename Logits<T>::Steps Steps;
                 const Steps steps = __builtin_elementwise_min(logits.below(x, r.top), (Steps)(uint16_t)values);
                 const Steps at = steps - __builtin_elementwise_min(__builtin_elementwise_max(steps, (Steps)gap_from) - gap_from, (Steps)gap_less);
-                bool gap = false;
+                uint64_t all = 0;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    mass += scratch().table[at[i]];
-                    ties += at[i] == tie_at;
-                    gap |= at[i] == gap_at;
-                }
-                if (!__any(gap)) return;
+                for (int i = 0; i < N; ++i) all += scratch().table[at[i]];
+                mass += all & ((1ull << kTies) - 1);
+                ties += (uint32_t)(all >> kTies) & 0xff;
+                if (!__any(all >> kGap != 0)) return;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     if (at[i] != gap_at) continue;
@@ -645,10 +643,10 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     const uint64_t each = cut.ties ? r.weight(cut_value) : 0;
     Sums own = {0, 0};
     if ((int)threadIdx.x < segments) own = Sums{sh.counts[threadIdx.x], sh.masses[threadIdx.x]};
-    const uint32_t ties_before = block_scan(Sums{own.count, 0}, sh).count - own.count;
-    auto among = [&](uint32_t before, uint32_t n) { return before >= cut.ties ? 0u : min(n, cut.ties - before); };
-    const uint64_t own_mass = own.mass + among(ties_before, own.count) * each;
-    const uint64_t upto = block_scan(Sums{0, own_mass}, sh).mass;
+    const Sums above = block_scan(own, sh);
+    const uint32_t ties_before = above.count - own.count;
+    // the first `ties` of the ties: those of the segments before, and of the segment
+    const uint64_t upto = above.mass + min(above.count, cut.ties) * each, own_mass = upto - (above.mass - own.mass) - min(ties_before, cut.ties) * each;
     __syncthreads();
     if (threadIdx.x == kThreads - 1) sh.above_mass = upto;
     __syncthreads();
