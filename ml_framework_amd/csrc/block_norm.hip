@@ -168,7 +168,7 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // output is codes, of n as it is before rounding: 128 columns are 16 lanes (32 with
 // fp32) next to each other, so a block's largest value is found within them and nothing
 // more is moved than the inputs, r' and a byte a value. 16384 x 4096 bf16 of all inputs,
-// 0.6 GB, in 115 us (5.3 TB/s, a copy's rate at this size); 16 x 4096 in 5, of which an
+// 0.6 GB, in 117 us (5.2 TB/s, a copy's rate at this size); 16 x 4096 in 5, of which an
 // empty launch is 3.3.
 template <class T, int K, int NT, int ROWS, bool CUT, bool F8>
 __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape s) {
@@ -243,10 +243,14 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
 #pragma unroll
         for (int k = 0; k < K; ++k) store_wide((T*)p.r_out + row * s.cols, place(k), y[k]);
     if (!F8 && !p.w2) return;
-    const float rstd2 = p.w2 ? rsqrtf(row_sum<NT>(sum, part, halves) / s.cols + p.eps) : 1.f;
+    const float sum2 = p.w2 ? row_sum<NT>(sum, part, halves) : 0.f, rstd2 = rsqrtf(sum2 / s.cols + p.eps);
     if (p.rstd2 && tid == 0) p.rstd2[row] = rstd2;
     if constexpr (F8) {
         const int padded = (int)f8_padded(s.cols);
+        // An n that is off by a part of its last place falls on the other side of a code's border now and
+        // then, which is half a code's step: the root is corrected by its remainder, and one of the two
+        // roundings of n is made good.
+        const float x = sum2 / s.cols + p.eps, root = fmaf(0.5f * rstd2, fmaf(-x * rstd2, rstd2, 1.f), rstd2);
         uint8_t* codes = p.codes + row * padded;
         float* scales = p.scales + row * (padded / kF8Block);
 #pragma unroll
@@ -259,7 +263,10 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
             if (p.w2) {
                 load_weights(w, p.w2, at, s.cols);
 #pragma unroll
-                for (int i = 0; i < N; ++i) n[i] = n[i] * rstd2 * w[i];
+                for (int i = 0; i < N; ++i) {
+                    const float hat = n[i] * root, rest = fmaf(n[i], root, -hat);
+                    n[i] = fmaf(hat, w[i], rest * w[i]);
+                }
             }
             uint32_t largest = 0;
 #pragma unroll
