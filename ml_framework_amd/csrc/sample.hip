@@ -65,7 +65,7 @@ struct Row {
     int reach;    // and how far below it the last place is that may have a weight
     double scale;   // 256 log2(e) / T
     const double* powers;
-    // The token's weight. -infinity has none; of infinities each has 1. 2^(z / 256) with z = 256 a + i + f is
+    // The weight of a token that is not below `least`. Of infinities each has 1. 2^(z / 256) with z = 256 a + i + f is
     // 2^a, a value of the table and three terms of 2^(f / 256)'s series: within 2^-42 of itself.
     // (No branch: the table's values of several tokens are asked for at once.)
     __device__ __forceinline__ uint64_t weight(float l) const {
@@ -76,13 +76,12 @@ struct Row {
         const double power = __hiloint2double(((whole >> 8) + 1023) << 20, 0);
         // rounded to a whole number by the addition of 2^52
         const uint64_t all = (uint64_t)(__double_as_longlong(fma(w, power, 0x1p52)) - __double_as_longlong(0x1p52));
-        return l == largest ? 1ull << kBits : l > -__builtin_huge_valf() && largest < __builtin_huge_valf() ? all : 0ull;
+        return l == largest ? 1ull << kBits : all;  // (else an infinity has none)
     }
     // The bin of a token, and its place in the finer bins that `outer` is divided into.
-    __device__ __forceinline__ int bin(float l) const { return l == largest ? 0 : (int)fminf((largest - l) * bins, kBins - 1.f); }
-    __device__ __forceinline__ int inner(float l, int outer) const {
-        return l == largest ? 0 : (int)fminf(fmaxf(((largest - l) * bins - outer) * kBins, 0.f), kBins - 1.f);
-    }
+    // (Infinities, whose difference is none, share a bin too.)
+    __device__ __forceinline__ int bin(float l) const { return (int)fminf((largest - l) * bins, kBins - 1.f); }
+    __device__ __forceinline__ int inner(float l, int outer) const { return (int)fminf(fmaxf(((largest - l) * bins - outer) * kBins, 0.f), kBins - 1.f); }
     // the order of 16-bit values as whole numbers (-0 counts as 0), and the value at a place
     template <class T>
     static __device__ __forceinline__ int place(T v) {
@@ -96,7 +95,7 @@ struct Row {
 };
 
 // A row of logits as a thread sees it: tiles of 64 N tokens for each wave in turn, a tile's
-// lane having N next to each other. -infinity past the end and in place of NaN.
+// lane having N next to each other, -infinity past the end. (NaN passes no comparison below.)
 template <class T>
 struct Logits {
     typedef T Type;
@@ -119,10 +118,6 @@ struct Logits {
     }
     __device__ __forceinline__ Logits(const T* logits, int n) : row(logits), vocab(n), tiles((n + 64 * N - 1) / (64 * N)) {
         lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    }
-    static __device__ __forceinline__ float value(T v) {
-        const float l = to_f32(v);
-        return l == l ? l : -__builtin_huge_valf();
     }
     // How far below the place `top` each of 16-bit values lies (two a register). NaN comes out farther than
     // the type's lowest value.
@@ -148,7 +143,7 @@ struct Logits {
     __device__ __forceinline__ void tokens(F f) const {
         each([&](const Values& x, int) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) f(value(x.v[i]));
+            for (int i = 0; i < N; ++i) f(to_f32(x.v[i]));
         });
     }
 };
@@ -372,7 +367,7 @@ __device__ __forceinline__ void histogram(const L& logits, const Row& r, bool co
             uint64_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float l = L::value(x.v[from + i]);
+                const float l = to_f32(x.v[from + i]);
                 bin[i] = l >= r.least ? r.bin(l) : -1;
                 w[i] = masses ? r.weight(l) : 0;
             }
@@ -498,7 +493,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 
     // the largest, and where it is first
     float best = lowest;
-    logits.tokens([&](float l) { best = fmaxf(best, l); });
+    logits.tokens([&](float l) { best = l > best ? l : best; });
 #pragma unroll
     for (int m = 32; m; m >>= 1) best = fmaxf(best, __shfl_xor(best, m));
     if (lane == 0) sh.best[wave] = best;
@@ -512,7 +507,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
             logits.each([&](const typename Logits<T>::Values& x, int tile) {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (logits.value(x.v[i]) == best) first = min(first, (tile * 64 + lane) * N + i);
+                    if (to_f32(x.v[i]) == best) first = min(first, (tile * 64 + lane) * N + i);
             });
         }
 #pragma unroll
@@ -599,7 +594,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     if (at[i] != gap_at) continue;
-                    const float l = logits.value(x.v[i]);
+                    const float l = to_f32(x.v[i]);
                     const int how = kept(l);
                     mass += how == 1 ? r.weight(l) : 0;
                     ties += how == 2;
@@ -609,7 +604,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float l = logits.value(x.v[i]);
+            const float l = to_f32(x.v[i]);
             if (!__any(l >= last)) continue;  // most tokens of a row are not kept
             const int how = kept(l);
             const uint64_t w = r.weight(l);
@@ -670,8 +665,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
         Sums mine = {0, 0};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int how = kept(logits.value(x.v[i]));
-            w[i] = how == 1 ? r.weight(logits.value(x.v[i])) : 0;
+            const int how = kept(to_f32(x.v[i]));
+            w[i] = how == 1 ? r.weight(to_f32(x.v[i])) : 0;
             tie[i] = how == 2;
             mine.count += tie[i];
         }
@@ -690,7 +685,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
                 if (m <= target && m + w[i] > target) {
                     a.tokens[at] = (t * 64 + lane) * N + i;
                     if (a.logp) {
-                        const float l = logits.value(x.v[i]);
+                        const float l = to_f32(x.v[i]);
                         const double d = l == r.largest ? 0.0 : ((double)l - (double)r.largest) / (double)temperature;
                         a.logp[at] = (float)(d - log((double)total * 0x1p-40));
                     }
