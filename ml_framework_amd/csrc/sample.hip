@@ -20,9 +20,9 @@
 // lowest value would meet at one counter.
 //
 // One workgroup has a row and reads it three to six times, mostly from the caches. 64 x 131072
-// bf16 with top-p 60 us (32 values a histogram bin and every token's weight summed there: 132),
-// 256 x 50001 fp16 with top-k and top-p 43 (64), 1 x 32768 fp32 with all cuts 36. Instructions
-// bind it, 118 a token of the last (40 of them a weight, of which 13 are on 64 bits), and with
+// bf16 with top-p 59 us (32 values a histogram bin and every token's weight summed there: 132),
+// 256 x 50001 fp16 with top-k and top-p 42 (64), 1 x 32768 fp32 with all cuts 32. Instructions
+// bind it, about 100 a token of the last (35 of them a weight, 12 of these on 64 bits), and with
 // 16-bit logits the random accesses to shared memory as well: an atomic and a read a token.
 #include <algorithm>
 #include <type_traits>
@@ -64,19 +64,19 @@ struct Row {
     int top;      // the largest's place among the type's values (16 bits)
     int reach;    // and how far below it the last place is that may have a weight
     double scale;   // 256 log2(e) / T
+    double lowest;  // of the exponent's 256 parts: no weight, or where the largest is infinite (z is none) 1
     const double* powers;
     // The weight of a token that is not below `least`. Of infinities each has 1. 2^(z / 256) with z = 256 a + i + f is
     // 2^a, a value of the table and three terms of 2^(f / 256)'s series: within 2^-42 of itself.
     // (No branch: the table's values of several tokens are asked for at once.)
     __device__ __forceinline__ uint64_t weight(float l) const {
-        const double z = fmax(((double)l - (double)largest) * scale, kNone * kPowers), n = rint(z), f = z - n;
+        const double z = fmax(((double)l - (double)largest) * scale, lowest), n = rint(z), f = z - n;
         const int whole = (int)n;
         constexpr double c1 = 0.6931471805599453 / kPowers, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3;
         const double w = powers[whole & (kPowers - 1)] * fma(f, fma(f, fma(f, c3, c2), c1), 1.0);
         const double power = __hiloint2double(((whole >> 8) + 1023) << 20, 0);
         // rounded to a whole number by the addition of 2^52
-        const uint64_t all = (uint64_t)(__double_as_longlong(fma(w, power, 0x1p52)) - __double_as_longlong(0x1p52));
-        return l == largest ? 1ull << kBits : all;  // (else an infinity has none)
+        return (uint64_t)(__double_as_longlong(fma(w, power, 0x1p52)) - __double_as_longlong(0x1p52));
     }
     // The bin of a token, and its place in the finer bins that `outer` is divided into.
     // (Infinities, whose difference is none, share a bin too.)
@@ -527,6 +527,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     r.powers = sh.powers;
     r.bins = (float)min(1.4426950408889634 / (double)temperature * (double)kBinsPerBit, 3e38);
     r.scale = kPowers * 1.4426950408889634 / (double)temperature;
+    r.lowest = best < __builtin_huge_valf() ? kNone * kPowers : 0.0;
     // (rounding it does not carry it past a value)
     r.least = best < __builtin_huge_valf() ? fmaxf((float)((double)best + kNone * kPowers / r.scale), -3.4028235e38f) : best;
     if constexpr (N == 8) {
