@@ -16,12 +16,13 @@
 // bin is a stretch of the order); the tokens of the bin that holds the cut are listed and
 // compared with each other, after a histogram of that bin alone if they are too many for
 // it, or told apart digit by digit of their values if that is not enough. Tokens too
-// far below the largest to have a weight take no part: rows masked by the type's
-// lowest value would meet at one counter.
+// far below the largest to have a weight take no part, and the largest are counted apart where
+// many threads have met them: in rows masked by the type's lowest value or of equal logits,
+// all would meet at one counter.
 //
 // One workgroup has a row and reads it three to six times, mostly from the caches. 64 x 131072
-// bf16 with top-p 59 us (32 values a histogram bin and every token's weight summed there: 132),
-// 256 x 50001 fp16 with top-k and top-p 42 (64), 1 x 32768 fp32 with all cuts 32. Instructions
+// bf16 with top-p 61 us (32 values a histogram bin and every token's weight summed there: 132),
+// 256 x 50001 fp16 with top-k and top-p 44 (64), 1 x 32768 fp32 with all cuts 33. Instructions
 // bind it, about 100 a token of the last (35 of them a weight, 12 of these on 64 bits), and with
 // 16-bit logits the random accesses to shared memory as well: an atomic and a read a token.
 #include <algorithm>
@@ -59,6 +60,7 @@ constexpr int kPowers = 256;
 
 struct Row {
     float largest;
+    bool many;    // many tokens are the largest: they are counted apart
     float least;  // tokens below it have no weight
     float bins;   // for each unit of distance
     int top;      // the largest's place among the type's values (16 bits)
@@ -157,7 +159,7 @@ struct Shared {
     uint32_t wave_count[kWaves];
     float best[kWaves];
     int best_at[kWaves];
-    uint32_t above_count, found_count, listed_count;
+    uint32_t above_count, found_count, listed_count, tops;
     uint32_t cut_key, cut_ties;
     int found;
 };
@@ -309,7 +311,7 @@ template <bool BY_COUNT, class L>
 __device__ __forceinline__ Cut cut_in_bin(const L& logits, const Row& r, int bin, uint32_t count, uint64_t mass, uint32_t above_count, uint64_t above_mass,
                                           Shared& sh) {
     Cut cut;
-    auto in_bin = [&](float l) { return l >= r.least && r.bin(l) == bin; };
+    auto in_bin = [&](float l) { return l >= r.least && !(r.many && l == r.largest) && r.bin(l) == bin; };
     if (cut_in_list<BY_COUNT>(logits, r, in_bin, count, mass, above_count, above_mass, sh, cut)) return cut;
     // the bin's own histogram
     __syncthreads();
@@ -354,12 +356,15 @@ __device__ __forceinline__ Cut cut_in_bin(const L& logits, const Row& r, int bin
     return Cut{prefix, ties, above_mass + ties * each};
 }
 
-// The histogram of the row's tokens.
-template <class L>
+// The histogram of the row's tokens; with TOPS of all but the largest ones, whose number is sh.tops: in
+// rows of equal logits all would meet at one counter (64 x 131072 1.3 ms; 0.05 without them).
+template <bool TOPS, class L>
 __device__ __forceinline__ void histogram(const L& logits, const Row& r, bool counts, bool masses, Shared& sh) {
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
+    if (threadIdx.x == 0) sh.tops = 0;
     __syncthreads();
+    uint32_t tops = 0;
     logits.each([&](const typename L::Values& x, int) {
 #pragma unroll
         for (int from = 0; from < L::N; from += 4) {  // four at a time: registers
@@ -368,7 +373,8 @@ __device__ __forceinline__ void histogram(const L& logits, const Row& r, bool co
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float l = to_f32(x.v[from + i]);
-                bin[i] = l >= r.least ? r.bin(l) : -1;
+                if (TOPS) tops += l == r.largest;
+                bin[i] = l >= r.least && (!TOPS || l != r.largest) ? r.bin(l) : -1;
                 w[i] = masses ? r.weight(l) : 0;
             }
 #pragma unroll
@@ -379,12 +385,13 @@ __device__ __forceinline__ void histogram(const L& logits, const Row& r, bool co
             }
         }
     });
+    if (TOPS && tops) atomicAdd(&sh.tops, tops);
     __syncthreads();
 }
 
-// 16-bit logits: the tokens of each value, of kChunk values their sums. False if a counter
-// ran over, which leaves fewer than there are.
-template <class L>
+// 16-bit logits: the tokens of each value (but the largest, as above); of kChunk values their sums.
+// False if a counter ran over, which leaves fewer than there are.
+template <bool TOPS, class L>
 __device__ __forceinline__ bool count_values(const L& logits, const Row& r, bool masses, Shared& sh) {
     typedef typename L::Type T;
     uint32_t* words = scratch().words;
@@ -392,18 +399,21 @@ __device__ __forceinline__ bool count_values(const L& logits, const Row& r, bool
     __syncthreads();
     for (int i = threadIdx.x; i < chunks * (kChunk / 8); i += kThreads) ((uint4*)words)[i] = make_uint4(0, 0, 0, 0);
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh.counts[i] = 0, sh.masses[i] = 0;
+    if (threadIdx.x == 0) sh.tops = 0;
     __syncthreads();
-    uint32_t counted = 0;
+    uint32_t counted = 0, tops = 0;
     logits.each([&](const typename L::Values& x, int) {
         const typename L::Steps steps = L::below(x, r.top);
 #pragma unroll
         for (int i = 0; i < L::N; ++i) {
             const uint32_t at = steps[i];
-            if (at > (uint32_t)r.reach) continue;
+            if (TOPS) tops += at == 0;
+            if (TOPS ? at - 1 >= (uint32_t)r.reach : at > (uint32_t)r.reach) continue;
             atomicAdd(&words[at >> 1], at & 1 ? 65536u : 1u);
             ++counted;
         }
     });
+    if (TOPS && tops) atomicAdd(&sh.tops, tops);
     __syncthreads();
     for (int c = logits.wave; c < chunks; c += kWaves) {
         const uint32_t word = words[c * 64 + logits.lane];
@@ -450,23 +460,34 @@ __device__ __forceinline__ Cut find_cut(const L& logits, const Row& r, uint32_t 
     const bool by_mass = p < 1.f;
     if (!k && !by_mass) return cut;
     bool counted = false;
-    if constexpr (L::N == 8) counted = count_values(logits, r, by_mass, sh);
-    if (!counted) histogram(logits, r, k != 0, by_mass, sh);
+    if constexpr (L::N == 8) counted = r.many ? count_values<true>(logits, r, by_mass, sh) : count_values<false>(logits, r, by_mass, sh);
+    if (!counted) {
+        if (r.many) histogram<true>(logits, r, k != 0, by_mass, sh);
+        else histogram<false>(logits, r, k != 0, by_mass, sh);
+    }
+    const uint32_t tops = sh.tops;
+    const uint64_t top_mass = (uint64_t)tops << kBits;
     auto cut_in = [&](auto by_count, uint32_t count, uint64_t mass) {
         constexpr bool BY_COUNT = decltype(by_count)::value;
-        find<BY_COUNT>(counted ? kChunks : kBins, count, mass, sh);
+        if (BY_COUNT ? count <= tops : mass <= top_mass) {
+            const uint32_t ties = BY_COUNT ? count : (uint32_t)((mass + (1ull << kBits) - 1) >> kBits);
+            return Cut{key_of(r.largest), ties, (uint64_t)ties << kBits};
+        }
+        find<BY_COUNT>(counted ? kChunks : kBins, count - tops, mass - top_mass, sh);
         const int found = sh.found;
         if (found < 0) return Cut{0, 0, 0};
+        const uint32_t above_count = BY_COUNT ? sh.above_count + tops : 0;
+        const uint64_t above_mass = sh.above_mass + top_mass;
         if constexpr (L::N == 8)
-            if (counted) return cut_in_chunk<BY_COUNT>(logits, r, found, count, mass, sh.above_count, sh.above_mass, sh);
-        return cut_in_bin<BY_COUNT>(logits, r, found, count, mass, BY_COUNT ? sh.above_count : 0, sh.above_mass, sh);
+            if (counted) return cut_in_chunk<BY_COUNT>(logits, r, found, count, mass, above_count, above_mass, sh);
+        return cut_in_bin<BY_COUNT>(logits, r, found, count, mass, above_count, above_mass, sh);
     };
     // the bins of the masses stay where they are wanted after the first cut has used their memory
     uint64_t kept[kBins / kThreads], all = 0;
     if (by_mass) {
 #pragma unroll
         for (int i = 0; i < kBins / kThreads; ++i) all += kept[i] = sh.masses[threadIdx.x + i * kThreads];
-        all = block_total(all, sh);
+        all = block_total(all, sh) + top_mass;
     }
     if (k) cut = cut_in(std::true_type(), k, 0);  // none if there are not so many
     if (cut.key) all = cut.mass;
@@ -494,12 +515,17 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
     // the largest, and where it is first
     float best = lowest;
     logits.tokens([&](float l) { best = l > best ? l : best; });
+    const float own_best = best;
 #pragma unroll
     for (int m = 32; m; m >>= 1) best = fmaxf(best, __shfl_xor(best, m));
-    if (lane == 0) sh.best[wave] = best;
+    const int alike = __popcll(__ballot(own_best == best));
+    if (lane == 0) sh.best[wave] = best, sh.wave_count[wave] = alike;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) best = fmaxf(best, sh.best[w]);
+    int many = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) many += sh.best[w] == best ? (int)sh.wave_count[w] : 0;
     const float temperature = a.temperature ? a.temperature[at] : 1.f;
     if (best == lowest || !(temperature > 0.f)) {
         int first = 0x7fffffff;
@@ -524,6 +550,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(Sample a) {
 
     Row r;
     r.largest = best;
+    r.many = many >= kThreads / 16;  // as many threads have met it
     r.powers = sh.powers;
     r.bins = (float)min(1.4426950408889634 / (double)temperature * (double)kBinsPerBit, 3e38);
     r.scale = kPowers * 1.4426950408889634 / (double)temperature;
