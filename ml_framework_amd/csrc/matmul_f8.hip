@@ -15,7 +15,7 @@
 // and multiplied by v_mfma_f32_16x16x32_f16, at half the rate (2e-8 of the result).
 //
 // bf16 results, us: 1 x 4096 x 4096 5.4 (codes of W at a copy's 5 TB/s 3.4, an empty launch
-// 3.3), 64 x 12288 x 4096 15.8 (10 + 3.3), 8192 x 12288 x 4096 345 to 357: 2.3 PFLOP/s, where
+// 3.3), 64 x 12288 x 4096 15.8 (10 + 3.3), 8192 x 12288 x 4096 344 to 359: 2.3 PFLOP/s, where
 // a product without scales reaches 3.1. The last is bound by power: the clock falls to 1.65 GHz with
 // the matrix cores busy for 0.74 of it. Instructions of 32 x 32 x 64 are no faster (3.9 against
 // 4.3 PFLOP/s from registers alone); stores, DMA or scaling left out gave 5 % each.
