@@ -250,7 +250,8 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
         // An n that is off by a part of its last place falls on the other side of a code's border now and
         // then, which is half a code's step: the root is corrected by its remainder, and one of the two
         // roundings of n is made good.
-        const float x = sum2 / s.cols + p.eps, root = fmaf(0.5f * rstd2, fmaf(-x * rstd2, rstd2, 1.f), rstd2);
+        const float x = sum2 / s.cols + p.eps;
+        const float root = rstd2 > 0.f && rstd2 < __builtin_huge_valf() ? fmaf(0.5f * rstd2, fmaf(-x * rstd2, rstd2, 1.f), rstd2) : rstd2;
         uint8_t* codes = p.codes + row * padded;
         float* scales = p.scales + row * (padded / kF8Block);
 #pragma unroll
@@ -264,8 +265,8 @@ __global__ __launch_bounds__(NT * ROWS) void norm_fwd_rows(NormFwd p, NormShape 
                 load_weights(w, p.w2, at, s.cols);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float hat = n[i] * root, rest = fmaf(n[i], root, -hat);
-                    n[i] = fmaf(hat, w[i], rest * w[i]);
+                    const float hat = n[i] * root, over = fmaf(-n[i], root, hat);  // (a zero keeps its sign)
+                    n[i] = fmaf(hat, w[i], -(over * w[i]));
                 }
             }
             uint32_t largest = 0;

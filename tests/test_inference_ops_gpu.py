@@ -167,6 +167,24 @@ def test_norm_of_tiny_and_huge_values(lib):
     _check_norm(lib, 6, 256, s.F32, "", d={"y": y.astype(np.float64)})
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_norm_of_rows_whose_squares_leave_the_range(lib, eps):
+    """Sums of squares that are infinite or none: n is what the plain forward has, 0 or not a number."""
+    y = np.random.default_rng(9).standard_normal((5, 256)).astype(np.float32)
+    y *= np.float32([1e25, 1e30, 3e-30, 0.0, 1.0])[:, None]
+    d = {"y": y.astype(np.float64), "w2": np.ones(256)}
+    _, codes, scales = _norm(lib, d, s.F32, r_out=False, eps=eps)
+    m, w, n, r = (Rows(v.shape, s.F32, None, 0, v) for v in (d["y"], d["w2"][None], d["y"], d["y"]))
+    rstd2 = Bytes((5,), np.float32)
+    capi.call("seera_hip_block_norm_fwd", m.ptr, None, None, None, None, w.ptr, r.ptr, n.ptr, None, rstd2.ptr, 5, 256, 256, 256, eps, 0, s.F32)
+    want, want_scales = q.quantize_rows(n.values().astype(np.float32)[:4])
+    assert np.array_equal(scales[[0, 1, 3]], want_scales[[0, 1, 3]], equal_nan=True)
+    # (a root's unit in the last place, two or three roundings of n and one of the scale, on either side)
+    assert np.allclose(scales[2], want_scales[2], rtol=2.0**-21, atol=0, equal_nan=True)
+    assert np.array_equal(codes[:2], want[:2]) and not (want[:2] & 0x7F).any()  # zeros keep their signs
+    assert np.isfinite(scales[4]).all() and codes[4].any()
+
+
 # ---- weights ----
 
 
