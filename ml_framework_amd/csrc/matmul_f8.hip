@@ -484,8 +484,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
                 }
             }
         }
+        // the next tile adds these sums, times these scales, before its own: both are 0, as 0 * NaN is none
 #pragma unroll
         for (int i = 0; i < RING; ++i) sums[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < TAIL; ++i) before[i] = 0.f;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
