@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "f8.h"
+#include "f8_routes.h"
 #include "half_tile.h"
 #include "inference.h"
 #include "io_types.h"
@@ -515,48 +516,12 @@ int launch_tiles(const MatmulF8& g, hipStream_t st) {
     return SEERA_OK;
 }
 
-// The ways to compute a product: tiles of rows x cols, `at_once` workgroups a compute unit. A
-// launch takes `start` us (3.3 of them an empty one) and, for each slice of 128 along K, `few` where most
-// compute units have nothing to do, `full` where each has its workgroup, `pair` where each has two. Fitted
-// to times of 16 to 8192 rows with every way at K = 1024, 4096 and 16384 (bf16; fp32 below).
-enum Way { kSplit, kStream16x64, kStream32x32, kStream32x64, kStream64x64, kTiles128, kTiles128x256, kTiles256, kWays };
-struct Cost {
-    int rows, cols, at_once;
-    double start, few, full, pair;
-};
-constexpr Cost kCosts16[kWays] = {{16, 16, 1, 1.9, 0, 0, 0}, {16, 64, 1, 3.0, .20, .23, 0}, {32, 32, 1, 3.4, .18, .19, 0}, {32, 64, 1, 3.2, .22, .23, 0},
-                                  {64, 64, 2, 3.2, .38, .39, .49}, {128, 128, 1, 4.6, .49, .66, 0}, {128, 256, 1, 6.0, .68, .96, 0}, {256, 256, 1, 9.0, 1.15, 1.63, 0}};
-// (fp32 results: twice the matrix instructions' time, which binds the larger tiles)
-constexpr Cost kCosts32[kWays] = {{16, 16, 1, 1.9, 0, 0, 0}, {16, 64, 1, 3.2, .27, .28, 0}, {32, 32, 1, 3.6, .26, .26, 0}, {32, 64, 1, 3.4, .34, .34, 0},
-                                  {64, 64, 2, 3.4, .46, .48, .76}, {128, 128, 1, 4.6, 1.40, 1.45, 0}, {128, 256, 1, 6.0, 1.65, 1.95, 0}, {256, 256, 0, 0, 0, 0, 0}};
-
-double time_of(const Cost& c, int64_t m, int64_t n, int64_t slices, int64_t cus) {
-    const int64_t tiles = ((m + c.rows - 1) / c.rows) * ((n + c.cols - 1) / c.cols);
-    // the way from registers reads a row of A and of W for each of its 16 (where there are as many)
-    const double full = c.rows == 16 && c.cols == 16 ? .10 + .003 * std::min<int64_t>(m, 16) : c.full, few = c.few > 0 ? c.few : full;
-    const int64_t round = cus * c.at_once, rounds = tiles / round, rest = tiles % round;
-    double slice = rounds * (c.at_once == 2 ? c.pair : full);
-    if (rest) slice += c.at_once == 2 && rest > cus ? c.pair : few + (full - few) * std::min<int64_t>(rest, cus) / cus;
-    return c.start + slices * slice;
-}
-
 template <class T>
 int launch_t(const MatmulF8& g, hipStream_t st) {
     constexpr bool F32 = sizeof(T) == 4;
-    const Cost* costs = F32 ? kCosts32 : kCosts16;
     // offsets inside a tile are 31 bits
     const bool short_rows = (int64_t)256 * g.blocks * kF8Block < kMaxTileSpanBytes;
-    int best = kSplit;
-    if (g.blocks && short_rows) {
-        const int64_t cus = device_cus();
-        double least = g.m <= 16 ? time_of(costs[kSplit], g.m, g.n, g.blocks, cus) : 1e300;
-        for (int way = kSplit + 1; way < kWays; ++way) {
-            if (!costs[way].at_once) continue;
-            const double t = time_of(costs[way], g.m, g.n, g.blocks, cus);
-            if (t < least) least = t, best = way;
-        }
-    }
-    switch (best) {
+    switch (g.blocks && short_rows ? f8_way(F32, g.m, g.n, g.blocks, device_cus()) : kSplit) {
         case kStream16x64: return launch_stream<T, 16, 64, 5>(g, st);
         case kStream32x32: return launch_stream<T, 32, 32, 8>(g, st);
         case kStream32x64: return launch_stream<T, 32, 64, 5>(g, st);
@@ -565,8 +530,8 @@ int launch_t(const MatmulF8& g, hipStream_t st) {
         case kTiles128x256: return launch_tiles<T, 128, 256, 2, 4, 3>(g, st);
         case kTiles256:
             if constexpr (!F32) return launch_tiles<T, 256, 256, 2, 4, 2>(g, st);
+        default: return launch_split<T>(g, st);
     }
-    return launch_split<T>(g, st);
 }
 
 }  // namespace

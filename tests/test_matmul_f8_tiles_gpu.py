@@ -1,12 +1,75 @@
-"""Products of operands in 8 bits whose workgroups take several tiles one after
-another, at sizes where each of the large tiles is chosen."""
+"""Products of operands in 8 bits at sizes where each way of computing them is chosen, the large tiles with
+several for each workgroup, one after another."""
 import numpy as np
 import pytest
 
+from ml_framework_amd import capi
+from oracle import inference as q
 from oracle import sequence as s
-from tests.test_inference_ops_gpu import _matmul, _operands, lib  # noqa: F401 (a fixture)
+from tests.matmul_f8_ways import WAYS
+from tests.test_inference_ops_gpu import Bytes, _matmul, _operands, lib  # noqa: F401 (a fixture)
+from tests.test_sequence_ops_gpu import Rows, _close
 
 pytestmark = pytest.mark.gpu
+
+# a way's 16-bit code serves both types: every other size has one
+SIZES = [(s.F32 if f32 else (s.BF16, s.F16)[i % 2], m, n, k) for i, (f32, m, n, k, _) in enumerate(WAYS)]
+
+
+def _stored(ops, n, k, bias, dtype, gap, shift):
+    """C as it is stored, of operands on the host."""
+    m = ops[0].shape[0]
+    dev = [Bytes(x.shape, x.dtype, x) for x in ops]
+    b = Bytes(bias.shape, np.float32, bias)
+    c = Rows((m, n), dtype, n + gap, shift)
+    capi.call("seera_hip_matmul_f8", *[x.ptr for x in dev], b.ptr, c.ptr, m, n, k, n + gap, dtype)
+    return c.raw()
+
+
+def _parts(ops, bias, some=True):
+    """(where in C, operands and bias of that part): a few rows of each 64, with the first and the last, and four
+    blocks of 128 columns, the last one among them; or all of it."""
+    a, sa, w, sw = ops
+    m, n = a.shape[0], w.shape[0]
+    if not some:
+        yield np.s_[:, :], ops, bias
+        return
+    r = np.random.default_rng(m)
+    rows = np.unique(np.r_[0, m - 1, np.arange(m)[r.random(m) < 3 / 64]])
+    yield np.s_[rows], (a[rows], sa[rows], w, sw), bias
+    for block in sorted({0, 1, n // 256, (n - 1) // 128}):
+        cols = np.s_[block * 128:(block + 1) * 128]
+        yield np.s_[:, cols], (a, sa, w[cols], sw[block:block + 1]), bias[cols]
+
+
+@pytest.mark.parametrize("dtype,m,n,k", SIZES)
+def test_every_way(lib, dtype, m, n, k):  # noqa: F811
+    (a, sa, w, sw), bias = _operands(m, n, k, k, True)
+    ops = a, sa / 16, w, sw  # inside fp16's range
+    got = _stored(ops, n, k, bias, dtype, 3, 1)
+    for at, part, b in _parts(ops, bias):
+        want, bound = q.matmul(*part, b, fp32=dtype == s.F32)
+        _close(s.load(got[at], dtype), want, bound, dtype, "C")
+
+
+@pytest.mark.parametrize("dtype,m,n,k", SIZES)
+def test_every_way_is_exact_on_whole_numbers(lib, dtype, m, n, k):  # noqa: F811
+    """Small whole numbers with scales of powers of two: every sum is a whole number below 2^24 and no product is
+    cut, so that the one rounding is the result's, and a term in a wrong place shows."""
+    r = np.random.default_rng(m)
+    kp = q.padded(k)
+    a, w = np.zeros((m, kp), np.int8), np.zeros((n, kp), np.int8)
+    a[:, :k], w[:, :k] = r.integers(-8, 9, (m, k), np.int8), r.integers(-8, 9, (n, k), np.int8)
+    codes = q.encode(np.arange(-8, 9))
+    sa, sw = 2.0 ** r.integers(0, 3, (m, kp // 128)), 2.0 ** r.integers(0, 3, (q.padded(n) // 128, kp // 128))
+    bias = r.integers(-1000, 1001, n).astype(np.float32)
+    ops = codes[a + 8], sa.astype(np.float32), codes[w + 8], sw.astype(np.float32)
+    got = _stored(ops, n, k, bias, dtype, 0, 0)
+    # numbers that fp16 cannot hold are infinite
+    for at, part, b in _parts(ops, bias, m * n > 3e7):
+        want, _ = q.matmul(*part, b)
+        assert np.abs(want).max() < 2**24
+        assert np.array_equal(got[at], s.store(want, dtype)), "C"
 
 
 @pytest.mark.parametrize("scale", [np.nan, np.inf])
