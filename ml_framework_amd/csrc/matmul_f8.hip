@@ -88,6 +88,78 @@ __device__ __forceinline__ void store4(const MatmulF8& g, int m, int n, floatx4 
     for (int i = 0; n + i < g.n; ++i) c[i] = from_f32<T>(v[i] + (g.bias ? g.bias[n + i] : 0.f));
 }
 
+// Two scales are multiplied with each other first. Where their product overflows, or lies below the
+// normal numbers and has lost bits, a block's sums may still give ordinary values (0 among them, which times infinity is
+// NaN): there the sums are multiplied by the product of the mantissas, and the exponents added. (With a scale that is
+// infinite this comes out the same. A block's sums are below 2^25: a product that rounds to 0 costs less than 2^-125.)
+__device__ __forceinline__ bool out_of_range(float s) {
+    return __builtin_amdgcn_classf(s, 0x004 | 0x010 | 0x080 | 0x200);  // infinite or subnormal
+}
+__device__ __forceinline__ floatx4 add_scaled(floatx4 acc, floatx4 p, float sa, float sw) {
+    const float s = sa * sw, by = __builtin_amdgcn_frexp_mantf(sa) * __builtin_amdgcn_frexp_mantf(sw);
+    const int power = __builtin_amdgcn_frexp_expf(sa) + __builtin_amdgcn_frexp_expf(sw);
+    const bool apart = out_of_range(s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float there = fmaf(p[e], s, acc[e]), here = acc[e] + __builtin_amdgcn_ldexpf(p[e] * by, power);
+        acc[e] = apart ? here : there;
+    }
+    return acc;
+}
+
+// Whether any of the products that a lane has noted was out of range: three instructions for two of them, no
+// branch and no mask among the matrix instructions, where a comparison each costs 2 to 6 % of the small tiles' time. With
+// these, 8192 x 12288 x 4096 is as fast as without them, 64 x 4096 x 4096 9.3 -> 9.7 us, 256 x 4096 x 4096 15.3 -> 13.6 (the
+// compiler's order of the LDS reads, not theirs).
+struct Noted {
+    float most = 0.f;
+    uint32_t least = ~0u;  // without the sign, less 1: 0 is above all others
+    __device__ __forceinline__ void take(float s) {
+        most = fmaxf(most, fabsf(s));
+        least = min(least, (__float_as_uint(s) << 1) - 1);
+    }
+    __device__ __forceinline__ bool apart() const { return __any(most == __builtin_huge_valf() || least < (0x00800000u << 1) - 1); }
+};
+
+// The sums of every step-th block from `first` on, of scales whose product may be out of range: the kernels only
+// note such products, and their waves come here in the end.
+template <class T>
+__device__ __forceinline__ floatx4 sums_again(const MatmulF8& g, const uint8_t* a, const uint8_t* w, const float* sa, const float* sw, int first, int step) {
+    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int b = first; b < g.blocks; b += step)
+        acc = add_scaled(acc, products(Codes<T>(fragment(w + (int64_t)b * kF8Block)), Codes<T>(fragment(a + (int64_t)b * kF8Block))), sa[b], sw[b]);
+    return acc;
+}
+
+// Where a lane's operands of a tile of 16 x 16 begin in memory.
+struct Operands {
+    const uint8_t *a, *w;
+    const float *sa, *sw;
+    __device__ __forceinline__ Operands(const MatmulF8& g, int m0, int n0, int lane) {
+        const int64_t kp = (int64_t)g.blocks * kF8Block;
+        // rows past the end repeat the last one: their results are not stored
+        const int64_t row = min(m0 + (lane & 15), g.m - 1);
+        a = g.a + row * kp + 16 * (lane >> 4);
+        w = g.w + min(n0 + (lane & 15), g.n - 1) * kp + 16 * (lane >> 4);
+        sa = g.a_scales + row * g.blocks, sw = g.w_scales + (int64_t)(n0 / kF8Block) * g.blocks;
+    }
+};
+
+// The wave's ROWS x COLS results from (m0, n0) on in this way.
+template <class T, int ROWS, int COLS>
+__device__ __forceinline__ void results_again(const MatmulF8& g, int m0, int n0) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int t = 0; t < ROWS / 16 * (COLS / 16); ++t) {
+        const int m = m0 + t % (ROWS / 16) * 16, n = n0 + t / (ROWS / 16) * 16;
+        if (m >= g.m || n >= g.n) continue;
+        const Operands o(g, m, n, lane);
+        const floatx4 acc = sums_again<T>(g, o.a, o.w, o.sa, o.sw, 0, 1);
+        if (m + (lane & 15) < g.m) store4<T>(g, m + (lane & 15), n + 4 * (lane >> 4), acc);
+    }
+}
+
 // ---- few rows: operands from memory to registers ----
 
 // A tile of 16 x 16, with the blocks along K dealt to eight waves, whose sums are joined
@@ -100,20 +172,18 @@ __global__ __launch_bounds__(64 * kSplitWaves) void matmul_f8_split(MatmulF8 g) 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_n = (g.n + 15) / 16;
     const int n0 = (int)(blockIdx.x % tiles_n) * 16, m0 = (int)(blockIdx.x / tiles_n) * 16;
-    const int64_t kp = (int64_t)g.blocks * kF8Block;
-    // rows past the end repeat the last one: their results are not stored
-    const int64_t row = min(m0 + (lane & 15), g.m - 1);
-    const uint8_t* a = g.a + row * kp + 16 * (lane >> 4);
-    const uint8_t* w = g.w + min(n0 + (lane & 15), g.n - 1) * kp + 16 * (lane >> 4);
-    const float *sa = g.a_scales + row * g.blocks, *sw = g.w_scales + (int64_t)(n0 / kF8Block) * g.blocks;
+    const Operands o(g, m0, n0, lane);
     floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    Noted noted;
     for (int b = wave; b < g.blocks; b += kSplitWaves) {
-        const Codes<T> cw(fragment(w + (int64_t)b * kF8Block)), ca(fragment(a + (int64_t)b * kF8Block));
-        const float s = sa[b] * sw[b];
+        const Codes<T> cw(fragment(o.w + (int64_t)b * kF8Block)), ca(fragment(o.a + (int64_t)b * kF8Block));
+        const float s = o.sa[b] * o.sw[b];
         const floatx4 p = products(cw, ca);
+        noted.take(s);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] = fmaf(p[e], s, acc[e]);
     }
+    if (noted.apart()) acc = sums_again<T>(g, o.a, o.w, o.sa, o.sw, wave, kSplitWaves);
     sums[wave][lane] = acc;
     __syncthreads();
     if (wave) return;
@@ -222,6 +292,7 @@ __global__ __launch_bounds__(256, 1) void matmul_f8_stream(MatmulF8 g, int tiles
 #pragma unroll
     for (int k = 0; k < (STAGES - 1) * KS; ++k) load(k, smem + k * SLICE);
     int stage = 0;
+    Noted noted;
     for (int it = 0; it < rounds; ++it) {
         // this stage has landed, and every wave has read all of the one before, which is filled anew
         wait_vm<(STAGES - 2) * LOADS>();
@@ -263,14 +334,22 @@ __global__ __launch_bounds__(256, 1) void matmul_f8_stream(MatmulF8 g, int tiles
                 }
             }
         }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) noted.take(s[k][i]);
     }
+    if (noted.apart()) {
+        results_again<T, 16 * MT, 16 * NT>(g, m0 + wm, n0 + wn);
+    } else {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int m = m0 + wm + 16 * i + r, n = n0 + wn + 16 * j + 4 * gk;
-            if (m < g.m) store4<T>(g, m, n, acc[i][j]);
-        }
+            for (int j = 0; j < NT; ++j) {
+                const int m = m0 + wm + 16 * i + r, n = n0 + wn + 16 * j + 4 * gk;
+                if (m < g.m) store4<T>(g, m, n, acc[i][j]);
+            }
+    }
     wait_vm<0>();  // (zeros on their way to LDS that another block may have next)
 }
 
@@ -380,7 +459,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
     auto col_of = [](int t) { return t < HEAD ? t % NT : (t - HEAD) / TAIL; };
     floatx4 acc[MT][NT], sums[RING];
     Codes<T> w[NT], a[AS];
-    float scale[MT], w_scale, before[TAIL];  // of this slice; of the last rows in the one before
+    float scale[MT], w_scale, quarter[MT / 4], before[TAIL];  // of this slice; of the last rows in the one before
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -398,6 +477,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
         const float* s = (const float*)(stage + A_BYTES + W_BYTES);
         __builtin_memcpy(scale, __builtin_assume_aligned(s + wm + r * MT, MT % 4 == 0 ? 16 : 8), sizeof(scale));
         w_scale = s[BM + wn / kF8Block];
+        // four lanes have the same rows' scales: each looks at a quarter of them
+        __builtin_memcpy(quarter, __builtin_assume_aligned(s + wm + r * MT + gk * (MT / 4), MT), sizeof(quarter));
     };
     auto add = [&](int t, float by) {
 #pragma unroll
@@ -414,6 +495,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
 #pragma unroll
     for (int j = 0; j < NT; ++j) read_w(smem, j);
     int stage = 0;
+    Noted noted;
     for (; v < total; v += gridDim.x) {
         for (int s = 0; s < slices; ++s) {
             uint8_t* now = smem + stage * STAGE;
@@ -427,6 +509,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
                 }
                 if (t >= RING && t - RING < HEAD && (t - RING) % NT == 0) scale[(t - RING) / NT] *= w_scale;
                 if (t >= RING && t - RING >= HEAD && t - RING < HEAD + TAIL) scale[row_of(t - RING)] *= w_scale;
+                if (t == RING + 1)
+#pragma unroll
+                    for (int i = 0; i < MT / 4; ++i) noted.take(quarter[i] * w_scale);
                 if (t < RING) add(ALL - RING + t, before[row_of(ALL - RING + t) - (MT - TAIL)]);
                 else add(t - RING, scale[row_of(t - RING)]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -451,37 +536,42 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void matmul_f8_tiles(MatmulF8 g, i
         }
 #pragma unroll
         for (int t = ALL - RING; t < ALL; ++t) add(t, before[row_of(t) - (MT - TAIL)]);
-        typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));  // at any alignment of T
-        const bool whole = tile.m0 + BM <= g.m && tile.n0 + BN <= g.n;
+        if (noted.apart()) {
+            results_again<T, 16 * MT, 16 * NT>(g, tile.m0 + wm, tile.n0 + wn);
+            noted = Noted();
+        } else {
+            typedef uint32_t Bits __attribute__((ext_vector_type(4), aligned(2), may_alias));  // at any alignment of T
+            const bool whole = tile.m0 + BM <= g.m && tile.n0 + BN <= g.n;
 #pragma unroll
-        for (int q = 0; q < NT / JJ; ++q) {
-            const int n = tile.n0 + wn + 16 * JJ * q + N * gk;
-            float bias[N];
+            for (int q = 0; q < NT / JJ; ++q) {
+                const int n = tile.n0 + wn + 16 * JJ * q + N * gk;
+                float bias[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) bias[e] = 0.f;
-            if (g.bias) {
-                if (whole) {
-                    __builtin_memcpy(bias, g.bias + n, sizeof(bias));
-                } else {
+                for (int e = 0; e < N; ++e) bias[e] = 0.f;
+                if (g.bias) {
+                    if (whole) {
+                        __builtin_memcpy(bias, g.bias + n, sizeof(bias));
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) bias[e] = g.bias[min(n + e, g.n - 1)];
+                        for (int e = 0; e < N; ++e) bias[e] = g.bias[min(n + e, g.n - 1)];
+                    }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int m = tile.m0 + wm + 16 * i + r;
-                T* c = (T*)g.c + (int64_t)m * g.ldc + n;
-                Pack<T, N> v;
+                for (int i = 0; i < MT; ++i) {
+                    const int m = tile.m0 + wm + 16 * i + r;
+                    T* c = (T*)g.c + (int64_t)m * g.ldc + n;
+                    Pack<T, N> v;
 #pragma unroll
-                for (int e = 0; e < N; ++e) v.v[e] = from_f32<T>(acc[i][q * JJ + e / 4][e % 4] + bias[e]);
-                if (whole || (m < g.m && n + N <= g.n)) {
-                    Bits bits;
-                    __builtin_memcpy(&bits, &v, 16);
-                    __builtin_nontemporal_store(bits, (Bits*)c);
-                } else if (m < g.m) {
+                    for (int e = 0; e < N; ++e) v.v[e] = from_f32<T>(acc[i][q * JJ + e / 4][e % 4] + bias[e]);
+                    if (whole || (m < g.m && n + N <= g.n)) {
+                        Bits bits;
+                        __builtin_memcpy(&bits, &v, 16);
+                        __builtin_nontemporal_store(bits, (Bits*)c);
+                    } else if (m < g.m) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (n + e < g.n) c[e] = v.v[e];
+                        for (int e = 0; e < N; ++e)
+                            if (n + e < g.n) c[e] = v.v[e];
+                    }
                 }
             }
         }

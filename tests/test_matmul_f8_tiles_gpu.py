@@ -94,3 +94,44 @@ def test_a_tile_leaves_nothing_to_the_next(lib, dtype, m, n, k, scale):  # noqa:
         assert not np.isfinite(got[:, block * 128:(block + 1) * 128]).any()
         rest = np.r_[0:block * 128, min((block + 1) * 128, n):n]
         assert np.array_equal(got[:, rest], clean[:, rest]), "W"
+
+
+@pytest.mark.parametrize("dtype,m,n,k", [next(c for c, w in zip(SIZES, WAYS) if w[0] == f32 and w[4] == way) for f32, way in sorted({(w[0], w[4]) for w in WAYS})])
+def test_scales_whose_product_leaves_the_range(lib, dtype, m, n, k):  # noqa: F811
+    """Scales of 2^70 and 2^-62 (times ordinary ones), whose products fp32 holds no longer or with few
+    bits, where their products with the sums are ordinary numbers: 0, sums of the smallest codes, sums of large ones.
+    What has ordinary scales has the same bits as without them."""
+    (a, sa, w, sw), bias = _operands(m, n, k, 5, True)
+    clean = _stored((a, sa, w, sw), n, k, bias, dtype, 1, 0)
+    a, sa, w, sw = a.copy(), sa.copy(), w.copy(), sw.copy()
+    r = np.random.default_rng(n)
+    few = lambda shape: np.where(r.random(shape) < 0.02, r.choice(np.array([1, 2, 3, 129], np.uint8), shape), 0).astype(np.uint8)  # noqa: E731
+    high, low = np.unique(np.r_[0, r.integers(0, m, 9)]), np.unique(np.r_[m // 2, m - 1, r.integers(0, m, 9)])
+    low = np.setdiff1d(low, high)
+    a[high, :k], sa[high] = few((len(high), k)), sa[high] * np.float32(2.0**70)
+    sa[low] *= np.float32(2.0**-62)
+    w[128:256, :k], sw[1] = few((128, k)), sw[1] * np.float32(2.0**70)
+    blocks = np.unique([2, n // 128])
+    sw[blocks] *= np.float32(2.0**-62)
+    changed = np.unique(np.r_[high, low])
+    ordinary_rows = np.setdiff1d(np.arange(m), changed)
+    ordinary = np.ones(n, bool)
+    ordinary[128:256] = False
+    for b in blocks:
+        ordinary[b * 128:(b + 1) * 128] = False
+    zero = np.zeros(n, np.float32)
+    for bias in (bias, zero):
+        got = _stored((a, sa, w, sw), n, k, bias, dtype, 1, 0)
+        want, bound = q.matmul(a[changed], sa[changed], w, sw, bias, fp32=dtype == s.F32)
+        if dtype == s.F16:  # beyond its range the results are infinite, and near its end they may be
+            near = np.abs(np.abs(want) - 65520) <= bound
+            values = np.where(near, 0, s.load(got[changed], dtype))
+            over = (np.abs(want) > 65520) & ~near
+            assert np.array_equal(values[over], np.copysign(np.inf, want[over]))
+            keep = ~over & ~near
+            _close(values[keep], want[keep], bound[keep], dtype, "C")
+        else:
+            _close(s.load(got[changed], dtype), want, bound, dtype, "C")
+        if bias is not zero:
+            at = np.ix_(ordinary_rows, ordinary)
+            assert np.array_equal(got[at], clean[at])
