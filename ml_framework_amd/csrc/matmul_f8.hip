@@ -609,9 +609,15 @@ int launch_tiles(const MatmulF8& g, hipStream_t st) {
 template <class T>
 int launch_t(const MatmulF8& g, hipStream_t st) {
     constexpr bool F32 = sizeof(T) == 4;
+    if (!g.blocks) {
+        // the bias alone: slices of zeros, for which nothing is read, at any size. (Operands may be null then)
+        MatmulF8 zeros = g;
+        zeros.a = zeros.w = (const uint8_t*)g.c, zeros.a_scales = zeros.w_scales = (const float*)g.c;
+        return launch_tiles<T, 128, 128, 2, 2, 3>(zeros, st);
+    }
     // offsets inside a tile are 31 bits
     const bool short_rows = (int64_t)256 * g.blocks * kF8Block < kMaxTileSpanBytes;
-    switch (g.blocks && short_rows ? f8_way(F32, g.m, g.n, g.blocks, device_cus()) : kSplit) {
+    switch (short_rows ? f8_way(F32, g.m, g.n, g.blocks, device_cus()) : kSplit) {
         case kStream16x64: return launch_stream<T, 16, 64, 5>(g, st);
         case kStream32x32: return launch_stream<T, 32, 32, 8>(g, st);
         case kStream32x64: return launch_stream<T, 32, 64, 5>(g, st);

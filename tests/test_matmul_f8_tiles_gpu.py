@@ -135,3 +135,19 @@ def test_scales_whose_product_leaves_the_range(lib, dtype, m, n, k):  # noqa: F8
         if bias is not zero:
             at = np.ix_(ordinary_rows, ordinary)
             assert np.array_equal(got[at], clean[at])
+
+
+@pytest.mark.parametrize("m,n", [(66000, 33000), (1, (1 << 27) + 5)])
+def test_no_k_of_any_size(lib, m, n):  # noqa: F811
+    """K == 0 gives the bias at sizes beyond 2^31 results, and of rows beyond 2^27."""
+    bias = np.random.default_rng(n).integers(-128, 129, n).astype(np.float32)
+    want = s.store(bias, s.BF16)
+    b, c = Bytes((n,), np.float32, bias), capi.DeviceBuffer(m * n * 2)
+    capi.call("seera_hip_matmul_f8", None, None, None, None, b.ptr, c.ptr, m, n, 0, n, s.BF16)
+    for i in sorted({0, 1, 127, 128, m // 2, m - 1} & set(range(m))):
+        row = np.empty(n, np.uint16)
+        capi.check(lib.seera_hip_memcpy_d2h(row.ctypes.data, c.ptr + i * n * 2, row.nbytes))
+        assert np.array_equal(row, want), i
+    c.close()
+    b.buf.close()
+    capi.check(lib.seera_hip_empty_cache())
