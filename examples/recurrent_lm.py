@@ -14,7 +14,8 @@ Each block is
 and the step is cuda_adamw_step over all tensors: the products' weights with
 8-bit states, the norms' with 32-bit ones.
 
-The trained model then answers in 8 bits, on the GPU from one token to the next:
+The trained model then answers in 8 bits. From a token's row of the embedding, which
+the host picks, to the next token nothing else passes through the host:
 
     weights     cuda_quantize_weights_f8, once
     n           cuda_block_norm_fwd_f8: the same norms, their output in 8 bits

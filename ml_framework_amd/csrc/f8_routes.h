@@ -11,7 +11,9 @@ namespace seera {
 // The ways to compute a product: tiles of rows x cols, `at_once` workgroups a compute unit. A
 // launch takes `start` us (3.3 of them an empty one) and, for each slice of 128 along K, `few` where most
 // compute units have nothing to do, `full` where each has its workgroup, `pair` where each has two. Fitted
-// to times of 16 to 8192 rows with every way at K = 1024, 4096 and 16384 (bf16; fp32 below).
+// to times of each way at 16 to 512 rows with K = 1024, 4096 and 16384 (bf16; fp32 below: 32 to 777 rows, K = 1024 and
+// 4096). Of the chosen way's times at 1024 to 8192 rows it was within 15 % (bf16), and 25 % too low at fp32
+// 5501 x 1300 x 1500; memory's rate is not in it (64 x 131072 x 4096 takes 138 us, not 66).
 enum F8Way { kSplit, kStream16x64, kStream32x32, kStream32x64, kStream64x64, kTiles128, kTiles128x256, kTiles256, kF8Ways };
 struct F8Cost {
     int rows, cols, at_once;

@@ -9,13 +9,14 @@
 // 16 g .. 16 g + 15 hold its 16-byte pieces g and g + 4), which changes no sum of products.
 //
 // 16-bit results take v_mfma_f32_16x16x128_f8f6f4. It cuts each product below 2^-13 of
-// the largest of its group of 8 along K (measured; towards zero), and adds in fp32 from there:
-// 1.4e-5 of the result, where rounding it to 16 bits is 1.7e-3 or 2e-4. An fp32 result
+// the largest of its group of 8 along K (measured; towards zero), and adds in fp32 from there: less than
+// 7 * 2^-13 of the sum of the groups' largest products, and 1.4e-5 of the results of random operands, where
+// rounding them to 16 bits is 1.7e-3 or 2e-4. An fp32 result
 // is held to fp32's roundings: its codes are widened to fp16, which holds each of them,
 // and multiplied by v_mfma_f32_16x16x32_f16, at half the rate (2e-8 of the result).
 //
-// bf16 results, us: 1 x 4096 x 4096 5.4 (codes of W at a copy's 5 TB/s 3.4, an empty launch
-// 3.3), 64 x 12288 x 4096 15.8 (10 + 3.3), 8192 x 12288 x 4096 344 to 359: 2.3 PFLOP/s, where
+// bf16 results, us: 1 x 4096 x 4096 5.5 (codes of W at a copy's 5 TB/s 3.4, an empty launch
+// 3.3), 64 x 12288 x 4096 15.4 (10 + 3.3), 8192 x 12288 x 4096 342 to 364: 2.3 PFLOP/s, where
 // a product without scales reaches 3.1. The last is bound by power: the clock falls to 1.65 GHz with
 // the matrix cores busy for 0.74 of it. Instructions of 32 x 32 x 64 are no faster (3.9 against
 // 4.3 PFLOP/s from registers alone); stores, DMA or scaling left out gave 5 % each.
@@ -164,7 +165,8 @@ __device__ __forceinline__ void results_again(const MatmulF8& g, int m0, int n0)
 
 // A tile of 16 x 16, with the blocks along K dealt to eight waves, whose sums are joined
 // in the waves' order. All of a wave's loads for K up to 4096 are in flight at once: 1 x 4096 x
-// 4096 in 4.4 us, of which an empty launch is 3.3 (loads a ring of registers ahead: 4.6; 16 waves: 4.7).
+// 4096 in 5.5 us, and 4.4 with W in the caches from the call before, of which an empty launch is 3.3 (the latter
+// with loads a ring of registers ahead: 4.6; 16 waves: 4.7).
 constexpr int kSplitWaves = 8;
 template <class T>
 __global__ __launch_bounds__(64 * kSplitWaves) void matmul_f8_split(MatmulF8 g) {
